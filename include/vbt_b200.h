@@ -479,6 +479,137 @@ VBT_B200_API vbt_b200_status vbt_b200_rmsnorm_backward(void* dx, float* dgamma, 
                                           void* stream);
 
 /* =====================================================================================
+ * 4b. Around a transformer block's matrix products (no counterpart on the reference's path)
+ *    Row ops like the ones above: rows of `cols` values with column stride 1 and any row
+ *    stride, dense outputs, F32 / BF16 / F16 storage, FP32 math, gammas F32 [cols] or NULL
+ *    (all ones).  Scratch comes from the caller; nothing is kept between calls.
+ * ===================================================================================== */
+/* The join of a branch with the residual stream, between the norm behind the branch and the norm
+ * in front of the next block:
+ *   v = y * inv_post * gamma_post,  inv_post = rsqrt(mean(y^2) + eps)    (v = y without POST)
+ *   r = residual_scale * x + branch_scale * gate * v
+ *   n = r * inv_pre * gamma_pre,    inv_pre = rsqrt(mean(r^2) + eps)     (only with PRE; from the
+ *                                                                        unrounded r)
+ * gate: storage dtype or NULL (ones); row i uses gate row i / rows_per_gate, so one row serves all
+ * (rows_per_gate = rows), a sample's rows, or one row (rows_per_gate = 1).  inv_post / inv_pre: F32
+ * [rows], may be NULL.  Outputs must not overlap inputs. */
+#define VBT_B200_RESNORM_POST 1
+#define VBT_B200_RESNORM_PRE 2
+VBT_B200_API vbt_b200_status vbt_b200_residual_norm(void* r, void* n, float* inv_post, float* inv_pre, const void* x,
+                                       const void* y, const float* gamma_post, const void* gate,
+                                       const float* gamma_pre, int32_t dtype, int64_t rows, int64_t cols,
+                                       int64_t x_row_stride, int64_t y_row_stride, int64_t gate_row_stride,
+                                       int64_t rows_per_gate, float residual_scale, float branch_scale,
+                                       float eps, int32_t flags, void* stream);
+/* Its backward.  With G the gradient that arrives at r,
+ *   G  = dr + inv_pre * dn * gamma_pre - r * inv_pre^3 * mean(dn * gamma_pre * r)
+ *   dx = residual_scale * G;  dgamma_pre = sum over rows of dn * r * inv_pre
+ *   dgate = branch_scale * G * v, summed over the rows that share a gate row
+ *   dv = branch_scale * G * gate;  dgamma_post = sum over rows of dv * y * inv_post
+ *   dy = inv_post * dv * gamma_post - y * inv_post^3 * mean(dv * gamma_post * y)   (dv without POST)
+ * dr may be NULL (no gradient from the stream), dn / r / inv_pre are needed with PRE, y with POST or
+ * when dgate is wanted, inv_post with POST.  dgate: storage dtype, dense [rows / rows_per_gate, cols];
+ * dgamma_*: F32 [cols]; each may be NULL to skip it.  Sums over rows are FP32 in a fixed order
+ * (per-block partial rows in `workspace`, folded by a second launch): reproducible run to run. */
+VBT_B200_API vbt_b200_status vbt_b200_residual_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int32_t dtype,
+                                                                int64_t rows_per_gate, int32_t device,
+                                                                size_t* bytes);
+VBT_B200_API vbt_b200_status vbt_b200_residual_norm_backward(
+    void* dx, void* dy, float* dgamma_post, void* dgate, float* dgamma_pre, const void* dr, const void* dn,
+    const void* y, const void* r, const float* inv_post, const float* inv_pre, const float* gamma_post,
+    const void* gate, const float* gamma_pre, int32_t dtype, int64_t rows, int64_t cols, int64_t dr_row_stride,
+    int64_t dn_row_stride, int64_t y_row_stride, int64_t r_row_stride, int64_t gate_row_stride,
+    int64_t rows_per_gate, float residual_scale, float branch_scale, int32_t flags, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/* Activations kept in 8 bits for the backward pass.  A row is cut into groups of VBT_B200_Q8_GROUP
+ * values (the last one may be shorter); a group is held as 8-bit levels and one F32 scale:
+ *   amax = max |x|;  scale = amax * fl(1/top);  q = rn(fl(x * fl(top / amax)));  x' = q * scale
+ * with top = 127 (INT8) or 448 (E4M3); amax < 2^-119 gives zeros.  A group with a NaN or an infinity
+ * reads back as NaN throughout.  q: one byte per value, dense [rows, cols]; scale: F32, dense
+ * [rows, ceil(cols / VBT_B200_Q8_GROUP)]. */
+#define VBT_B200_Q8_INT8 0
+#define VBT_B200_Q8_E4M3 1
+#define VBT_B200_Q8_GROUP 128
+VBT_B200_API vbt_b200_status vbt_b200_checkpoint8(void* q, float* scale, const void* x, int32_t dtype, int32_t format,
+                                     int64_t rows, int64_t cols, int64_t x_row_stride, void* stream);
+VBT_B200_API vbt_b200_status vbt_b200_checkpoint8_restore(void* out, const void* q, const float* scale, int32_t dtype,
+                                             int32_t format, int64_t rows, int64_t cols, void* stream);
+/* rmsnorm and the 8-bit copy of its input from one read of x. */
+VBT_B200_API vbt_b200_status vbt_b200_rmsnorm_checkpoint8(void* out, float* inv_rms, void* q, float* scale, const void* x,
+                                             const float* gamma, int32_t dtype, int32_t format, int64_t rows,
+                                             int64_t cols, int64_t x_row_stride, float eps, void* stream);
+/* rmsnorm_backward with x read from its 8-bit copy (same formulas, same kind of workspace). */
+VBT_B200_API vbt_b200_status vbt_b200_rmsnorm_backward8_workspace_bytes(int64_t rows, int64_t cols, int32_t dtype,
+                                                           int32_t device, size_t* bytes);
+VBT_B200_API vbt_b200_status vbt_b200_rmsnorm_backward8(void* dx, float* dgamma, const void* dy, const void* q,
+                                           const float* scale, const float* inv_rms, const float* gamma,
+                                           int32_t dtype, int32_t format, int64_t rows, int64_t cols,
+                                           int64_t dy_row_stride, void* workspace, size_t workspace_bytes,
+                                           void* stream);
+/* The gated activation h = silu(gate) * up, silu(g) = g / (1 + exp(-g)), with the 8-bit copies of
+ * both factors when q_gate is not NULL (then q_up, scale_gate and scale_up are needed too). */
+VBT_B200_API vbt_b200_status vbt_b200_silu_mul(void* out, void* q_gate, float* scale_gate, void* q_up, float* scale_up,
+                                  const void* gate, const void* up, int32_t dtype, int32_t format, int64_t rows,
+                                  int64_t cols, int64_t gate_row_stride, int64_t up_row_stride, void* stream);
+/* dgate = dout * up * silu'(gate), dup = dout * silu(gate).  gate and up are storage-dtype rows
+ * (scale_gate and scale_up NULL) or dense 8-bit copies (row strides ignored). */
+VBT_B200_API vbt_b200_status vbt_b200_silu_mul_backward(void* dgate, void* dup, const void* dout, const void* gate,
+                                           const float* scale_gate, const void* up, const float* scale_up,
+                                           int32_t dtype, int32_t format, int64_t rows, int64_t cols,
+                                           int64_t dout_row_stride, int64_t gate_row_stride,
+                                           int64_t up_row_stride, void* stream);
+
+/* Rotary positions with up to VBT_B200_ROTARY_MAX_AXES axes, queries and keys in one launch.  Pair i
+ * of a head (i < half) turns by positions[axis(i), b, t] * inv_freq[i]; axis(i) is the section of
+ * `sections` (naxes counts that sum to half) that i falls into.  A pair is (i, half + i), or
+ * (2i, 2i + 1) with interleaved != 0; values behind 2 * half are copied.
+ *   a' = a cos - b sin,  b' = b cos + a sin;  inverse != 0 turns back, which is the backward pass.
+ * The angle is formed in 64 bits and reduced to a part of a turn there, so positions far into a long
+ * sequence lose nothing.  q and k: [batch, tokens, heads, dim], last stride 1, other strides (in
+ * elements) given as {batch, token, head}; q_out, k_out likewise (an output may be its own input).
+ * k may be NULL.  positions: I64, I32 or F32 with strides {axis, batch, token}; inv_freq: F32 [half].
+ * The stride and section arrays are host memory, read before the call returns. */
+#define VBT_B200_ROTARY_MAX_AXES 4
+VBT_B200_API vbt_b200_status vbt_b200_rotary(void* q_out, const int64_t* q_out_strides, const void* q,
+                                const int64_t* q_strides, int64_t q_heads, void* k_out,
+                                const int64_t* k_out_strides, const void* k, const int64_t* k_strides,
+                                int64_t k_heads, int32_t dtype, int64_t batch, int64_t tokens, int64_t dim,
+                                const void* positions, int32_t positions_dtype,
+                                const int64_t* positions_strides, const float* inv_freq, int64_t half,
+                                const int64_t* sections, int32_t naxes, int32_t interleaved, int32_t inverse,
+                                void* stream);
+
+/* A paged key/value cache in 8 bits (the format above, one scale per slot and head).  k_cache and
+ * v_cache: dense [num_slots, heads, dim] bytes, num_slots = pages * page_size; k_scale, v_scale: F32
+ * dense [num_slots, heads].
+ * write: token i of k and v ([tokens, heads, dim], last stride 1, strides {token, head}) goes to slot
+ * slots[i] (I64 or I32).  A negative slot skips the token; a slot >= num_slots is skipped and counted in
+ * `index_status` (as in section 3; may be NULL).  Of several tokens with one slot the LAST is kept, whole, with
+ * its scales: `owner` (I32 [num_slots], zeroed once when the cache is made) is where they settle it, and
+ * every call leaves it zero again.  Calls that write the same slot must not overlap on the GPU; others
+ * may. */
+VBT_B200_API vbt_b200_status vbt_b200_kv_cache_write(void* k_cache, float* k_scale, void* v_cache, float* v_scale,
+                                        int64_t num_slots, int64_t heads, int64_t dim, int32_t format,
+                                        const void* k, const int64_t* k_strides, const void* v,
+                                        const int64_t* v_strides, int32_t dtype, const void* slots,
+                                        int32_t slots_dtype, int64_t tokens, int32_t* owner, void* index_status,
+                                        void* stream);
+/* read: output row i in [starts[0], starts[seqs]) and below `rows` belongs to the sequence s with
+ * starts[s] <= i < starts[s + 1] and receives the slot page_table[s, p / page_size] * page_size +
+ * p % page_size, p = i - starts[s].  starts: I64 [seqs + 1], ascending (device).  page_table: I64 or I32
+ * [seqs, pages_per_seq] with a row stride.  Rows outside every sequence are left as they are, or set
+ * to zero with fill != 0.  A page outside [0, num_slots / page_size), or a position behind the table's
+ * last page, reads as zeros and is counted in `index_status`.  k_out, v_out: dense [rows, heads, dim]. */
+VBT_B200_API vbt_b200_status vbt_b200_kv_cache_read(void* k_out, void* v_out, int32_t dtype, int64_t rows,
+                                       const void* k_cache, const float* k_scale, const void* v_cache,
+                                       const float* v_scale, int64_t num_slots, int64_t page_size,
+                                       int64_t heads, int64_t dim, int32_t format, const void* page_table,
+                                       int32_t page_table_dtype, int64_t page_table_stride,
+                                       int64_t pages_per_seq, const int64_t* starts, int64_t seqs, int32_t fill,
+                                       void* index_status, void* stream);
+
+/* =====================================================================================
  * 5. Fabric: sharded reductions and elementwise on a row-sharded tensor
  *    sits behind FabricTensor.sharded_1d_row (python/vibetensor/fabric.py:483-533) and
  *    replaces fabric_binary_kernel (src/vbt/cuda/fabric_elementwise.cu:122-162).
@@ -607,12 +738,20 @@ VBT_B200_API vbt_b200_status vbt_b200_scale_cast(void* out, int32_t out_dtype, c
 #define VBT_B200_IK_MASK_SELECT 8
 #define VBT_B200_IK_LASTDIM_WIDE 9    /* 4-byte rows of up to 65 536 elements: outputs in registers,
                                          all shared memory for the row; `splits` = pieces   */
+#define VBT_B200_IK_KV_CACHE_WRITE 10
+#define VBT_B200_IK_KV_CACHE_READ 11
 /* ROWOP: */
 #define VBT_B200_WK_GROUP 1
 #define VBT_B200_WK_BLOCK 2
 #define VBT_B200_WK_STREAM 3
 #define VBT_B200_WK_BACKWARD 4
 #define VBT_B200_WK_SCALE_CAST 5
+#define VBT_B200_WK_RESIDUAL_NORM 6
+#define VBT_B200_WK_RESIDUAL_NORM_BACKWARD 7
+#define VBT_B200_WK_CHECKPOINT8 8     /* checkpoint8, its restore and rmsnorm_checkpoint8            */
+#define VBT_B200_WK_RMSNORM_BACKWARD8 9
+#define VBT_B200_WK_SILU_MUL 10       /* both directions                                             */
+#define VBT_B200_WK_ROTARY 11
 /* FABRIC: */
 #define VBT_B200_FK_PEER_LOAD 1      /* the elementwise kernel reads the peer operand over NVLink */
 #define VBT_B200_FK_COPY_FALLBACK 2  /* peer operand copied to local scratch first           */

@@ -22,6 +22,8 @@ _TORCH_TO_CODE = {
     torch.complex64: C64, torch.complex128: C128,
 }
 MAX_NDIM = 25
+Q8_GROUP = 128
+Q8_FORMATS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 FABRIC_HANDLE_BYTES = 128
 
 
@@ -42,6 +44,7 @@ _P = ctypes.POINTER(VbtTensor)
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
+_f32 = ctypes.c_float
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
@@ -88,6 +91,24 @@ SIGNATURES = {
     "vbt_b200_rmsnorm_backward_workspace_bytes": (_i32, [_i64, _i64, _i32, _i32, ctypes.POINTER(ctypes.c_size_t)]),
     "vbt_b200_rmsnorm_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp,
                                          ctypes.c_size_t, _vp]),
+    "vbt_b200_residual_norm": (_i32, [_vp] * 9 + [_i32] + [_i64] * 6 + [_f32] * 3 + [_i32, _vp]),
+    "vbt_b200_residual_norm_backward_workspace_bytes": (_i32, [_i64, _i64, _i32, _i64, _i32,
+                                                               ctypes.POINTER(ctypes.c_size_t)]),
+    "vbt_b200_residual_norm_backward": (_i32, [_vp] * 14 + [_i32] + [_i64] * 8 + [_f32] * 2 +
+                                        [_i32, _vp, ctypes.c_size_t, _vp]),
+    "vbt_b200_checkpoint8": (_i32, [_vp] * 3 + [_i32] * 2 + [_i64] * 3 + [_vp]),
+    "vbt_b200_checkpoint8_restore": (_i32, [_vp] * 3 + [_i32] * 2 + [_i64] * 2 + [_vp]),
+    "vbt_b200_rmsnorm_checkpoint8": (_i32, [_vp] * 6 + [_i32] * 2 + [_i64] * 3 + [_f32, _vp]),
+    "vbt_b200_rmsnorm_backward8_workspace_bytes": (_i32, [_i64, _i64, _i32, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "vbt_b200_rmsnorm_backward8": (_i32, [_vp] * 7 + [_i32] * 2 + [_i64] * 3 + [_vp, ctypes.c_size_t, _vp]),
+    "vbt_b200_silu_mul": (_i32, [_vp] * 7 + [_i32] * 2 + [_i64] * 4 + [_vp]),
+    "vbt_b200_silu_mul_backward": (_i32, [_vp] * 7 + [_i32] * 2 + [_i64] * 5 + [_vp]),
+    "vbt_b200_rotary": (_i32, [_vp, _i64p, _vp, _i64p, _i64] * 2 + [_i32] + [_i64] * 3 + [_vp, _i32, _i64p, _vp, _i64,
+                               _i64p, _i32, _i32, _i32, _vp]),
+    "vbt_b200_kv_cache_write": (_i32, [_vp] * 4 + [_i64] * 3 + [_i32] + [_vp, _i64p] * 2 +
+                                [_i32, _vp, _i32, _i64, _vp, _vp, _vp]),
+    "vbt_b200_kv_cache_read": (_i32, [_vp] * 2 + [_i32, _i64] + [_vp] * 4 + [_i64] * 4 + [_i32, _vp, _i32] + [_i64] * 2 +
+                               [_vp, _i64, _i32, _vp, _vp]),
     "vbt_b200_enable_peer_access": (_i32, [_i32, _i32]),
     "vbt_b200_reduce_partial": (_i32, [_i32, _P, _P, _i64p, _i32, _i32, _vp, ctypes.c_size_t, _i32, _vp]),
     "vbt_b200_scale_cast": (_i32, [_vp, _i32, _vp, _i64, ctypes.c_float, _vp]),

@@ -1,0 +1,796 @@
+// Activations kept in 8 bits for the backward pass, and the passes that make and use them (sm_100a):
+//
+//   checkpoint8            x -> (q, scale), groups of 128 values with a scale of their own
+//   checkpoint8_restore    (q, scale) -> x'
+//   rmsnorm_checkpoint8    RMSNorm and the 8-bit copy of its input from one read of x
+//   rmsnorm_backward8      the backward of RMSNorm with x' in the place of x:
+//                            n = x' r;  dx = r (dy g - n mean(dy g n));  dg = sum_rows dy n
+//   silu_mul               h = silu(gate) * up, with the 8-bit copies of both factors on request
+//   silu_mul_backward      dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, s = sigmoid(gate)
+//
+// All are bound by memory: every operand is touched once.  The lanes that hold one group are
+// neighbours (16 lanes of 8 values for 16-bit types, 32 of 4 otherwise), so a group's largest
+// magnitude is a few shuffles and nothing goes through shared memory.
+#include <algorithm>
+
+#include "quant8.cuh"
+#include "row_tile.cuh"
+
+namespace vb {
+namespace {
+
+// How a group of up to 128 neighbouring values lies in the lanes of a warp.  VEC: 16-byte vectors
+// (needs rows of whole vectors, 16-byte aligned); else 32 lanes with the values lane, lane + 32, ...
+template <class T, bool VEC> struct Lanes {
+  static constexpr int V = VEC ? 16 / sizeof(T) : 1;
+  static constexpr int L = VEC ? kQ8Group / V : 32;
+  static constexpr int N = kQ8Group / L;  // values per lane
+  using Raw = Vec<T, N>;
+  using Q = typename Q8Raw<N>::type;
+
+  static __device__ __forceinline__ Raw load(const T* group, int lane, int len) {
+    Raw r;
+    if constexpr (VEC) {
+      if (lane * V < len) return *reinterpret_cast<const Raw*>(group + lane * V);
+#pragma unroll
+      for (int e = 0; e < N; ++e) r.v[e] = from_f<T>(0.f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) r.v[e] = lane + 32 * e < len ? group[lane + 32 * e] : from_f<T>(0.f);
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void store(T* group, int lane, int len, const float (&v)[N]) {
+    if constexpr (VEC) {
+      if (lane * V >= len) return;
+      Raw r;
+#pragma unroll
+      for (int e = 0; e < N; ++e) r.v[e] = from_f<T>(v[e]);
+      *reinterpret_cast<Raw*>(group + lane * V) = r;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (lane + 32 * e < len) group[lane + 32 * e] = from_f<T>(v[e]);
+    }
+  }
+  static __device__ __forceinline__ Q load_q(const uint8_t* group, int lane, int len) {
+    if constexpr (VEC) {
+      Q q{};
+      if (lane * V < len) q = *reinterpret_cast<const Q*>(group + lane * V);
+      return q;
+    } else {
+      uint32_t q = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (lane + 32 * e < len) q |= static_cast<uint32_t>(group[lane + 32 * e]) << (8 * e);
+      return q;
+    }
+  }
+  // quantises the group: returns its stored scale
+  template <int F>
+  static __device__ __forceinline__ float store_q(uint8_t* group, int lane, int len, const float (&v)[N]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) m = max(m, mag_bits(v[e]));
+    const Q8Scale s = q8_scale<F>(lanes_max<L>(m));
+    if constexpr (VEC) {
+      if (lane * V < len) q8_store<F, N>(group + lane * V, v, s.up);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (lane + 32 * e < len) group[lane + 32 * e] = q8_pack1<F>(v[e], s.up);
+    }
+    return s.down;
+  }
+};
+
+// the groups of [rows, cols] in order: group i is group `g` of row `row`
+struct Groups {
+  int64_t total, per_row, cols;
+  FastDiv div;
+  int small;
+  void fill(int64_t rows, int64_t c) {
+    cols = c;
+    per_row = (c + kQ8Group - 1) / kQ8Group;
+    total = rows * per_row;
+    small = total < (int64_t{1} << 31);
+    if (small) div = FastDiv(static_cast<uint32_t>(per_row));
+  }
+  __device__ __forceinline__ void find(int64_t i, int64_t& row, int64_t& col, int& len) const {
+    int64_t g;
+    if (small) {
+      uint32_t q, r;
+      div.divmod(static_cast<uint32_t>(i), q, r);
+      row = q; g = r;
+    } else {
+      row = i / per_row; g = i - row * per_row;
+    }
+    col = g * kQ8Group;
+    len = static_cast<int>(min(int64_t{kQ8Group}, cols - col));
+  }
+};
+
+struct CkParams {
+  const void* x;
+  void* out;
+  uint8_t* q;
+  float* scale;
+  int64_t x_stride;
+  Groups g;
+};
+
+constexpr int kCkThreads = 256;
+
+template <class T, bool VEC, int F, int U>
+__global__ void __launch_bounds__(kCkThreads) checkpoint8_kernel(const __grid_constant__ CkParams p) {
+  using A = Lanes<T, VEC>;
+  constexpr int S = kCkThreads / A::L;
+  const int lane = threadIdx.x % A::L;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
+  typename A::Raw x[U];
+  int64_t row[U], col[U];
+  int len[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = first + u * S;
+    len[u] = 0; row[u] = col[u] = 0;
+    if (i < p.g.total) p.g.find(i, row[u], col[u], len[u]);
+    x[u] = A::load(static_cast<const T*>(p.x) + row[u] * p.x_stride + col[u], lane, len[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[A::N];
+#pragma unroll
+    for (int e = 0; e < A::N; ++e) v[e] = to_f(x[u].v[e]);
+    const float s = A::template store_q<F>(p.q + row[u] * p.g.cols + col[u], lane, len[u], v);
+    if (lane == 0 && len[u]) p.scale[first + u * S] = s;
+  }
+}
+
+template <class T, bool VEC, int F, int U>
+__global__ void __launch_bounds__(kCkThreads) restore8_kernel(const __grid_constant__ CkParams p) {
+  using A = Lanes<T, VEC>;
+  constexpr int S = kCkThreads / A::L;
+  const int lane = threadIdx.x % A::L;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
+  typename A::Q q[U];
+  float s[U];
+  int64_t row[U], col[U];
+  int len[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = first + u * S;
+    len[u] = 0; row[u] = col[u] = 0; s[u] = 0.f;
+    if (i < p.g.total) {
+      p.g.find(i, row[u], col[u], len[u]);
+      s[u] = __ldg(p.scale + i);
+    }
+    q[u] = A::load_q(p.q + row[u] * p.g.cols + col[u], lane, len[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[A::N];
+    q8_widen<F, A::N>(q[u], s[u], v);
+    A::store(static_cast<T*>(p.out) + row[u] * p.g.cols + col[u], lane, len[u], v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// gated activation
+// ---------------------------------------------------------------------------------------
+struct GluParams {
+  const void* dout;    // backward
+  const void* gate;    // storage type, or levels
+  const void* up;
+  const float* gate_scale;
+  const float* up_scale;
+  void* out;           // forward
+  void* dgate;
+  void* dup;
+  uint8_t* q_gate;
+  uint8_t* q_up;
+  float* s_gate;
+  float* s_up;
+  int64_t dout_stride, gate_stride, up_stride;
+  Groups g;
+};
+
+// KEEP: also writes the 8-bit copies
+template <class T, bool VEC, int F, bool KEEP, int U>
+__global__ void __launch_bounds__(kCkThreads) silu_mul_kernel(const __grid_constant__ GluParams p) {
+  using A = Lanes<T, VEC>;
+  constexpr int S = kCkThreads / A::L;
+  const int lane = threadIdx.x % A::L;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
+  typename A::Raw ga[U], up[U];
+  int64_t row[U], col[U];
+  int len[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = first + u * S;
+    len[u] = 0; row[u] = col[u] = 0;
+    if (i < p.g.total) p.g.find(i, row[u], col[u], len[u]);
+    ga[u] = A::load(static_cast<const T*>(p.gate) + row[u] * p.gate_stride + col[u], lane, len[u]);
+    up[u] = A::load(static_cast<const T*>(p.up) + row[u] * p.up_stride + col[u], lane, len[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float a[A::N], b[A::N], h[A::N];
+#pragma unroll
+    for (int e = 0; e < A::N; ++e) {
+      a[e] = to_f(ga[u].v[e]);
+      b[e] = to_f(up[u].v[e]);
+      h[e] = a[e] / (1.f + expf(-a[e])) * b[e];
+    }
+    const int64_t at = row[u] * p.g.cols + col[u];
+    A::store(static_cast<T*>(p.out) + at, lane, len[u], h);
+    if constexpr (KEEP) {
+      const float sa = A::template store_q<F>(p.q_gate + at, lane, len[u], a);
+      const float sb = A::template store_q<F>(p.q_up + at, lane, len[u], b);
+      if (lane == 0 && len[u]) {
+        p.s_gate[first + u * S] = sa;
+        p.s_up[first + u * S] = sb;
+      }
+    }
+  }
+}
+
+// KEPT: gate and up come from their 8-bit copies
+template <class T, bool VEC, int F, bool KEPT, int U>
+__global__ void __launch_bounds__(kCkThreads) silu_mul_bwd_kernel(const __grid_constant__ GluParams p) {
+  using A = Lanes<T, VEC>;
+  constexpr int S = kCkThreads / A::L;
+  const int lane = threadIdx.x % A::L;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
+  typename A::Raw d[U], ga[U], up[U];
+  typename A::Q qa[U], qb[U];
+  float sa[U], sb[U];
+  int64_t row[U], col[U];
+  int len[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = first + u * S;
+    len[u] = 0; row[u] = col[u] = 0; sa[u] = sb[u] = 0.f;
+    if (i < p.g.total) p.g.find(i, row[u], col[u], len[u]);
+    d[u] = A::load(static_cast<const T*>(p.dout) + row[u] * p.dout_stride + col[u], lane, len[u]);
+    if constexpr (KEPT) {
+      const int64_t at = row[u] * p.g.cols + col[u];
+      qa[u] = A::load_q(static_cast<const uint8_t*>(p.gate) + at, lane, len[u]);
+      qb[u] = A::load_q(static_cast<const uint8_t*>(p.up) + at, lane, len[u]);
+      if (len[u]) {
+        sa[u] = __ldg(p.gate_scale + i);
+        sb[u] = __ldg(p.up_scale + i);
+      }
+    } else {
+      ga[u] = A::load(static_cast<const T*>(p.gate) + row[u] * p.gate_stride + col[u], lane, len[u]);
+      up[u] = A::load(static_cast<const T*>(p.up) + row[u] * p.up_stride + col[u], lane, len[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float a[A::N], b[A::N], da[A::N], db[A::N];
+    if constexpr (KEPT) {
+      q8_widen<F, A::N>(qa[u], sa[u], a);
+      q8_widen<F, A::N>(qb[u], sb[u], b);
+    } else {
+#pragma unroll
+      for (int e = 0; e < A::N; ++e) {
+        a[e] = to_f(ga[u].v[e]);
+        b[e] = to_f(up[u].v[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < A::N; ++e) {
+      const float s = 1.f / (1.f + expf(-a[e])), dv = to_f(d[u].v[e]);
+      da[e] = dv * b[e] * s * (1.f + a[e] * (1.f - s));
+      db[e] = dv * a[e] * s;
+    }
+    const int64_t at = row[u] * p.g.cols + col[u];
+    A::store(static_cast<T*>(p.dgate) + at, lane, len[u], da);
+    A::store(static_cast<T*>(p.dup) + at, lane, len[u], db);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// RMSNorm with the 8-bit copy of its input, and its backward from that copy
+// ---------------------------------------------------------------------------------------
+struct Norm8Params {
+  const void* x;       // forward
+  const void* dy;      // backward
+  const float* gamma;
+  void* out;           // forward: the norm; backward: dx
+  uint8_t* q;
+  float* scale;
+  float* inv;
+  float* ws;           // backward: [gridDim.x][cols] partial sums of dgamma, or null
+  int64_t rows, cols, groups;
+  int64_t stride;      // of x or dy
+  float eps;
+};
+
+template <class T, int F, int VPL, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rmsnorm8_kernel(const __grid_constant__ Norm8Params p) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  constexpr int R = THREADS / TPR;
+  constexpr int V = 16 / sizeof(T);
+  constexpr int L = kQ8Group / V;
+  static_assert(TPR % L == 0, "a group's lanes are neighbours");
+  __shared__ float red[2][1][THREADS / 32];
+  RowFold<TPR, 1, THREADS> fold{red};
+  const int rl = threadIdx.x / TPR, tl = threadIdx.x % TPR;
+  const int nvec = static_cast<int>(p.cols / V);
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * R; r0 < p.rows; r0 += static_cast<int64_t>(gridDim.x) * R) {
+    const bool live = r0 + rl < p.rows;
+    const int64_t row = live ? r0 + rl : 0;
+    const int nv = live ? nvec : 0;
+    Vec<T, V> x[VPL];
+    load_vecs<T, V, VPL>(static_cast<const T*>(p.x) + row * p.stride, tl, TPR, nv, x);
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < VPL; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[0] = fmaf(to_f(x[k].v[e]), to_f(x[k].v[e]), s[0]);
+    // the 8-bit copy needs nothing of the row's sum: its shuffles hide the wait for it
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int j = tl + k * TPR;
+      float v[V];
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[e] = to_f(x[k].v[e]);
+        m = max(m, mag_bits(v[e]));
+      }
+      const Q8Scale sc = q8_scale<F>(lanes_max<L>(m));
+      if (j < nv) {
+        q8_store<F, V>(p.q + row * p.cols + static_cast<int64_t>(j) * V, v, sc.up);
+        if (tl % L == 0) p.scale[row * p.groups + j / L] = sc.down;
+      }
+    }
+    fold(s);
+    const float inv = rsqrtf(s[0] / static_cast<float>(p.cols) + p.eps);
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int j = tl + k * TPR;
+      if (j >= nv) continue;
+      float g[V];
+      load_floats<V>(p.gamma, j, nv, g, 1.f);
+      Vec<T, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(to_f(x[k].v[e]) * inv * g[e]);
+      *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.out) + row * p.cols + static_cast<int64_t>(j) * V) = o;
+    }
+    if (live && tl == 0 && p.inv) p.inv[row] = inv;
+  }
+}
+
+// any length and alignment: a block per row, a warp per group
+template <class T, int F>
+__global__ void __launch_bounds__(256) rmsnorm8_stream_kernel(const __grid_constant__ Norm8Params p) {
+  using A = Lanes<T, false>;
+  __shared__ float red[2][1][8];
+  RowFold<256, 1, 256> fold{red};
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(p.x) + row * p.stride;
+    float s[1] = {0.f};
+    for (int64_t g = w; g < p.groups; g += 8) {
+      const int len = static_cast<int>(min(int64_t{kQ8Group}, p.cols - g * kQ8Group));
+      const typename A::Raw raw = A::load(x + g * kQ8Group, lane, len);
+      float v[A::N];
+#pragma unroll
+      for (int e = 0; e < A::N; ++e) {
+        v[e] = to_f(raw.v[e]);
+        s[0] = fmaf(v[e], v[e], s[0]);
+      }
+      const float sc = A::template store_q<F>(p.q + row * p.cols + g * kQ8Group, lane, len, v);
+      if (lane == 0) p.scale[row * p.groups + g] = sc;
+    }
+    fold(s);
+    const float inv = rsqrtf(s[0] / static_cast<float>(p.cols) + p.eps);
+    for (int64_t j = threadIdx.x; j < p.cols; j += 256)
+      static_cast<T*>(p.out)[row * p.cols + j] = from_f<T>(to_f(x[j]) * inv * (p.gamma ? p.gamma[j] : 1.f));
+    if (threadIdx.x == 0 && p.inv) p.inv[row] = inv;
+  }
+}
+
+template <class T, int F, int VPL, int TPR>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_bwd8_kernel(const __grid_constant__ Norm8Params p) {
+  constexpr int THREADS = TPR < 128 ? 128 : TPR;
+  constexpr int R = THREADS / TPR;
+  constexpr int V = 16 / sizeof(T);
+  constexpr int E = V * VPL;
+  __shared__ float red[2][1][THREADS / 32];
+  __shared__ float slots[R > 1 ? E * (THREADS + TPR) : 1];
+  RowFold<TPR, 1, THREADS> fold{red};
+  const int rl = threadIdx.x / TPR, tl = threadIdx.x % TPR;
+  const int nvec = static_cast<int>(p.cols / V);
+  float sum[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = 0.f;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * R; r0 < p.rows; r0 += static_cast<int64_t>(gridDim.x) * R) {
+    const bool live = r0 + rl < p.rows;
+    const int64_t row = live ? r0 + rl : 0;
+    const int nv = live ? nvec : 0;
+    Vec<T, V> dy[VPL];
+    typename Q8Raw<V>::type q[VPL];
+    float sc[VPL];
+    load_vecs<T, V, VPL>(static_cast<const T*>(p.dy) + row * p.stride, tl, TPR, nv, dy);
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int j = tl + k * TPR;
+      q[k] = {};
+      sc[k] = 0.f;
+      if (j < nv) {
+        q[k] = *reinterpret_cast<const typename Q8Raw<V>::type*>(p.q + row * p.cols + static_cast<int64_t>(j) * V);
+        sc[k] = __ldg(p.scale + row * p.groups + j / (kQ8Group / V));
+      }
+    }
+    const float inv = live ? p.inv[row] : 0.f;
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      float x[V], g[V];
+      q8_widen<F, V>(q[k], sc[k], x);
+      load_floats<V>(p.gamma, tl + k * TPR, nv, g, 1.f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float t = to_f(dy[k].v[e]) * x[e];
+        sum[k * V + e] = fmaf(t, inv, sum[k * V + e]);
+        s[0] = fmaf(t, g[e], s[0]);
+      }
+    }
+    fold(s);
+    const float c = inv * inv * (s[0] * inv / static_cast<float>(p.cols));
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int j = tl + k * TPR;
+      if (j >= nv) continue;
+      float x[V], g[V];
+      q8_widen<F, V>(q[k], sc[k], x);
+      load_floats<V>(p.gamma, j, nv, g, 1.f);
+      Vec<T, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(fmaf(inv * to_f(dy[k].v[e]), g[e], -c * x[e]));
+      *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.out) + row * p.cols + static_cast<int64_t>(j) * V) = o;
+    }
+  }
+  if (p.ws == nullptr) return;
+  if constexpr (R > 1) {  // the row slots' sums, in slot order
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) slots[e * (THREADS + TPR) + threadIdx.x] = sum[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float t = 0.f;
+#pragma unroll
+      for (int k = 0; k < R; ++k) t += slots[e * (THREADS + TPR) + k * TPR + tl];
+      sum[e] = t;
+    }
+  }
+  if (rl == 0) {
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int j = tl + k * TPR;
+      if (j >= nvec) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        p.ws[static_cast<int64_t>(blockIdx.x) * p.cols + static_cast<int64_t>(j) * V + e] = sum[k * V + e];
+    }
+  }
+}
+
+template <class T, int F>
+__global__ void __launch_bounds__(256) rmsnorm_bwd8_stream_kernel(const __grid_constant__ Norm8Params p) {
+  __shared__ float red[2][1][8];
+  RowFold<256, 1, 256> fold{red};
+  const int t = threadIdx.x;
+  float* w = p.ws ? p.ws + static_cast<int64_t>(blockIdx.x) * p.cols : nullptr;
+  if (w)
+    for (int64_t j = t; j < p.cols; j += 256) w[j] = 0.f;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const T* dy = static_cast<const T*>(p.dy) + row * p.stride;
+    const uint8_t* q = p.q + row * p.cols;
+    const float* sc = p.scale + row * p.groups;
+    const float inv = p.inv[row];
+    float s[1] = {0.f};
+    for (int64_t j = t; j < p.cols; j += 256) {
+      const float d = to_f(dy[j]) * __fmul_rn(q8_level1<F>(q[j]), sc[j / kQ8Group]);
+      if (w) w[j] = fmaf(d, inv, w[j]);
+      s[0] = fmaf(d, p.gamma ? p.gamma[j] : 1.f, s[0]);
+    }
+    fold(s);
+    const float c = inv * inv * (s[0] * inv / static_cast<float>(p.cols));
+    for (int64_t j = t; j < p.cols; j += 256) {
+      const float x = __fmul_rn(q8_level1<F>(q[j]), sc[j / kQ8Group]);
+      static_cast<T*>(p.out)[row * p.cols + j] =
+          from_f<T>(fmaf(inv * to_f(dy[j]), p.gamma ? p.gamma[j] : 1.f, -c * x));
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) rmsnorm_bwd8_fold_kernel(float* dgamma, const float* ws, int64_t parts, int64_t cols) {
+  __shared__ float sm[8][8];
+  const float s = strip_sum(ws, parts, cols, sm);
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x;
+  if (threadIdx.x < 8 && c < cols) dgamma[c] = s;
+}
+
+// ---------------------------------------------------------------------------------------
+inline unsigned flat_grid(int64_t groups, int lanes, int u) {
+  const int64_t per = int64_t{kCkThreads} / lanes * u;
+  return static_cast<unsigned>((groups + per - 1) / per);
+}
+inline bool rows_fit(int64_t groups) { return groups < (int64_t{1} << 34); }  // a grid of 2^31 blocks
+
+// calls fn(format constant)
+#define VB_FORMAT(format, F, ...)                                                     \
+  do {                                                                                \
+    if ((format) == VBT_B200_Q8_INT8) { constexpr int F = VBT_B200_Q8_INT8; __VA_ARGS__; } \
+    else { constexpr int F = VBT_B200_Q8_E4M3; __VA_ARGS__; }                         \
+  } while (0)
+
+template <class T>
+void launch_checkpoint(const CkParams& p, int format, bool restore, cudaStream_t s) {
+  constexpr int VW = 16 / sizeof(T);
+  const bool vec = p.g.cols % VW == 0 && p.x_stride % VW == 0 && a16(p.x) && a16(p.out) &&
+                   reinterpret_cast<uintptr_t>(p.q) % VW == 0;
+  constexpr int U = 4;
+  unsigned grid = 0;
+#define VB_CK(VEC)                                                                   \
+  do {                                                                               \
+    grid = flat_grid(p.g.total, Lanes<T, VEC>::L, U);                                \
+    if (restore) VB_FORMAT(format, F, (restore8_kernel<T, VEC, F, U><<<grid, kCkThreads, 0, s>>>(p)));    \
+    else VB_FORMAT(format, F, (checkpoint8_kernel<T, VEC, F, U><<<grid, kCkThreads, 0, s>>>(p)));         \
+  } while (0)
+  if (vec) VB_CK(true);
+  else VB_CK(false);
+#undef VB_CK
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_CHECKPOINT8, dim3(grid), dim3(kCkThreads), vec ? VW : 1, 1, 0, 1,
+              p.g.total / p.g.per_row * p.g.cols, p.g.cols, 0, s);
+}
+
+template <class T>
+void launch_glu(const GluParams& p, int format, bool backward, bool kept, cudaStream_t s) {
+  constexpr int VW = 16 / sizeof(T);
+  auto q_ok = [&](const void* q) { return reinterpret_cast<uintptr_t>(q) % VW == 0; };
+  bool vec = p.g.cols % VW == 0 && a16(p.out) && a16(p.dout) && a16(p.dgate) && a16(p.dup) &&
+             p.dout_stride % VW == 0 && q_ok(p.q_gate) && q_ok(p.q_up);
+  if (backward && kept) vec = vec && q_ok(p.gate) && q_ok(p.up);
+  else vec = vec && a16(p.gate) && a16(p.up) && p.gate_stride % VW == 0 && p.up_stride % VW == 0;
+  constexpr int U = 2;
+  unsigned grid = 0;
+#define VB_GLU(VEC)                                                                                             \
+  do {                                                                                                          \
+    grid = flat_grid(p.g.total, Lanes<T, VEC>::L, U);                                                           \
+    if (!backward && !kept) silu_mul_kernel<T, VEC, 0, false, U><<<grid, kCkThreads, 0, s>>>(p);                \
+    else if (!backward) VB_FORMAT(format, F, (silu_mul_kernel<T, VEC, F, true, U><<<grid, kCkThreads, 0, s>>>(p)));   \
+    else if (!kept) silu_mul_bwd_kernel<T, VEC, 0, false, U><<<grid, kCkThreads, 0, s>>>(p);                    \
+    else VB_FORMAT(format, F, (silu_mul_bwd_kernel<T, VEC, F, true, U><<<grid, kCkThreads, 0, s>>>(p)));              \
+  } while (0)
+  if (vec) VB_GLU(true);
+  else VB_GLU(false);
+#undef VB_GLU
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_SILU_MUL, dim3(grid), dim3(kCkThreads), vec ? VW : 1, 1, 0, 1,
+              p.g.total / p.g.per_row * p.g.cols, p.g.cols, 0, s);
+}
+
+template <class T>
+void launch_norm8(const Norm8Params& p, int format, cudaStream_t s, int device) {
+  constexpr int VW = 16 / sizeof(T);
+  constexpr int E = 16;
+  const int sms = sm_count(device);
+  const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.x) && a16(p.out) && a16(p.gamma) &&
+                   reinterpret_cast<uintptr_t>(p.q) % VW == 0;
+  unsigned g = 0;
+  int threads = 256;
+  auto grid = [&](int per_block, int per_sm) {
+    return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((p.rows + per_block - 1) / per_block, int64_t{sms} * per_sm)));
+  };
+#define VB_N8(TPR)                                                                                      \
+  do {                                                                                                  \
+    threads = TPR < 256 ? 256 : TPR;                                                                    \
+    g = grid(threads / TPR, 2048 / threads);                                                            \
+    VB_FORMAT(format, F, (rmsnorm8_kernel<T, F, E / VW, TPR><<<g, threads, 0, s>>>(p)));                \
+  } while (0)
+  if (!vec || p.cols > 1024 * E) {
+    g = grid(1, 8);
+    VB_FORMAT(format, F, (rmsnorm8_stream_kernel<T, F><<<g, threads, 0, s>>>(p)));
+  } else if (p.cols <= 32 * E) VB_N8(32);
+  else if (p.cols <= 128 * E) VB_N8(128);
+  else if (p.cols <= 256 * E) VB_N8(256);
+  else if (p.cols <= 512 * E) VB_N8(512);
+  else VB_N8(1024);
+#undef VB_N8
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_CHECKPOINT8, dim3(g), dim3(threads), vec ? VW : 1, 1, 0, 1,
+              p.rows * p.cols, p.cols, 0, s);
+}
+
+constexpr int bwd8_elts(int elt) { return elt == 2 ? 16 : 8; }
+inline unsigned bwd8_grid(int64_t rows, int sms) {
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(rows, int64_t{sms} * 6)));
+}
+
+template <class T>
+int launch_norm_bwd8(const Norm8Params& p, float* dgamma, int format, cudaStream_t s, int device) {
+  constexpr int VW = 16 / sizeof(T);
+  constexpr int E = bwd8_elts(sizeof(T));
+  const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.dy) && a16(p.out) && a16(p.gamma) &&
+                   reinterpret_cast<uintptr_t>(p.q) % VW == 0;
+  const unsigned most = bwd8_grid(p.rows, sm_count(device));
+  unsigned g = most;
+  int threads = 256;
+#define VB_B8(TPR)                                                                                      \
+  do {                                                                                                  \
+    threads = TPR < 128 ? 128 : TPR;                                                                    \
+    g = static_cast<unsigned>(std::min<int64_t>(most, (p.rows + threads / TPR - 1) / (threads / TPR))); \
+    VB_FORMAT(format, F, (rmsnorm_bwd8_kernel<T, F, E / VW, TPR><<<g, threads, 0, s>>>(p)));            \
+  } while (0)
+  if (!vec || p.cols > 512 * E) VB_FORMAT(format, F, (rmsnorm_bwd8_stream_kernel<T, F><<<g, threads, 0, s>>>(p)));
+  else if (p.cols <= 8 * E) VB_B8(8);
+  else if (p.cols <= 32 * E) VB_B8(32);
+  else if (p.cols <= 128 * E) VB_B8(128);
+  else if (p.cols <= 256 * E) VB_B8(256);
+  else VB_B8(512);
+#undef VB_B8
+  if (p.ws) rmsnorm_bwd8_fold_kernel<<<static_cast<unsigned>((p.cols + 7) / 8), 256, 0, s>>>(dgamma, p.ws, g, p.cols);
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_RMSNORM_BACKWARD8, dim3(g), dim3(threads), vec ? VW : 1, 1, 0,
+              p.ws ? 2 : 1, p.rows * p.cols, p.cols, p.ws ? static_cast<size_t>(g) * p.cols * 4 : 0, s);
+  return 0;
+}
+
+vbt_b200_status check_common(const char* name, int32_t dtype, int32_t format, int64_t rows, int64_t cols) {
+  VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
+  VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
+  VB_ARG(format == VBT_B200_Q8_INT8 || format == VBT_B200_Q8_E4M3, std::string(name) + ": unknown 8-bit format");
+  VB_ARG(cols == 0 || rows_fit(rows * ((cols + kQ8Group - 1) / kQ8Group)), std::string(name) + ": too many groups");
+  return VBT_B200_OK;
+}
+
+#define VB_BY_DTYPE(dtype, T, ...)                                            \
+  switch (dtype) {                                                            \
+    case VBT_B200_F32: { using T = float; __VA_ARGS__; break; }               \
+    case VBT_B200_F16: { using T = __half; __VA_ARGS__; break; }              \
+    default: { using T = __nv_bfloat16; __VA_ARGS__; break; }                 \
+  }
+
+}  // namespace
+}  // namespace vb
+
+extern "C" {
+
+vbt_b200_status vbt_b200_checkpoint8(void* q, float* scale, const void* x, int32_t dtype, int32_t format, int64_t rows,
+                                     int64_t cols, int64_t x_row_stride, void* stream) {
+  using namespace vb;
+  VB_TRY(check_common("checkpoint8", dtype, format, rows, cols));
+  if (rows == 0 || cols == 0) return VBT_B200_OK;
+  VB_ARG(q && scale && x, "checkpoint8: null pointer");
+  VB_ARG(x_row_stride >= 0, "checkpoint8: negative row stride");
+  DeviceScope scope(q);
+  CkParams p{};
+  p.x = x; p.q = static_cast<uint8_t*>(q); p.scale = scale; p.x_stride = x_row_stride;
+  p.g.fill(rows, cols);
+  VB_BY_DTYPE(dtype, T, launch_checkpoint<T>(p, format, false, static_cast<cudaStream_t>(stream)));
+  VB_LAUNCH_CHECK();
+  return VBT_B200_OK;
+}
+
+vbt_b200_status vbt_b200_checkpoint8_restore(void* out, const void* q, const float* scale, int32_t dtype, int32_t format,
+                                             int64_t rows, int64_t cols, void* stream) {
+  using namespace vb;
+  VB_TRY(check_common("checkpoint8_restore", dtype, format, rows, cols));
+  if (rows == 0 || cols == 0) return VBT_B200_OK;
+  VB_ARG(out && q && scale, "checkpoint8_restore: null pointer");
+  DeviceScope scope(out);
+  CkParams p{};
+  p.out = out; p.q = static_cast<uint8_t*>(const_cast<void*>(q)); p.scale = const_cast<float*>(scale);
+  p.g.fill(rows, cols);
+  VB_BY_DTYPE(dtype, T, launch_checkpoint<T>(p, format, true, static_cast<cudaStream_t>(stream)));
+  VB_LAUNCH_CHECK();
+  return VBT_B200_OK;
+}
+
+vbt_b200_status vbt_b200_rmsnorm_checkpoint8(void* out, float* inv_rms, void* q, float* scale, const void* x,
+                                             const float* gamma, int32_t dtype, int32_t format, int64_t rows,
+                                             int64_t cols, int64_t x_row_stride, float eps, void* stream) {
+  using namespace vb;
+  VB_TRY(check_common("rmsnorm_checkpoint8", dtype, format, rows, cols));
+  if (rows == 0 || cols == 0) return VBT_B200_OK;
+  VB_ARG(out && q && scale && x, "rmsnorm_checkpoint8: null pointer");
+  VB_ARG(x_row_stride >= 0, "rmsnorm_checkpoint8: negative row stride");
+  DeviceScope scope(out);
+  Norm8Params p{};
+  p.x = x; p.gamma = gamma; p.out = out; p.q = static_cast<uint8_t*>(q); p.scale = scale; p.inv = inv_rms;
+  p.rows = rows; p.cols = cols; p.groups = (cols + kQ8Group - 1) / kQ8Group; p.stride = x_row_stride; p.eps = eps;
+  VB_BY_DTYPE(dtype, T, launch_norm8<T>(p, format, static_cast<cudaStream_t>(stream), scope.device()));
+  VB_LAUNCH_CHECK();
+  return VBT_B200_OK;
+}
+
+vbt_b200_status vbt_b200_rmsnorm_backward8_workspace_bytes(int64_t rows, int64_t cols, int32_t dtype, int32_t device,
+                                                           size_t* bytes) {
+  using namespace vb;
+  VB_ARG(bytes != nullptr, "rmsnorm_backward8: null output");
+  VB_TRY(check_common("rmsnorm_backward8", dtype, VBT_B200_Q8_INT8, rows, cols));
+  *bytes = static_cast<size_t>(bwd8_grid(rows, sm_count(device))) * static_cast<size_t>(cols) * 4;
+  return VBT_B200_OK;
+}
+
+vbt_b200_status vbt_b200_rmsnorm_backward8(void* dx, float* dgamma, const void* dy, const void* q, const float* scale,
+                                           const float* inv_rms, const float* gamma, int32_t dtype, int32_t format,
+                                           int64_t rows, int64_t cols, int64_t dy_row_stride, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  using namespace vb;
+  VB_TRY(check_common("rmsnorm_backward8", dtype, format, rows, cols));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cols == 0) return VBT_B200_OK;
+  if (rows == 0) {
+    if (dgamma) {
+      DeviceScope scope(dgamma);
+      VB_CUDA(cudaMemsetAsync(dgamma, 0, static_cast<size_t>(cols) * 4, s));
+    }
+    return VBT_B200_OK;
+  }
+  VB_ARG(dx && dy && q && scale && inv_rms, "rmsnorm_backward8: null pointer");
+  VB_ARG(dy_row_stride >= 0, "rmsnorm_backward8: negative row stride");
+  DeviceScope scope(dx);
+  Norm8Params p{};
+  p.dy = dy; p.gamma = gamma; p.out = dx; p.q = static_cast<uint8_t*>(const_cast<void*>(q));
+  p.scale = const_cast<float*>(scale); p.inv = const_cast<float*>(inv_rms);
+  p.rows = rows; p.cols = cols; p.groups = (cols + kQ8Group - 1) / kQ8Group; p.stride = dy_row_stride;
+  if (dgamma) {
+    size_t need = 0;
+    VB_TRY(vbt_b200_rmsnorm_backward8_workspace_bytes(rows, cols, dtype, scope.device(), &need));
+    VB_ARG(workspace != nullptr && workspace_bytes >= need,
+           "rmsnorm_backward8: workspace too small (see vbt_b200_rmsnorm_backward8_workspace_bytes)");
+    p.ws = static_cast<float*>(workspace);
+  }
+  VB_BY_DTYPE(dtype, T, launch_norm_bwd8<T>(p, dgamma, format, s, scope.device()));
+  VB_LAUNCH_CHECK();
+  return VBT_B200_OK;
+}
+
+vbt_b200_status vbt_b200_silu_mul(void* out, void* q_gate, float* scale_gate, void* q_up, float* scale_up,
+                                  const void* gate, const void* up, int32_t dtype, int32_t format, int64_t rows,
+                                  int64_t cols, int64_t gate_row_stride, int64_t up_row_stride, void* stream) {
+  using namespace vb;
+  VB_TRY(check_common("silu_mul", dtype, format, rows, cols));
+  if (rows == 0 || cols == 0) return VBT_B200_OK;
+  VB_ARG(out && gate && up, "silu_mul: null pointer");
+  VB_ARG(q_gate == nullptr || (scale_gate && q_up && scale_up), "silu_mul: the 8-bit copies need all four outputs");
+  VB_ARG(gate_row_stride >= 0 && up_row_stride >= 0, "silu_mul: negative row stride");
+  DeviceScope scope(out);
+  GluParams p{};
+  p.gate = gate; p.up = up; p.out = out; p.gate_stride = gate_row_stride; p.up_stride = up_row_stride;
+  p.q_gate = static_cast<uint8_t*>(q_gate); p.s_gate = scale_gate;
+  p.q_up = static_cast<uint8_t*>(q_up); p.s_up = scale_up;
+  p.g.fill(rows, cols);
+  VB_BY_DTYPE(dtype, T, launch_glu<T>(p, format, false, q_gate != nullptr, static_cast<cudaStream_t>(stream)));
+  VB_LAUNCH_CHECK();
+  return VBT_B200_OK;
+}
+
+vbt_b200_status vbt_b200_silu_mul_backward(void* dgate, void* dup, const void* dout, const void* gate,
+                                           const float* scale_gate, const void* up, const float* scale_up,
+                                           int32_t dtype, int32_t format, int64_t rows, int64_t cols,
+                                           int64_t dout_row_stride, int64_t gate_row_stride, int64_t up_row_stride,
+                                           void* stream) {
+  using namespace vb;
+  VB_TRY(check_common("silu_mul_backward", dtype, format, rows, cols));
+  if (rows == 0 || cols == 0) return VBT_B200_OK;
+  VB_ARG(dgate && dup && dout && gate && up, "silu_mul_backward: null pointer");
+  VB_ARG((scale_gate == nullptr) == (scale_up == nullptr), "silu_mul_backward: both factors or neither in 8 bits");
+  VB_ARG(dout_row_stride >= 0 && gate_row_stride >= 0 && up_row_stride >= 0, "silu_mul_backward: negative row stride");
+  DeviceScope scope(dgate);
+  GluParams p{};
+  p.dout = dout; p.gate = gate; p.up = up; p.gate_scale = scale_gate; p.up_scale = scale_up;
+  p.dgate = dgate; p.dup = dup;
+  p.dout_stride = dout_row_stride; p.gate_stride = gate_row_stride; p.up_stride = up_row_stride;
+  p.g.fill(rows, cols);
+  VB_BY_DTYPE(dtype, T, launch_glu<T>(p, format, true, scale_gate != nullptr, static_cast<cudaStream_t>(stream)));
+  VB_LAUNCH_CHECK();
+  return VBT_B200_OK;
+}
+
+}  // extern "C"

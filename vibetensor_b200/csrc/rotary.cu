@@ -1,0 +1,260 @@
+// Rotary positions with several axes, queries and keys in one launch (sm_100a).
+//
+//   pair i of a head turns by  angle = positions[axis(i), b, t] * inv_freq[i]
+//   a' = a cos - b sin,  b' = b cos + a sin      (the backward pass turns by -angle)
+//
+// The angle is formed in 64 bits and reduced there to the part of a turn behind the nearest
+// quarter, so a position of a million keeps every bit of its angle; sine and cosine of what is left
+// are 32-bit.  A block computes the table of its tokens' cosines and sines once in shared memory
+// and turns all the heads it owns with it: the operator moves every value once and is bound by
+// memory.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace vb {
+namespace {
+
+constexpr int kRotThreads = 256;
+
+struct RotSide {
+  const void* in;
+  void* out;
+  int64_t in_b, in_t, in_h;     // strides in elements
+  int64_t out_b, out_t, out_h;
+};
+struct RotParams {
+  RotSide q, k;
+  const void* pos;
+  const float* freq;
+  int64_t pos_a, pos_b, pos_t;
+  int64_t count;        // batch * tokens
+  int64_t tokens;
+  int pos_dtype;
+  int q_heads, heads;   // heads: q and k together
+  int dim, half;
+  int rot_items, items; // per head: vector pairs that turn, all pieces of work
+  int tb, hb;           // tokens and heads of a block
+  int end[VBT_B200_ROTARY_MAX_AXES];  // end[a]: first pair behind axis a's section
+  FastDiv div_items, div_half;
+  float sign;
+};
+
+// cos and sin of 2 pi * turns
+__device__ __forceinline__ void turn(double turns, float& c, float& s) {
+  const double quarter = rint(turns * 4.0);
+  const float left = static_cast<float>((turns - quarter * 0.25) * 2.0);  // half turns, |left| <= 1/4
+  float sl, cl;
+  sincospif(left, &sl, &cl);
+  // quarter mod 4 without a trip through a 64-bit integer
+  const int qd = static_cast<int>(quarter - 4.0 * floor(quarter * 0.25));
+  c = (qd & 1) ? sl : cl;
+  s = (qd & 1) ? cl : sl;
+  if (qd == 1 || qd == 2) c = -c;
+  if (qd >= 2) s = -s;
+}
+
+// P pairs per piece of work.  PAIRED: neighbours (2i, 2i + 1) in one vector of 2P values; else P
+// values at i and P at half + i.  VEC: the vectors may be read whole.
+template <class T, int P, bool PAIRED, bool VEC>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotParams p) {
+  extern __shared__ float table[];  // cosines [tb][half], then sines
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tb;
+  const int tb = static_cast<int>(min(static_cast<int64_t>(p.tb), p.count - first));
+  float* cosines = table;
+  float* sines = table + p.tb * p.half;
+  for (int i = threadIdx.x; i < tb * p.half; i += kRotThreads) {
+    uint32_t tok, f;
+    p.div_half.divmod(static_cast<uint32_t>(i), tok, f);
+    const int64_t at = first + tok, b = at / p.tokens, t = at - b * p.tokens;
+    int axis = 0;
+#pragma unroll
+    for (int a = 0; a < VBT_B200_ROTARY_MAX_AXES - 1; ++a) axis += static_cast<int>(f) >= p.end[a];
+    const int64_t src = axis * p.pos_a + b * p.pos_b + t * p.pos_t;
+    const double pos = p.pos_dtype == VBT_B200_I64   ? static_cast<double>(static_cast<const int64_t*>(p.pos)[src])
+                       : p.pos_dtype == VBT_B200_I32 ? static_cast<double>(static_cast<const int32_t*>(p.pos)[src])
+                                                     : static_cast<double>(static_cast<const float*>(p.pos)[src]);
+    float c, s;
+    turn(pos * static_cast<double>(p.freq[f]) * 0.15915494309189533577, c, s);
+    cosines[i] = c;
+    sines[i] = p.sign * s;
+  }
+  __syncthreads();
+  const int h0 = blockIdx.y * p.hb;
+  const int hn = min(p.hb, p.heads - h0);
+  const int per_token = hn * p.items;
+  constexpr int W = PAIRED ? 2 * P : P;
+  for (int tok = 0; tok < tb; ++tok) {
+    const int64_t at = first + tok, b = at / p.tokens, t = at - b * p.tokens;
+    const float* ct = cosines + tok * p.half;
+    const float* st = sines + tok * p.half;
+    for (int i = threadIdx.x; i < per_token; i += kRotThreads) {
+      uint32_t hl, item;
+      p.div_items.divmod(static_cast<uint32_t>(i), hl, item);
+      const int h = h0 + static_cast<int>(hl);
+      const bool isq = h < p.q_heads;
+      const RotSide& side = isq ? p.q : p.k;
+      const int hh = isq ? h : h - p.q_heads;
+      const T* in = static_cast<const T*>(side.in) + b * side.in_b + t * side.in_t + hh * side.in_h;
+      T* out = static_cast<T*>(side.out) + b * side.out_b + t * side.out_t + hh * side.out_h;
+      if (static_cast<int>(item) >= p.rot_items) {  // values behind the turned ones
+        const int e0 = 2 * p.half + (static_cast<int>(item) - p.rot_items) * W;
+        if constexpr (VEC) {
+          *reinterpret_cast<Vec<T, W>*>(out + e0) = *reinterpret_cast<const Vec<T, W>*>(in + e0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+            if (e0 + e < p.dim) out[e0 + e] = in[e0 + e];
+        }
+        continue;
+      }
+      const int i0 = static_cast<int>(item) * P;
+      if constexpr (PAIRED) {
+        Vec<T, 2 * P> v;
+        if constexpr (VEC) v = *reinterpret_cast<const Vec<T, 2 * P>*>(in + 2 * i0);
+        else { v.v[0] = in[2 * i0]; v.v[1] = in[2 * i0 + 1]; }
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const float c = ct[i0 + e], s = st[i0 + e], x = to_f(v.v[2 * e]), y = to_f(v.v[2 * e + 1]);
+          v.v[2 * e] = from_f<T>(x * c - y * s);
+          v.v[2 * e + 1] = from_f<T>(y * c + x * s);
+        }
+        if constexpr (VEC) *reinterpret_cast<Vec<T, 2 * P>*>(out + 2 * i0) = v;
+        else { out[2 * i0] = v.v[0]; out[2 * i0 + 1] = v.v[1]; }
+      } else {
+        Vec<T, P> x = *reinterpret_cast<const Vec<T, P>*>(in + i0);
+        Vec<T, P> y = *reinterpret_cast<const Vec<T, P>*>(in + p.half + i0);
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const float c = ct[i0 + e], s = st[i0 + e], xf = to_f(x.v[e]), yf = to_f(y.v[e]);
+          x.v[e] = from_f<T>(xf * c - yf * s);
+          y.v[e] = from_f<T>(yf * c + xf * s);
+        }
+        *reinterpret_cast<Vec<T, P>*>(out + i0) = x;
+        *reinterpret_cast<Vec<T, P>*>(out + p.half + i0) = y;
+      }
+    }
+  }
+}
+
+template <class T>
+bool side_fits(const RotSide& s, int values) {
+  const int bytes = values * static_cast<int>(sizeof(T));
+  auto ok = [&](int64_t stride) { return stride % values == 0; };
+  return reinterpret_cast<uintptr_t>(s.in) % bytes == 0 && reinterpret_cast<uintptr_t>(s.out) % bytes == 0 &&
+         ok(s.in_b) && ok(s.in_t) && ok(s.in_h) && ok(s.out_b) && ok(s.out_t) && ok(s.out_h);
+}
+
+template <class T>
+vbt_b200_status launch_rotary(RotParams p, int interleaved, cudaStream_t s) {
+  constexpr int most = 16 / sizeof(T);
+  const bool has_k = p.heads > p.q_heads, has_q = p.q_heads > 0;
+  auto fits = [&](int values) {
+    return (!has_q || side_fits<T>(p.q, values)) && (!has_k || side_fits<T>(p.k, values)) &&
+           (p.dim - 2 * p.half) % values == 0;
+  };
+  // the widest vector that every address, the pairs and the rest of a head divide into
+  int values = most, pairs = 1;
+  bool vec = false;
+  for (; values >= (interleaved ? 2 : 1); values /= 2) {
+    pairs = interleaved ? values / 2 : values;
+    if (p.half % pairs == 0 && fits(values)) { vec = true; break; }
+  }
+  if (!vec) { pairs = 1; values = interleaved ? 2 : 1; }
+  p.rot_items = p.half / pairs;
+  p.items = p.rot_items + (p.dim - 2 * p.half + values - 1) / values;
+  p.div_items = FastDiv(static_cast<uint32_t>(p.items));
+  p.div_half = FastDiv(static_cast<uint32_t>(std::max(p.half, 1)));
+  // a block takes all heads of as many tokens as give each thread four pieces (the table is worked out once
+  // per token); with too few tokens to fill the card the heads are cut instead
+  const int64_t per_token = int64_t{p.heads} * p.items;
+  p.tb = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4 * kRotThreads / std::max<int64_t>(per_token, 1), 4096 / std::max(p.half, 1))));
+  p.hb = p.heads;
+  if (p.count <= 296) {
+    p.tb = 1;
+    p.hb = std::max(1, std::min(p.heads, kRotThreads / std::max(p.items, 1)));
+  }
+  dim3 grid(static_cast<unsigned>((p.count + p.tb - 1) / p.tb), static_cast<unsigned>((p.heads + p.hb - 1) / p.hb));
+  const size_t smem = static_cast<size_t>(p.tb) * p.half * 8;
+#define VB_ROT(P, PAIRED, VEC) rotary_kernel<T, P, PAIRED, VEC><<<grid, kRotThreads, smem, s>>>(p)
+  if (interleaved) {
+    if (!vec) VB_ROT(1, true, false);
+    else if (pairs == 1) VB_ROT(1, true, true);
+    else if (pairs == 2) VB_ROT(2, true, true);
+    else if constexpr (most == 8) VB_ROT(4, true, true);
+  } else {
+    if (pairs == 1) VB_ROT(1, false, true);
+    else if (pairs == 2) VB_ROT(2, false, true);
+    else if (pairs == 4) VB_ROT(4, false, true);
+    else if constexpr (most == 8) VB_ROT(8, false, true);
+  }
+#undef VB_ROT
+  VB_LAUNCH_CHECK();
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_ROTARY, grid, dim3(kRotThreads), values, 1, 0, 1,
+              p.count * p.heads * p.dim, p.dim, 0, s);
+  return VBT_B200_OK;
+}
+
+}  // namespace
+}  // namespace vb
+
+extern "C" {
+
+vbt_b200_status vbt_b200_rotary(void* q_out, const int64_t* q_out_strides, const void* q, const int64_t* q_strides,
+                                int64_t q_heads, void* k_out, const int64_t* k_out_strides, const void* k,
+                                const int64_t* k_strides, int64_t k_heads, int32_t dtype, int64_t batch, int64_t tokens,
+                                int64_t dim, const void* positions, int32_t positions_dtype,
+                                const int64_t* positions_strides, const float* inv_freq, int64_t half,
+                                const int64_t* sections, int32_t naxes, int32_t interleaved, int32_t inverse,
+                                void* stream) {
+  using namespace vb;
+  VB_ARG(is_float_dtype(dtype), "rotary: expected a floating dtype");
+  VB_ARG(batch >= 0 && tokens >= 0 && dim >= 0 && q_heads >= 0 && k_heads >= 0 && half >= 0, "rotary: negative size");
+  VB_ARG(2 * half <= dim, "rotary: more pairs than the head has values for");
+  VB_ARG(naxes >= 1 && naxes <= VBT_B200_ROTARY_MAX_AXES && sections, "rotary: expected 1 to 4 sections");
+  int64_t sum = 0;
+  for (int a = 0; a < naxes; ++a) {
+    VB_ARG(sections[a] >= 0, "rotary: negative section");
+    sum += sections[a];
+  }
+  VB_ARG(sum == half, "rotary: the sections do not sum to the number of pairs");
+  VB_ARG(positions_dtype == VBT_B200_I64 || positions_dtype == VBT_B200_I32 || positions_dtype == VBT_B200_F32,
+         "rotary: positions must be int64, int32 or float32");
+  if (k == nullptr) k_heads = 0;
+  if (batch == 0 || tokens == 0 || dim == 0 || q_heads + k_heads == 0) return VBT_B200_OK;
+  VB_ARG(half <= 4096 && q_heads <= 16384 && k_heads <= 16384 && dim <= (int64_t{1} << 28) / (q_heads + k_heads),
+         "rotary: head too wide or too many heads");
+  VB_ARG(q_heads == 0 || (q && q_out && q_strides && q_out_strides), "rotary: null pointer");
+  VB_ARG(k_heads == 0 || (k && k_out && k_strides && k_out_strides), "rotary: null pointer");
+  VB_ARG(positions_strides && (half == 0 || (positions && inv_freq)), "rotary: null pointer");
+  VB_ARG(batch <= (int64_t{1} << 31) / tokens, "rotary: too many tokens");
+  DeviceScope scope(q_heads ? q_out : k_out);
+  RotParams p{};
+  auto side = [](RotSide& s, const void* in, const int64_t* is, void* out, const int64_t* os) {
+    s.in = in; s.in_b = is[0]; s.in_t = is[1]; s.in_h = is[2];
+    s.out = out; s.out_b = os[0]; s.out_t = os[1]; s.out_h = os[2];
+  };
+  if (q_heads) side(p.q, q, q_strides, q_out, q_out_strides);
+  if (k_heads) side(p.k, k, k_strides, k_out, k_out_strides);
+  p.pos = positions; p.pos_dtype = positions_dtype;
+  p.pos_a = positions_strides[0]; p.pos_b = positions_strides[1]; p.pos_t = positions_strides[2];
+  p.freq = inv_freq;
+  p.count = batch * tokens; p.tokens = tokens;
+  p.q_heads = static_cast<int>(q_heads); p.heads = static_cast<int>(q_heads + k_heads);
+  p.dim = static_cast<int>(dim); p.half = static_cast<int>(half);
+  int64_t end = 0;
+  for (int a = 0; a < VBT_B200_ROTARY_MAX_AXES; ++a) {
+    end += a < naxes ? sections[a] : 0;
+    // behind the last given section every pair stays on its axis
+    p.end[a] = a < naxes - 1 ? static_cast<int>(end) : INT32_MAX;
+  }
+  p.sign = inverse ? -1.f : 1.f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case VBT_B200_F32: return launch_rotary<float>(p, interleaved, s);
+    case VBT_B200_F16: return launch_rotary<__half>(p, interleaved, s);
+    default: return launch_rotary<__nv_bfloat16>(p, interleaved, s);
+  }
+}
+
+}  // extern "C"

@@ -12,16 +12,24 @@ Triton kernels compiled at run time:
 Same argument meaning and the same exception classes for the same misuse (RuntimeError for a
 non-CUDA tensor, TypeError for a dtype, NotImplementedError for an unsupported dim); float16
 and bfloat16 inputs are accepted in addition to the reference's float32.
+
+Around a transformer block's matrix products, in the same manner (no counterpart in the reference):
+
+* ``residual_norm``              -- a branch joined with the residual stream between two norms
+* ``checkpoint8`` and its users  -- activations kept in 8 bits for the backward pass
+* ``silu_mul``                   -- the gated activation
+* ``rotary``                     -- rotary positions with several axes
 """
 from __future__ import annotations
 
+import builtins
 import ctypes
 from typing import Optional
 
 import torch
 
 from . import ops as _ops
-from ._lib import check, dtype_code, lib, stream_ptr
+from ._lib import Q8_FORMATS as _Q8_FORMATS, Q8_GROUP, check, dtype_code, i64_array, lib, stream_ptr
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -125,11 +133,14 @@ def log_softmax_backward(dy: torch.Tensor, log_y: torch.Tensor) -> torch.Tensor:
     return _softmax_backward(dy, log_y, True)
 
 
-def rmsnorm_backward(grad_output: torch.Tensor, x: torch.Tensor, inv_rms: torch.Tensor,
+def rmsnorm_backward(grad_output: torch.Tensor, x, inv_rms: torch.Tensor,
                      gamma: Optional[torch.Tensor] = None):
     """Returns (grad_input, grad_gamma); grad_gamma is None when gamma is None, float32
-    [hidden_size] otherwise.  inv_rms is the second result of ``rmsnorm``."""
+    [hidden_size] otherwise.  inv_rms is the second result of ``rmsnorm``.  x may be the
+    ``Checkpoint8`` that ``rmsnorm_checkpoint8`` kept in its place."""
     what = "rmsnorm_backward"
+    if isinstance(x, Checkpoint8):
+        return _rmsnorm_backward8(grad_output, x, inv_rms, gamma)
     if grad_output.shape != x.shape:
         raise ValueError(f"{what}: grad_output and x must have the same shape")
     if grad_output.dtype != x.dtype:
@@ -203,3 +214,434 @@ def scatter_add(out: torch.Tensor, dim: int, index: torch.Tensor, src: torch.Ten
     _ops.index_put_rows_(out2, index, src2, accumulate=True, policy=_ops.INDEX_CLAMP, status=status,
                          eager_check=False)
     return out
+
+
+# --------------------------------------------------------------------------------------
+# around a transformer block's matrix products
+# --------------------------------------------------------------------------------------
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} requires CUDA tensors")
+        if t.device != first.device:
+            raise ValueError(f"{what}: operands on {first.device} and {t.device}")
+
+
+def _like(what: str, name: str, t: torch.Tensor, x: torch.Tensor) -> None:
+    if t.shape != x.shape:
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(x.shape)}")
+    if t.dtype != x.dtype:
+        raise TypeError(f"{what}: {name} is {t.dtype}, expected {x.dtype}")
+
+
+def _gamma(name: str, g: Optional[torch.Tensor], cols: int) -> Optional[torch.Tensor]:
+    if g is None:
+        return None
+    if g.dtype != torch.float32 or g.numel() != cols:
+        raise TypeError(f"{name} must be float32 of shape [hidden_size]")
+    return g.contiguous()
+
+
+def _row_scalars(name: str, t: Optional[torch.Tensor], rows: int) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != rows:
+        raise TypeError(f"{name} must be float32 of shape [rows]")
+    return t.contiguous()
+
+
+def _gate_rows(what: str, gate: Optional[torch.Tensor], x: torch.Tensor, rows: int):
+    """(gate, row stride, rows of x per gate row) of a gate that broadcasts to x over its inner
+    leading dims: [hidden], x.shape[:k] + (1, ..., 1, hidden), or x's own shape."""
+    if gate is None:
+        return None, 0, max(rows, 1)
+    if gate.dtype != x.dtype:
+        raise TypeError(f"{what}: gate is {gate.dtype}, expected {x.dtype}")
+    lead, g = tuple(x.shape[:-1]), tuple(gate.shape[:-1])
+    if gate.dim() == 0 or gate.shape[-1] != x.shape[-1] or (gate.dim() != 1 and gate.dim() != x.dim()):
+        raise ValueError(f"{what}: gate of shape {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
+    k = 0
+    while k < len(g) and g[k] == lead[k]:
+        k += 1
+    if any(n != 1 for n in g[k:]):
+        raise ValueError(f"{what}: gate of shape {tuple(gate.shape)} does not broadcast to the last leading dims of "
+                         f"{tuple(x.shape)}")
+    gv, grows, _, stride = _rows_view(gate, what)
+    return gv, stride, max(rows // max(grows, 1), 1)
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, gamma_post: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, gamma_pre: Optional[torch.Tensor] = None, eps: float = 1e-6, *,
+                  post_norm: bool = True, pre_norm: bool = True, residual_scale: float = 1.0,
+                  branch_scale: float = 1.0):
+    """The join of a branch's output y with the residual stream x, and the norm in front of the next
+    block, in one pass over the rows:
+
+        v = y * inv_post * gamma_post           (post_norm; v = y without)
+        r = residual_scale * x + branch_scale * gate * v
+        n = r * inv_pre * gamma_pre             (pre_norm; from the unrounded r)
+
+    x and y are float32, float16 or bfloat16 of one shape; gate has their dtype and is None,
+    [hidden], x.shape[:k] + (1, ..., 1, hidden) (one row per sample, say) or x's own shape; gammas
+    are float32 [hidden] or None (ones).  Returns (r, n, inv_post, inv_pre), the last two float32
+    [rows]; what a switched-off norm would give is None."""
+    what = "residual_norm"
+    xv, rows, cols, rs_x = _rows_view(x, what)
+    _same_device(what, x, y, gamma_post, gate, gamma_pre)
+    _like(what, "y", y, x)
+    if gamma_post is not None and not post_norm or gamma_pre is not None and not pre_norm:
+        raise ValueError(f"{what}: a gamma of a norm that is switched off")
+    yv, _, _, rs_y = _rows_view(y, what)
+    gamma_post, gamma_pre = _gamma("gamma_post", gamma_post, cols), _gamma("gamma_pre", gamma_pre, cols)
+    gv, rs_g, per = _gate_rows(what, gate, x, rows)
+    r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre_norm else None
+    inv_post = torch.empty((rows,), dtype=torch.float32, device=x.device) if post_norm else None
+    inv_pre = torch.empty((rows,), dtype=torch.float32, device=x.device) if pre_norm else None
+    if rows and cols:
+        check(lib().vbt_b200_residual_norm(
+            _ptr(r), _ptr(n), _ptr(inv_post), _ptr(inv_pre), _ptr(xv), _ptr(yv), _ptr(gamma_post), _ptr(gv),
+            _ptr(gamma_pre), dtype_code(x.dtype), rows, cols, rs_x, rs_y, rs_g, per, float(residual_scale),
+            float(branch_scale), float(eps), int(post_norm) | 2 * int(pre_norm), stream_ptr(x)))
+    return r, n, inv_post, inv_pre
+
+
+def residual_norm_backward(grad_r: Optional[torch.Tensor], grad_n: Optional[torch.Tensor], y: Optional[torch.Tensor],
+                           r: Optional[torch.Tensor], inv_post: Optional[torch.Tensor],
+                           inv_pre: Optional[torch.Tensor], gamma_post: Optional[torch.Tensor] = None,
+                           gate: Optional[torch.Tensor] = None, gamma_pre: Optional[torch.Tensor] = None, *,
+                           residual_scale: float = 1.0, branch_scale: float = 1.0):
+    """Backward of ``residual_norm``: from the gradients that arrive at r (None: none) and n, the
+    branch's output y, and r and the reciprocal norms the forward pass returned (None where its norm
+    was off), returns (grad_x, grad_y, grad_gamma_post, grad_gate, grad_gamma_pre).  Gradients of
+    what was None are None; grad_gamma_* are float32 and sums over rows are reproducible run to run.
+    y is only needed with post_norm or a gate, r only with pre_norm."""
+    what = "residual_norm_backward"
+    first = grad_n if grad_n is not None else grad_r
+    if first is None:
+        raise ValueError(f"{what}: no gradient given")
+    post, pre = inv_post is not None, inv_pre is not None
+    if pre and (grad_n is None or r is None):
+        raise ValueError(f"{what}: inv_pre given without grad_n and r")
+    if not pre and grad_n is not None:
+        raise ValueError(f"{what}: grad_n given without inv_pre")
+    if (post or gate is not None) and y is None:
+        raise ValueError(f"{what}: y is needed with post_norm or a gate")
+    if gamma_post is not None and not post or gamma_pre is not None and not pre:
+        raise ValueError(f"{what}: a gamma of a norm that is switched off")
+    xv, rows, cols, _ = _rows_view(first, what)
+    _same_device(what, first, grad_r, grad_n, y, r, inv_post, inv_pre, gamma_post, gate, gamma_pre)
+    views = []
+    for name, t in (("grad_r", grad_r), ("grad_n", grad_n), ("y", y), ("r", r if pre else None)):
+        if t is None:
+            views.append((None, 0))
+            continue
+        _like(what, name, t, first)
+        v, _, _, rs = _rows_view(t, what)
+        views.append((v, rs))
+    inv_post, inv_pre = _row_scalars("inv_post", inv_post, rows), _row_scalars("inv_pre", inv_pre, rows)
+    gamma_post, gamma_pre = _gamma("gamma_post", gamma_post, cols), _gamma("gamma_pre", gamma_pre, cols)
+    gv, rs_g, per = _gate_rows(what, gate, first, rows)
+    dx = torch.empty(first.shape, dtype=first.dtype, device=first.device)
+    dy = torch.empty(first.shape, dtype=first.dtype, device=first.device)
+    dg1 = torch.empty((cols,), dtype=torch.float32, device=first.device) if gamma_post is not None else None
+    dg2 = torch.empty((cols,), dtype=torch.float32, device=first.device) if gamma_pre is not None else None
+    dgate = None
+    if gate is not None:  # a gate row that no row of x uses has a gradient of zero
+        dgate = (torch.empty if rows else torch.zeros)(gate.shape, dtype=gate.dtype, device=gate.device)
+    if cols == 0:
+        return dx, dy, dg1, dgate, dg2
+    ws, ws_bytes = None, 0
+    if rows and (dg1 is not None or dg2 is not None or dgate is not None):
+        need = ctypes.c_size_t()
+        check(lib().vbt_b200_residual_norm_backward_workspace_bytes(rows, cols, dtype_code(first.dtype), per,
+                                                                    first.device.index, ctypes.byref(need)))
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=first.device)
+        ws_bytes = need.value
+    (drv, rs_dr), (dnv, rs_dn), (yv, rs_y), (rv, rs_r) = views
+    check(lib().vbt_b200_residual_norm_backward(
+        _ptr(dx), _ptr(dy), _ptr(dg1), _ptr(dgate), _ptr(dg2), _ptr(drv), _ptr(dnv), _ptr(yv), _ptr(rv),
+        _ptr(inv_post), _ptr(inv_pre), _ptr(gamma_post), _ptr(gv), _ptr(gamma_pre), dtype_code(first.dtype), rows, cols,
+        rs_dr, rs_dn, rs_y, rs_r, rs_g, per, float(residual_scale), float(branch_scale), int(post) | 2 * int(pre),
+        _ptr(ws), ws_bytes, stream_ptr(first)))
+    return dx, dy, dg1, dgate, dg2
+
+
+class Checkpoint8:
+    """An activation kept in 8 bits: ``q`` (int8 or float8_e4m3fn, the activation's shape) and
+    ``scale`` (float32 [rows, ceil(hidden / 128)]), one scale per 128 neighbouring values of a row.
+    ``dtype`` is the activation's own, what ``checkpoint8_restore`` gives back."""
+
+    __slots__ = ("q", "scale", "fmt", "dtype")
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor, fmt: str, dtype: torch.dtype):
+        self.q, self.scale, self.fmt, self.dtype = q, scale, fmt, dtype
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def nbytes(self) -> int:
+        return self.q.numel() + 4 * self.scale.numel()
+
+
+def _q8_format(what: str, fmt: str):
+    try:
+        return _Q8_FORMATS[fmt]
+    except (KeyError, TypeError):
+        raise ValueError(f"{what}: fmt must be one of {sorted(_Q8_FORMATS)}") from None
+
+
+def _new_checkpoint(x: torch.Tensor, rows: int, cols: int, fmt: str, store: torch.dtype) -> Checkpoint8:
+    return Checkpoint8(torch.empty(x.shape, dtype=store, device=x.device),
+                       torch.empty((rows, -(-cols // Q8_GROUP)), dtype=torch.float32, device=x.device), fmt, x.dtype)
+
+
+def _held_rows(what: str, c: Checkpoint8):
+    """(rows, cols, format code) of a checkpoint, its parts checked."""
+    code, store = _q8_format(what, c.fmt)
+    cols = c.q.shape[-1] if c.q.dim() else 1
+    rows = c.q.numel() // cols if cols else 0
+    if not c.q.is_cuda or not c.scale.is_cuda:
+        raise RuntimeError(f"{what} requires CUDA tensors")
+    if c.q.dtype != store or c.scale.dtype != torch.float32 or c.dtype not in _FLOATS:
+        raise TypeError(f"{what}: not a checkpoint of format {c.fmt}")
+    if c.scale.device != c.q.device or c.scale.numel() != rows * -(-cols // Q8_GROUP) or \
+            not c.q.is_contiguous() or not c.scale.is_contiguous():
+        raise ValueError(f"{what}: the checkpoint's values and scales do not match")
+    return rows, cols, code
+
+
+def checkpoint8(x: torch.Tensor, fmt: str = "int8") -> Checkpoint8:
+    """Keeps x (float32, float16 or bfloat16) in 8 bits, ``fmt`` "int8" or "e4m3": with amax the
+    largest magnitude of 128 neighbours, scale = amax / top and q = round(x * (top / amax)), top 127 or 448.
+    A group whose amax is below 2^-119 is kept as zeros; one that holds a NaN or an infinity reads
+    back as NaN throughout."""
+    what = "checkpoint8"
+    code, store = _q8_format(what, fmt)
+    xv, rows, cols, rs = _rows_view(x, what)
+    c = _new_checkpoint(x, rows, cols, fmt, store)
+    if rows and cols:
+        check(lib().vbt_b200_checkpoint8(_ptr(c.q), _ptr(c.scale), _ptr(xv), dtype_code(x.dtype), code, rows, cols, rs,
+                                         stream_ptr(x)))
+    return c
+
+
+def checkpoint8_restore(c: Checkpoint8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The activation a checkpoint stands for, q * scale, in its own dtype or the given one."""
+    what = "checkpoint8_restore"
+    rows, cols, code = _held_rows(what, c)
+    dt = c.dtype if dtype is None else dtype
+    if dt not in _FLOATS:
+        raise TypeError(f"{what} gives float32, float16 or bfloat16")
+    out = torch.empty(c.q.shape, dtype=dt, device=c.q.device)
+    if rows and cols:
+        check(lib().vbt_b200_checkpoint8_restore(_ptr(out), _ptr(c.q), _ptr(c.scale), dtype_code(dt), code, rows, cols,
+                                                 stream_ptr(out)))
+    return out
+
+
+def rmsnorm_checkpoint8(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, eps: float = 1e-6, fmt: str = "int8"):
+    """``rmsnorm`` that also keeps its input in 8 bits, from one read of x: returns (out, inv_rms,
+    checkpoint).  The checkpoint takes x's place in ``rmsnorm_backward``."""
+    what = "rmsnorm_checkpoint8"
+    code, store = _q8_format(what, fmt)
+    xv, rows, cols, rs = _rows_view(x, what)
+    _same_device(what, x, gamma)
+    gamma = _gamma("gamma", gamma, cols)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    inv = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    c = _new_checkpoint(x, rows, cols, fmt, store)
+    if rows and cols:
+        check(lib().vbt_b200_rmsnorm_checkpoint8(_ptr(out), _ptr(inv), _ptr(c.q), _ptr(c.scale), _ptr(xv), _ptr(gamma),
+                                                 dtype_code(x.dtype), code, rows, cols, rs, float(eps), stream_ptr(x)))
+    return out, inv, c
+
+
+def _rmsnorm_backward8(grad_output: torch.Tensor, c: Checkpoint8, inv_rms: torch.Tensor,
+                       gamma: Optional[torch.Tensor]):
+    what = "rmsnorm_backward"
+    rows, cols, code = _held_rows(what, c)
+    if grad_output.shape != c.shape:
+        raise ValueError(f"{what}: grad_output and x must have the same shape")
+    if grad_output.dtype != c.dtype:
+        raise TypeError(f"{what}: grad_output and x must have the same dtype")
+    gv, _, _, rs = _rows_view(grad_output, what)
+    _same_device(what, grad_output, c.q, inv_rms, gamma)
+    inv_rms = _row_scalars("inv_rms", inv_rms, rows)
+    gamma = _gamma("gamma", gamma, cols)
+    dx = torch.empty(c.shape, dtype=c.dtype, device=c.device)
+    dgamma = torch.empty((cols,), dtype=torch.float32, device=c.device) if gamma is not None else None
+    if cols == 0:
+        return dx, dgamma
+    ws, ws_bytes = None, 0
+    if rows and dgamma is not None:
+        need = ctypes.c_size_t()
+        check(lib().vbt_b200_rmsnorm_backward8_workspace_bytes(rows, cols, dtype_code(c.dtype), c.device.index,
+                                                               ctypes.byref(need)))
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=c.device)
+        ws_bytes = need.value
+    check(lib().vbt_b200_rmsnorm_backward8(_ptr(dx), _ptr(dgamma), _ptr(gv), _ptr(c.q), _ptr(c.scale), _ptr(inv_rms),
+                                           _ptr(gamma), dtype_code(c.dtype), code, rows, cols, rs, _ptr(ws), ws_bytes,
+                                           stream_ptr(grad_output)))
+    return dx, dgamma
+
+
+def _silu_mul(gate: torch.Tensor, up: torch.Tensor, fmt: Optional[str], what: str):
+    gv, rows, cols, rs_g = _rows_view(gate, what)
+    _same_device(what, gate, up)
+    _like(what, "up", up, gate)
+    uv, _, _, rs_u = _rows_view(up, what)
+    out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    cg = cu = None
+    code = 0
+    if fmt is not None:
+        code, store = _q8_format(what, fmt)
+        cg, cu = _new_checkpoint(gate, rows, cols, fmt, store), _new_checkpoint(up, rows, cols, fmt, store)
+    if rows and cols:
+        check(lib().vbt_b200_silu_mul(_ptr(out), cg and _ptr(cg.q), cg and _ptr(cg.scale), cu and _ptr(cu.q),
+                                      cu and _ptr(cu.scale), _ptr(gv), _ptr(uv), dtype_code(gate.dtype), code, rows, cols,
+                                      rs_g, rs_u, stream_ptr(gate)))
+    return out, cg, cu
+
+
+def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """The gated activation silu(gate) * up; gate and up of one shape and dtype, rows of any stride
+    (the two halves of one projection, say)."""
+    return _silu_mul(gate, up, None, "silu_mul")[0]
+
+
+def silu_mul_checkpoint8(gate: torch.Tensor, up: torch.Tensor, fmt: str = "int8"):
+    """``silu_mul`` that also keeps both factors in 8 bits, from one read of them: returns (out,
+    gate's checkpoint, up's checkpoint) for ``silu_mul_backward``."""
+    if fmt is None:
+        raise ValueError("silu_mul_checkpoint8: fmt must be given")
+    return _silu_mul(gate, up, fmt, "silu_mul_checkpoint8")
+
+
+def silu_mul_backward(grad_output: torch.Tensor, gate, up):
+    """(grad_gate, grad_up) of ``silu_mul``; gate and up are both tensors or both checkpoints."""
+    what = "silu_mul_backward"
+    kept = isinstance(gate, Checkpoint8)
+    if kept != isinstance(up, Checkpoint8):
+        raise TypeError(f"{what}: gate and up must both be tensors or both checkpoints")
+    dv, rows, cols, rs_d = _rows_view(grad_output, what)
+    for name, t in (("gate", gate), ("up", up)):
+        _like(what, name, t, grad_output)
+    if kept:
+        if gate.fmt != up.fmt:
+            raise ValueError(f"{what}: checkpoints of two formats")
+        code = _held_rows(what, gate)[2]
+        _held_rows(what, up)
+        _same_device(what, grad_output, gate.q, up.q)
+        a, b, sa, sb, rs_g, rs_u = gate.q, up.q, gate.scale, up.scale, cols, cols
+    else:
+        _same_device(what, grad_output, gate, up)
+        a, _, _, rs_g = _rows_view(gate, what)
+        b, _, _, rs_u = _rows_view(up, what)
+        code, sa, sb = 0, None, None
+    dgate = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
+    dup = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
+    if rows and cols:
+        check(lib().vbt_b200_silu_mul_backward(_ptr(dgate), _ptr(dup), _ptr(dv), _ptr(a), _ptr(sa), _ptr(b), _ptr(sb),
+                                               dtype_code(grad_output.dtype), code, rows, cols, rs_d, rs_g, rs_u,
+                                               stream_ptr(grad_output)))
+    return dgate, dup
+
+
+def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what):
+    if not q.is_cuda:
+        raise RuntimeError(f"{what} requires CUDA tensors")
+    if q.dtype not in _FLOATS:
+        raise TypeError(f"{what} requires float32, float16 or bfloat16")
+    if q.dim() not in (3, 4):
+        raise ValueError(f"{what}: q must be [tokens, heads, dim] or [batch, tokens, heads, dim]")
+    _same_device(what, q, k, positions, inv_freq)
+    if k is not None:
+        if k.dtype != q.dtype:
+            raise TypeError(f"{what}: k is {k.dtype}, expected {q.dtype}")
+        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+            raise ValueError(f"{what}: k of shape {tuple(k.shape)} does not go with q of shape {tuple(q.shape)}")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+        raise TypeError(f"{what}: inv_freq must be float32 of shape [pairs]")
+    if positions.dtype not in (torch.int64, torch.int32, torch.float32):
+        raise TypeError(f"{what}: positions must be int64, int32 or float32")
+    half, dim = inv_freq.shape[0], q.shape[-1]
+    if 2 * half > dim:
+        raise ValueError(f"{what}: {half} pairs do not fit a head of {dim} values")
+    lead = tuple(q.shape[:-2])
+    pos = positions
+    if sections is None:
+        sections = (half,)
+        pos = pos.unsqueeze(0)
+    sections = [int(s) for s in sections]
+    if not 1 <= len(sections) <= 4 or builtins.sum(sections) != half or min(sections) < 0:
+        raise ValueError(f"{what}: 1 to 4 sections that sum to the {half} pairs are needed")
+    if pos.dim() != 1 + len(lead) or pos.shape[0] != len(sections):
+        raise ValueError(f"{what}: positions of shape {tuple(positions.shape)}; expected one of "
+                         f"{lead} per section")
+    try:
+        pos = pos.expand((len(sections),) + lead)
+    except RuntimeError:
+        raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} do not broadcast to {lead}") from None
+    inv_freq = inv_freq.contiguous()
+    batch, tokens = (1, lead[0]) if len(lead) == 1 else lead
+    ps = pos.stride() if len(lead) == 2 else (pos.stride(0), 0, pos.stride(1))
+    if out is not None:
+        if len(out) != 2 or (k is None) != (out[1] is None):
+            raise ValueError(f"{what}: out must be a pair like (q, k)")
+        for name, o, x in (("out[0]", out[0], q), ("out[1]", out[1], k)):
+            if o is None:
+                continue
+            _same_device(what, q, o)
+            _like(what, name, o, x)
+            if o.stride(-1) != 1 and o.shape[-1] > 1:
+                raise ValueError(f"{what}: {name} must have a last stride of 1")
+    res, args, keep = [], [], []
+    for i, x in enumerate((q, k)):
+        if x is None:
+            res.append(None)
+            args += [None, None, None, None, 0]
+            continue
+        if x.stride(-1) != 1 and dim > 1:
+            x = _ops.contiguous(x)
+        o = out[i] if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        res.append(o)
+        keep.append(x)
+        strides = [(0, *t.stride()[:-1]) if t.dim() == 3 else t.stride()[:-1] for t in (o, x)]
+        args += [_ptr(o), i64_array(strides[0]), _ptr(x), i64_array(strides[1]), x.shape[-2]]
+    check(lib().vbt_b200_rotary(*args, dtype_code(q.dtype), batch, tokens, dim, _ptr(pos), dtype_code(pos.dtype),
+                                i64_array(ps), _ptr(inv_freq), half, i64_array(sections), len(sections),
+                                int(interleaved), int(inverse), stream_ptr(q)))
+    return tuple(res)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
+           sections=None, interleaved: bool = False, out=None):
+    """Rotary positions on queries and keys, with one or several axes (time, height, width).
+
+    q [..., tokens, heads, dim] and k [..., tokens, kv_heads, dim] (or None), with or without a
+    leading batch dim and with any strides.  Pair i of a head turns by positions * inv_freq[i]
+    (inv_freq: float32 [pairs], 2 * pairs <= dim; values behind the pairs are copied).  With
+    ``sections`` -- how many pairs belong to each of up to four axes, in order -- positions is
+    [axes, ..., tokens], without it [..., tokens]; int64, int32 or float32, dims of size 1
+    broadcast.  A pair is (i, pairs + i), or (2i, 2i + 1) with ``interleaved``.  The angle is formed
+    in 64 bits: far positions keep it exact.  Returns (q, k) turned, dense, or written to the pair
+    ``out`` (which may be (q, k) itself)."""
+    return _rotary(q, k, positions, inv_freq, sections, interleaved, False, out, "rotary")
+
+
+def rotary_backward(grad_q: torch.Tensor, grad_k: Optional[torch.Tensor], positions: torch.Tensor,
+                    inv_freq: torch.Tensor, sections=None, interleaved: bool = False, out=None):
+    """Gradients of ``rotary``'s q and k: its outputs' gradients turned back by the same angles."""
+    return _rotary(grad_q, grad_k, positions, inv_freq, sections, interleaved, True, out, "rotary_backward")
