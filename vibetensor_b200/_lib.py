@@ -184,8 +184,14 @@ def desc(t: torch.Tensor) -> Desc:
     return Desc(t)
 
 
-def stream_ptr(t: torch.Tensor | None = None) -> ctypes.c_void_p:
+# the current stream's handle without a Stream object around it: 0.15 us a call against 2.4 us
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_ptr(t: torch.Tensor | None = None):
     """Current torch stream of the tensor's device as a cudaStream_t."""
+    if t is not None and _raw_stream is not None:
+        return _raw_stream(t.get_device())
     dev = t.device if t is not None else None
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 

@@ -8,13 +8,15 @@ tables are plain index tensors, as everywhere in ``ops``).
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
 
-from ._lib import Q8_FORMATS, check, dtype_code, i64_array, lib, stream_ptr
+from ._lib import Q8_FORMATS, check, dtype_code, lib, stream_ptr
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_I64x2 = ctypes.c_int64 * 2
 
 
 class QuantCache:
@@ -49,13 +51,12 @@ class QuantCache:
     def device(self):
         return self.k.device
 
-    def _on_device(self, what: str, *ts: Optional[torch.Tensor]) -> None:
+    def _on_device(self, what: str, *ts: torch.Tensor) -> None:
+        device = self.k.get_device()
         for t in ts:
-            if t is None:
-                continue
-            if not t.is_cuda:
-                raise RuntimeError(f"{what} requires CUDA tensors")
-            if t.device != self.device:
+            if t.get_device() != device:
+                if not t.is_cuda:
+                    raise RuntimeError(f"{what} requires CUDA tensors")
                 raise ValueError(f"{what}: operand on {t.device}, the cache is on {self.device}")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, status=None) -> None:
@@ -85,8 +86,8 @@ class QuantCache:
         slots = slots.contiguous()
         check(lib().vbt_b200_kv_cache_write(
             self.k.data_ptr(), self.k_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(), self.num_slots,
-            self.num_heads, self.head_dim, self._code, k.data_ptr(), i64_array(k.stride()[:2]), v.data_ptr(),
-            i64_array(v.stride()[:2]), dtype_code(k.dtype), slots.data_ptr(), dtype_code(slots.dtype), slots.shape[0],
+            self.num_heads, self.head_dim, self._code, k.data_ptr(), _I64x2(*k.stride()[:2]), v.data_ptr(),
+            _I64x2(*v.stride()[:2]), dtype_code(k.dtype), slots.data_ptr(), dtype_code(slots.dtype), slots.shape[0],
             self._owner.data_ptr(), status.ptr if status is not None else None, stream_ptr(self.k)))
 
     def read(self, page_table: torch.Tensor, starts: torch.Tensor, total: Optional[int] = None,
@@ -115,7 +116,7 @@ class QuantCache:
             if dtype not in _FLOATS:
                 raise TypeError(f"{what} gives float32, float16 or bfloat16")
             shape = (int(total), self.num_heads, self.head_dim)
-            ko, vo = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+            ko, vo = self.k.new_empty(shape, dtype=dtype), self.k.new_empty(shape, dtype=dtype)
         else:
             ko, vo = out
             self._on_device(what, ko, vo)

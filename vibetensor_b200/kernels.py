@@ -29,7 +29,7 @@ from typing import Optional
 import torch
 
 from . import ops as _ops
-from ._lib import Q8_FORMATS as _Q8_FORMATS, Q8_GROUP, check, dtype_code, i64_array, lib, stream_ptr
+from ._lib import Q8_FORMATS as _Q8_FORMATS, Q8_GROUP, check, dtype_code, lib, stream_ptr
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -45,6 +45,8 @@ def _rows_view(x: torch.Tensor, what: str):
         return x.reshape(1, 1), 1, 1, 1
     cols = x.shape[-1]
     rows = x.numel() // cols if cols else 0
+    if cols and x.is_contiguous():
+        return x, rows, cols, cols
     if x.dim() >= 2:
         lead_ok = x.stride(-1) == 1 or cols <= 1
         # leading dims must collapse onto one row stride
@@ -224,13 +226,20 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    device = first.get_device()
     for t in others:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} requires CUDA tensors")
-        if t.device != first.device:
+        if t is not None and t.get_device() != device:
+            if not t.is_cuda:
+                raise RuntimeError(f"{what} requires CUDA tensors")
             raise ValueError(f"{what}: operands on {first.device} and {t.device}")
+
+
+def _dense_like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _floats(x: torch.Tensor, n: int) -> torch.Tensor:
+    return x.new_empty((n,), dtype=torch.float32)
 
 
 def _like(what: str, name: str, t: torch.Tensor, x: torch.Tensor) -> None:
@@ -300,10 +309,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gamma_post: Optional[torch.T
     yv, _, _, rs_y = _rows_view(y, what)
     gamma_post, gamma_pre = _gamma("gamma_post", gamma_post, cols), _gamma("gamma_pre", gamma_pre, cols)
     gv, rs_g, per = _gate_rows(what, gate, x, rows)
-    r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre_norm else None
-    inv_post = torch.empty((rows,), dtype=torch.float32, device=x.device) if post_norm else None
-    inv_pre = torch.empty((rows,), dtype=torch.float32, device=x.device) if pre_norm else None
+    r = _dense_like(x)
+    n = _dense_like(x) if pre_norm else None
+    inv_post = _floats(x, rows) if post_norm else None
+    inv_pre = _floats(x, rows) if pre_norm else None
     if rows and cols:
         check(lib().vbt_b200_residual_norm(
             _ptr(r), _ptr(n), _ptr(inv_post), _ptr(inv_pre), _ptr(xv), _ptr(yv), _ptr(gamma_post), _ptr(gv),
@@ -348,13 +357,13 @@ def residual_norm_backward(grad_r: Optional[torch.Tensor], grad_n: Optional[torc
     inv_post, inv_pre = _row_scalars("inv_post", inv_post, rows), _row_scalars("inv_pre", inv_pre, rows)
     gamma_post, gamma_pre = _gamma("gamma_post", gamma_post, cols), _gamma("gamma_pre", gamma_pre, cols)
     gv, rs_g, per = _gate_rows(what, gate, first, rows)
-    dx = torch.empty(first.shape, dtype=first.dtype, device=first.device)
-    dy = torch.empty(first.shape, dtype=first.dtype, device=first.device)
-    dg1 = torch.empty((cols,), dtype=torch.float32, device=first.device) if gamma_post is not None else None
-    dg2 = torch.empty((cols,), dtype=torch.float32, device=first.device) if gamma_pre is not None else None
+    dx = _dense_like(first)
+    dy = _dense_like(first)
+    dg1 = _floats(first, cols) if gamma_post is not None else None
+    dg2 = _floats(first, cols) if gamma_pre is not None else None
     dgate = None
     if gate is not None:  # a gate row that no row of x uses has a gradient of zero
-        dgate = (torch.empty if rows else torch.zeros)(gate.shape, dtype=gate.dtype, device=gate.device)
+        dgate = _dense_like(gate) if rows else torch.zeros_like(gate, memory_format=torch.contiguous_format)
     if cols == 0:
         return dx, dy, dg1, dgate, dg2
     ws, ws_bytes = None, 0
@@ -362,7 +371,7 @@ def residual_norm_backward(grad_r: Optional[torch.Tensor], grad_n: Optional[torc
         need = ctypes.c_size_t()
         check(lib().vbt_b200_residual_norm_backward_workspace_bytes(rows, cols, dtype_code(first.dtype), per,
                                                                     first.device.index, ctypes.byref(need)))
-        ws = torch.empty((need.value,), dtype=torch.uint8, device=first.device)
+        ws = first.new_empty((need.value,), dtype=torch.uint8)
         ws_bytes = need.value
     (drv, rs_dr), (dnv, rs_dn), (yv, rs_y), (rv, rs_r) = views
     check(lib().vbt_b200_residual_norm_backward(
@@ -403,8 +412,8 @@ def _q8_format(what: str, fmt: str):
 
 
 def _new_checkpoint(x: torch.Tensor, rows: int, cols: int, fmt: str, store: torch.dtype) -> Checkpoint8:
-    return Checkpoint8(torch.empty(x.shape, dtype=store, device=x.device),
-                       torch.empty((rows, -(-cols // Q8_GROUP)), dtype=torch.float32, device=x.device), fmt, x.dtype)
+    return Checkpoint8(torch.empty_like(x, dtype=store, memory_format=torch.contiguous_format),
+                       x.new_empty((rows, -(-cols // Q8_GROUP)), dtype=torch.float32), fmt, x.dtype)
 
 
 def _held_rows(what: str, c: Checkpoint8):
@@ -444,7 +453,7 @@ def checkpoint8_restore(c: Checkpoint8, dtype: Optional[torch.dtype] = None) -> 
     dt = c.dtype if dtype is None else dtype
     if dt not in _FLOATS:
         raise TypeError(f"{what} gives float32, float16 or bfloat16")
-    out = torch.empty(c.q.shape, dtype=dt, device=c.q.device)
+    out = torch.empty_like(c.q, dtype=dt)
     if rows and cols:
         check(lib().vbt_b200_checkpoint8_restore(_ptr(out), _ptr(c.q), _ptr(c.scale), dtype_code(dt), code, rows, cols,
                                                  stream_ptr(out)))
@@ -459,8 +468,8 @@ def rmsnorm_checkpoint8(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, e
     xv, rows, cols, rs = _rows_view(x, what)
     _same_device(what, x, gamma)
     gamma = _gamma("gamma", gamma, cols)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    inv = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    out = _dense_like(x)
+    inv = _floats(x, rows)
     c = _new_checkpoint(x, rows, cols, fmt, store)
     if rows and cols:
         check(lib().vbt_b200_rmsnorm_checkpoint8(_ptr(out), _ptr(inv), _ptr(c.q), _ptr(c.scale), _ptr(xv), _ptr(gamma),
@@ -480,8 +489,8 @@ def _rmsnorm_backward8(grad_output: torch.Tensor, c: Checkpoint8, inv_rms: torch
     _same_device(what, grad_output, c.q, inv_rms, gamma)
     inv_rms = _row_scalars("inv_rms", inv_rms, rows)
     gamma = _gamma("gamma", gamma, cols)
-    dx = torch.empty(c.shape, dtype=c.dtype, device=c.device)
-    dgamma = torch.empty((cols,), dtype=torch.float32, device=c.device) if gamma is not None else None
+    dx = torch.empty_like(c.q, dtype=c.dtype)
+    dgamma = _floats(c.q, cols) if gamma is not None else None
     if cols == 0:
         return dx, dgamma
     ws, ws_bytes = None, 0
@@ -489,7 +498,7 @@ def _rmsnorm_backward8(grad_output: torch.Tensor, c: Checkpoint8, inv_rms: torch
         need = ctypes.c_size_t()
         check(lib().vbt_b200_rmsnorm_backward8_workspace_bytes(rows, cols, dtype_code(c.dtype), c.device.index,
                                                                ctypes.byref(need)))
-        ws = torch.empty((need.value,), dtype=torch.uint8, device=c.device)
+        ws = c.q.new_empty((need.value,), dtype=torch.uint8)
         ws_bytes = need.value
     check(lib().vbt_b200_rmsnorm_backward8(_ptr(dx), _ptr(dgamma), _ptr(gv), _ptr(c.q), _ptr(c.scale), _ptr(inv_rms),
                                            _ptr(gamma), dtype_code(c.dtype), code, rows, cols, rs, _ptr(ws), ws_bytes,
@@ -502,7 +511,7 @@ def _silu_mul(gate: torch.Tensor, up: torch.Tensor, fmt: Optional[str], what: st
     _same_device(what, gate, up)
     _like(what, "up", up, gate)
     uv, _, _, rs_u = _rows_view(up, what)
-    out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    out = _dense_like(gate)
     cg = cu = None
     code = 0
     if fmt is not None:
@@ -550,8 +559,8 @@ def silu_mul_backward(grad_output: torch.Tensor, gate, up):
         a, _, _, rs_g = _rows_view(gate, what)
         b, _, _, rs_u = _rows_view(up, what)
         code, sa, sb = 0, None, None
-    dgate = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
-    dup = torch.empty(grad_output.shape, dtype=grad_output.dtype, device=grad_output.device)
+    dgate = _dense_like(grad_output)
+    dup = _dense_like(grad_output)
     if rows and cols:
         check(lib().vbt_b200_silu_mul_backward(_ptr(dgate), _ptr(dup), _ptr(dv), _ptr(a), _ptr(sa), _ptr(b), _ptr(sb),
                                                dtype_code(grad_output.dtype), code, rows, cols, rs_d, rs_g, rs_u,
@@ -559,44 +568,58 @@ def silu_mul_backward(grad_output: torch.Tensor, gate, up):
     return dgate, dup
 
 
+_I64x3 = ctypes.c_int64 * 3
+
+
+def _head_strides(t: torch.Tensor):
+    """{batch, token, head} strides of [batch, tokens, heads, dim] or [tokens, heads, dim]."""
+    st = t.stride()
+    return _I64x3(0, st[0], st[1]) if len(st) == 3 else _I64x3(st[0], st[1], st[2])
+
+
 def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what):
     if not q.is_cuda:
         raise RuntimeError(f"{what} requires CUDA tensors")
     if q.dtype not in _FLOATS:
         raise TypeError(f"{what} requires float32, float16 or bfloat16")
-    if q.dim() not in (3, 4):
+    shape = q.shape
+    if len(shape) not in (3, 4):
         raise ValueError(f"{what}: q must be [tokens, heads, dim] or [batch, tokens, heads, dim]")
     _same_device(what, q, k, positions, inv_freq)
     if k is not None:
         if k.dtype != q.dtype:
             raise TypeError(f"{what}: k is {k.dtype}, expected {q.dtype}")
-        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
-            raise ValueError(f"{what}: k of shape {tuple(k.shape)} does not go with q of shape {tuple(q.shape)}")
+        if k.dim() != len(shape) or k.shape[:-2] != shape[:-2] or k.shape[-1] != shape[-1]:
+            raise ValueError(f"{what}: k of shape {tuple(k.shape)} does not go with q of shape {tuple(shape)}")
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
         raise TypeError(f"{what}: inv_freq must be float32 of shape [pairs]")
     if positions.dtype not in (torch.int64, torch.int32, torch.float32):
         raise TypeError(f"{what}: positions must be int64, int32 or float32")
-    half, dim = inv_freq.shape[0], q.shape[-1]
+    half, dim = inv_freq.shape[0], shape[-1]
     if 2 * half > dim:
         raise ValueError(f"{what}: {half} pairs do not fit a head of {dim} values")
-    lead = tuple(q.shape[:-2])
+    lead = tuple(shape[:-2])
     pos = positions
     if sections is None:
         sections = (half,)
         pos = pos.unsqueeze(0)
     sections = [int(s) for s in sections]
-    if not 1 <= len(sections) <= 4 or builtins.sum(sections) != half or min(sections) < 0:
+    axes = len(sections)
+    if not 1 <= axes <= 4 or builtins.sum(sections) != half or min(sections) < 0:
         raise ValueError(f"{what}: 1 to 4 sections that sum to the {half} pairs are needed")
-    if pos.dim() != 1 + len(lead) or pos.shape[0] != len(sections):
+    if pos.dim() != 1 + len(lead) or pos.shape[0] != axes:
         raise ValueError(f"{what}: positions of shape {tuple(positions.shape)}; expected one of "
                          f"{lead} per section")
-    try:
-        pos = pos.expand((len(sections),) + lead)
-    except RuntimeError:
-        raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} do not broadcast to {lead}") from None
+    if pos.shape != (axes, *lead):
+        try:
+            pos = pos.expand((axes, *lead))
+        except RuntimeError:
+            raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} do not broadcast to {lead}") from None
     inv_freq = inv_freq.contiguous()
     batch, tokens = (1, lead[0]) if len(lead) == 1 else lead
-    ps = pos.stride() if len(lead) == 2 else (pos.stride(0), 0, pos.stride(1))
+    ps = pos.stride()
+    if len(lead) == 1:
+        ps = (ps[0], 0, ps[1])
     if out is not None:
         if len(out) != 2 or (k is None) != (out[1] is None):
             raise ValueError(f"{what}: out must be a pair like (q, k)")
@@ -605,23 +628,22 @@ def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what
                 continue
             _same_device(what, q, o)
             _like(what, name, o, x)
-            if o.stride(-1) != 1 and o.shape[-1] > 1:
+            if o.stride(-1) != 1 and dim > 1:
                 raise ValueError(f"{what}: {name} must have a last stride of 1")
     res, args, keep = [], [], []
     for i, x in enumerate((q, k)):
         if x is None:
             res.append(None)
-            args += [None, None, None, None, 0]
+            args += (None, None, None, None, 0)
             continue
         if x.stride(-1) != 1 and dim > 1:
             x = _ops.contiguous(x)
-        o = out[i] if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        o = out[i] if out is not None else _dense_like(x)
         res.append(o)
         keep.append(x)
-        strides = [(0, *t.stride()[:-1]) if t.dim() == 3 else t.stride()[:-1] for t in (o, x)]
-        args += [_ptr(o), i64_array(strides[0]), _ptr(x), i64_array(strides[1]), x.shape[-2]]
+        args += (_ptr(o), _head_strides(o), _ptr(x), _head_strides(x), x.shape[-2])
     check(lib().vbt_b200_rotary(*args, dtype_code(q.dtype), batch, tokens, dim, _ptr(pos), dtype_code(pos.dtype),
-                                i64_array(ps), _ptr(inv_freq), half, i64_array(sections), len(sections),
+                                _I64x3(*ps), _ptr(inv_freq), half, (ctypes.c_int64 * axes)(*sections), axes,
                                 int(interleaved), int(inverse), stream_ptr(q)))
     return tuple(res)
 
