@@ -1,0 +1,566 @@
+// Backward of residual_norm (sm_100a):
+//
+//   G   = dr + i2 * (dn * g2) - r * i2^3 * mean(dn * g2 * r)
+//   dx  = a * G                         dg2   = sum_rows dn * r * i2
+//   dv  = b * G * gate                  dgate = sum_(rows of the gate row) b * G * y * i1 * g1
+//   dy  = i1 * dv * g1 - y * i1^3 * mean(dv * g1 * y)       dg1 = sum_rows dv * y * i1
+//
+// The second mean needs G, which needs the first.  It splits into sums that do not:
+//   sum(dv g1 y) = sum(w y (dr + i2 dn g2)) - c sum(w y r),  w = b gate g1, c = i2^3 mean(dn g2 r),
+// so a row costs one reduction of three sums.
+#include <algorithm>
+
+#include "row_tile.cuh"
+
+namespace vb {
+namespace {
+
+enum { GATE_NONE = 0, GATE_SHARED = 1, GATE_ROW = 2 };
+
+struct JoinBwdParams {
+  const void* dr;    // may be null
+  const void* dn;    // with pre
+  const void* y;     // with post, or for dgate
+  const void* r;     // with pre
+  const float* inv1;
+  const float* inv2;
+  const float* g1;
+  const void* gate;
+  const float* g2;
+  void* dx;
+  void* dy;
+  void* dgate;       // storage dtype; null to skip
+  float* ws_g1;      // [workers][cols] partial sums of dgamma_post, or null
+  float* ws_g2;      // the same of dgamma_pre
+  float* ws_gate;    // [units][cols] when a gate row's rows are cut into several units; the stream
+                     // kernel sums whole ones in [gridDim.x][cols]
+  int64_t rows, cols;
+  int64_t dr_stride, dn_stride, y_stride, r_stride, gate_stride;
+  int64_t per;       // rows of one gate row (GATE_SHARED), else all rows
+  int64_t chunk;     // rows of one unit
+  int64_t cuts;      // units per gate row
+  int64_t units;
+  float a, b;
+  int post, pre;
+  int stages;        // rows in flight, 1 or 2
+};
+
+// A worker (a warp when TPR lanes of it share a row, else the block) walks a range of neighbouring
+// units, each a run of rows that share one gate row.  Rows arrive in shared memory by asynchronous
+// copies, `stages` rows ahead; a thread reads back only what it copied itself, once for the three
+// sums and once for the outputs, so a row needs no barrier but the one of its reduction, and no
+// registers between the two passes.  w = b * gate * g1 and g2 lie beside them.
+// The sum over a unit of G * y * i1 gives the gate's gradient (times b * g1) and the unit's part of
+// dgamma_post (times b * gate).  A gate row of its own per row (GATE_ROW) is a factor of the sum.
+template <class T, int V, int TPR, int MODE>
+__global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
+  using A = RowChunks<T, V, TPR>;
+  constexpr int C = A::C, E = kRowElts;
+  constexpr int RW = TPR ? 32 / TPR : 1;                 // rows a worker takes at once
+  constexpr int ARRAYS = MODE == GATE_ROW ? 5 : 4;       // dr, dn, r, y, gate
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float4 red[2][32];
+  const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
+  const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  // a warp's part of the shared memory: w, g2, then `stages` times the arrays
+  unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + p.stages * ARRAYS * A::WARP_ARRAY);
+  unsigned char* gbuf = wbuf + A::WARP_FACTORS;
+  unsigned char* ring = gbuf + A::WARP_FACTORS;
+  auto buf = [&](int stage, int array) { return ring + stage * (ARRAYS * A::WARP_ARRAY) + array * A::WARP_ARRAY; };
+  for (int st = 0; st < p.stages; ++st)
+#pragma unroll
+    for (int a = 0; a < ARRAYS; ++a) {
+      const bool present = a == 0 ? p.dr != nullptr : a == 3 ? p.y != nullptr : a == 4 || p.pre;
+      A::zero_rest(buf(st, a), present, left);
+    }
+  const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
+  const float* g2p = p.pre && p.g2 ? p.g2 + j0 : nullptr;
+  A::fill_factors(gbuf, left, [&](int o) { return g2p ? g2p[o] : 1.f; });
+  if constexpr (MODE != GATE_SHARED) A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f); });
+
+  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  const int64_t workers = TPR ? static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  // units [u, last) of this worker; rows [row, end) of its unit
+  struct Walk {
+    int64_t u, last, row, end;
+    __device__ __forceinline__ void enter(const JoinBwdParams& q) {
+      if (u >= last) return;
+      const int64_t group = u / q.cuts;
+      row = group * q.per + (u - group * q.cuts) * q.chunk;
+      end = min(row + q.chunk, (group + 1) * q.per);
+    }
+    __device__ __forceinline__ void next(const JoinBwdParams& q) {
+      row += RW;
+      if (row >= end) { ++u; enter(q); }
+    }
+  };
+  Walk at;
+  at.u = worker * p.units / workers;
+  at.last = (worker + 1) * p.units / workers;
+  at.row = at.end = 0;
+  at.enter(p);
+  Walk ahead = at;
+  float i1_next[2] = {0.f, 0.f}, i2_next[2] = {0.f, 0.f};
+  auto fetch = [&](int stage, float& i1, float& i2) {
+    const int64_t row = ahead.row + rl;
+    if (ahead.u < ahead.last && row < ahead.end) {
+      if (p.dr) A::copy(buf(stage, 0), static_cast<const T*>(p.dr) + row * p.dr_stride + j0, left);
+      if (p.pre) {
+        A::copy(buf(stage, 1), static_cast<const T*>(p.dn) + row * p.dn_stride + j0, left);
+        A::copy(buf(stage, 2), static_cast<const T*>(p.r) + row * p.r_stride + j0, left);
+        i2 = p.inv2[row];
+      }
+      if (p.y) A::copy(buf(stage, 3), static_cast<const T*>(p.y) + row * p.y_stride + j0, left);
+      if constexpr (MODE == GATE_ROW)
+        A::copy(buf(stage, 4), static_cast<const T*>(p.gate) + row * p.gate_stride + j0, left);
+      i1 = p.post ? p.inv1[row] : 1.f;
+    }
+    copy_commit();
+    if (ahead.u < ahead.last) ahead.next(p);
+  };
+  fetch(0, i1_next[0], i2_next[0]);
+  if (p.stages == 2) fetch(1, i1_next[1], i2_next[1]);
+
+  float sum1[E], sum2[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) sum1[i] = sum2[i] = 0.f;
+  // adds the values of a worker's RW rows; every lane gets the result
+  auto over_rows = [&](float (&v)[E]) {
+    if constexpr (RW > 1) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int d = TPR; d < 32; d <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
+    }
+  };
+  const T* gate = nullptr;
+  bool first_unit = true, enter = true;
+  int phase = 0, stage = 0;
+  while (at.u < at.last) {
+    if constexpr (MODE == GATE_SHARED) {
+      if (enter) {
+        gate = static_cast<const T*>(p.gate) + at.u / p.cuts * p.gate_stride + j0;
+        A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
+      }
+    }
+    if (p.stages == 2) copy_wait<1>();
+    else copy_wait<0>();
+    const bool live = at.row + rl < at.end;
+    const int64_t row = at.row + rl;
+    const float i1 = i1_next[0], i2 = i2_next[0];
+    float s[3] = {0.f, 0.f, 0.f};
+    float up[E];  // dr + i2 dn g2, kept for the second pass
+    if (live) {
+#pragma unroll
+      for (int c = 0; c < A::N; ++c) {
+        float dr[C], dn[C], r[C], y[C], w[C], g2[C];
+        A::read(buf(stage, 0), c, dr);
+        A::read(buf(stage, 1), c, dn);
+        A::read(buf(stage, 2), c, r);
+        A::read(buf(stage, 3), c, y);
+        A::read_factors(wbuf, c, w);
+        A::read_factors(gbuf, c, g2);
+        if constexpr (MODE == GATE_ROW) {
+          float gt[C];
+          A::read(buf(stage, 4), c, gt);
+#pragma unroll
+          for (int e = 0; e < C; ++e) w[e] *= gt[e];
+        }
+#pragma unroll
+        for (int e = 0; e < C; ++e) {
+          const int i = c * C + e;
+          const float dnr = dn[e] * r[e], wy = w[e] * y[e];
+          up[i] = fmaf(i2, dn[e] * g2[e], dr[e]);
+          s[0] = fmaf(dnr, g2[e], s[0]);
+          s[1] = fmaf(wy, up[i], s[1]);
+          s[2] = fmaf(wy, r[e], s[2]);
+          sum2[i] = fmaf(dnr, i2, sum2[i]);
+        }
+      }
+    }
+    sum_row<TPR, 3>(s, red, phase);
+    const float c2 = i2 * i2 * i2 * s[0] * inv_cols;
+    const float c1 = p.post ? i1 * i1 * i1 * (s[1] - c2 * s[2]) * inv_cols : 0.f;
+    if (live) {
+      T* dx = static_cast<T*>(p.dx) + row * p.cols + j0;
+      T* dy = static_cast<T*>(p.dy) + row * p.cols + j0;
+#pragma unroll
+      for (int c = 0; c < A::N; ++c) {
+        float r[C], y[C], w[C], gt[C], ox[C], oy[C], og[C];
+        A::read(buf(stage, 2), c, r);
+        A::read(buf(stage, 3), c, y);
+        A::read_factors(wbuf, c, w);
+        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), c, gt);
+#pragma unroll
+        for (int e = 0; e < C; ++e) {
+          const int i = c * C + e;
+          const float G = fmaf(-c2, r[e], up[i]), Gi = G * i1;
+          ox[e] = p.a * G;
+          if constexpr (MODE == GATE_ROW) {
+            const float Gy = Gi * y[e];
+            og[e] = Gy * w[e];
+            sum1[i] = fmaf(Gy, gt[e], sum1[i]);
+            w[e] *= gt[e];
+          } else {
+            sum1[i] = fmaf(Gi, y[e], sum1[i]);
+          }
+          // without the norm (c1 = 0, i1 = 1) dy does not depend on y, not even on a NaN in it
+          oy[e] = p.post ? fmaf(Gi, w[e], -c1 * y[e]) : Gi * w[e];
+        }
+        A::write(dx, c, left, ox);
+        A::write(dy, c, left, oy);
+        if constexpr (MODE == GATE_ROW) {
+          if (p.dgate) A::write(static_cast<T*>(p.dgate) + row * p.cols + j0, c, left, og);
+        }
+      }
+    }
+    if (p.stages == 2) {
+      i1_next[0] = i1_next[1];
+      i2_next[0] = i2_next[1];
+      fetch(stage, i1_next[1], i2_next[1]);
+      stage ^= 1;
+    } else {
+      fetch(0, i1_next[0], i2_next[0]);
+    }
+    const int64_t unit = at.u;
+    at.next(p);
+    enter = at.u != unit;
+    if constexpr (MODE == GATE_SHARED) {
+      if (!enter) continue;
+      over_rows(sum1);
+      const int64_t group = unit / p.cuts;
+      if (rl == 0) {
+#pragma unroll
+        for (int c = 0; c < A::N; ++c) {
+          float og[C];
+#pragma unroll
+          for (int e = 0; e < C; ++e) {
+            const int o = A::off(c, e);
+            const float P = p.b * sum1[c * C + e];
+            const float Pg = o < left && g1 ? P * g1[o] : P;
+            og[e] = Pg;
+            if (o >= left) continue;
+            if (p.ws_gate) p.ws_gate[unit * p.cols + j0 + o] = Pg;
+            if (p.ws_g1) {  // the worker's running part, in its own row
+              float* part = p.ws_g1 + worker * p.cols + j0 + o;
+              *part = (first_unit ? 0.f : *part) + P * to_f(gate[o]);
+            }
+          }
+          if (p.dgate && p.ws_gate == nullptr)
+            A::write(static_cast<T*>(p.dgate) + group * p.cols + j0, c, left, og);
+        }
+      }
+      first_unit = false;
+#pragma unroll
+      for (int i = 0; i < E; ++i) sum1[i] = 0.f;
+    }
+  }
+  copy_wait<0>();
+  if constexpr (MODE != GATE_SHARED) over_rows(sum1);
+  over_rows(sum2);
+  if (rl == 0) {
+#pragma unroll
+    for (int c = 0; c < A::N; ++c)
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        if (A::off(c, e) >= left) continue;
+        const int64_t o = worker * p.cols + j0 + A::off(c, e);
+        if (p.ws_g1) {
+          if constexpr (MODE == GATE_SHARED) {
+            if (first_unit) p.ws_g1[o] = 0.f;  // a worker without rows
+          } else {
+            p.ws_g1[o] = p.b * sum1[c * C + e];
+          }
+        }
+        if (p.ws_g2) p.ws_g2[o] = sum2[c * C + e];
+      }
+  }
+}
+
+// any length and alignment: a block per unit, scalar accesses, each row read twice (again from L2);
+// the column sums live in the block's own workspace rows (a column is always the same thread's)
+template <class T, int MODE>
+__global__ void __launch_bounds__(512) residual_norm_bwd_stream_kernel(const __grid_constant__ JoinBwdParams p) {
+  constexpr int THREADS = 512;
+  __shared__ float red[2][3][THREADS / 32];
+  RowFold<THREADS, 3, THREADS> fold{red};
+  const int t = threadIdx.x;
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  float* s1 = p.ws_g1 ? p.ws_g1 + static_cast<int64_t>(blockIdx.x) * p.cols : nullptr;
+  float* s2 = p.ws_g2 ? p.ws_g2 + static_cast<int64_t>(blockIdx.x) * p.cols : nullptr;
+  for (int64_t j = t; j < p.cols; j += THREADS) {
+    if (s1) s1[j] = 0.f;
+    if (s2) s2[j] = 0.f;
+  }
+  for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+    const int64_t group = u / p.cuts;
+    const int64_t begin = group * p.per + (u - group * p.cuts) * p.chunk;
+    const int64_t end = min(begin + p.chunk, (group + 1) * p.per);
+    float* sg = MODE == GATE_SHARED && p.ws_gate ? p.ws_gate + (p.cuts > 1 ? u : blockIdx.x) * p.cols : nullptr;
+    if (sg)
+      for (int64_t j = t; j < p.cols; j += THREADS) sg[j] = 0.f;
+    for (int64_t row = begin; row < end; ++row) {
+      const T* dr = p.dr ? static_cast<const T*>(p.dr) + row * p.dr_stride : nullptr;
+      const T* dn = p.pre ? static_cast<const T*>(p.dn) + row * p.dn_stride : nullptr;
+      const T* rr = p.pre ? static_cast<const T*>(p.r) + row * p.r_stride : nullptr;
+      const T* y = p.y ? static_cast<const T*>(p.y) + row * p.y_stride : nullptr;
+      const T* gt = MODE == GATE_NONE ? nullptr
+                                      : static_cast<const T*>(p.gate) + (MODE == GATE_ROW ? row : group) * p.gate_stride;
+      const float i1 = p.post ? p.inv1[row] : 1.f;
+      const float i2 = p.pre ? p.inv2[row] : 0.f;
+      float s[3] = {0.f, 0.f, 0.f};
+      for (int64_t j = t; j < p.cols; j += THREADS) {
+        const float d = dn ? to_f(dn[j]) : 0.f, rv = rr ? to_f(rr[j]) : 0.f, yv = y ? to_f(y[j]) : 0.f;
+        float w = p.b * (p.post && p.g1 ? p.g1[j] : 1.f);
+        if (gt) w *= to_f(gt[j]);
+        const float dg = d * (p.pre && p.g2 ? p.g2[j] : 1.f), wy = w * yv;
+        s[0] = fmaf(dg, rv, s[0]);
+        s[1] = fmaf(wy, fmaf(i2, dg, dr ? to_f(dr[j]) : 0.f), s[1]);
+        s[2] = fmaf(wy, rv, s[2]);
+        if (s2) s2[j] = fmaf(d * i2, rv, s2[j]);
+      }
+      fold(s);
+      const float c2 = i2 * i2 * i2 * s[0] * inv_cols;
+      const float c1 = p.post ? i1 * i1 * i1 * (s[1] - c2 * s[2]) * inv_cols : 0.f;
+      for (int64_t j = t; j < p.cols; j += THREADS) {
+        const float d = dn ? to_f(dn[j]) : 0.f, rv = rr ? to_f(rr[j]) : 0.f, yv = y ? to_f(y[j]) : 0.f;
+        const float g1 = p.post && p.g1 ? p.g1[j] : 1.f;
+        const float G = fmaf(-c2, rv, fmaf(i2 * d, p.pre && p.g2 ? p.g2[j] : 1.f, dr ? to_f(dr[j]) : 0.f));
+        float bg = p.b * G;
+        const float hat = yv * i1, full = bg * hat;
+        const int64_t at = row * p.cols + j;
+        static_cast<T*>(p.dx)[at] = from_f<T>(p.a * G);
+        if (MODE == GATE_ROW && p.dgate) static_cast<T*>(p.dgate)[at] = from_f<T>(full * g1);
+        if (gt) bg *= to_f(gt[j]);
+        if (sg) sg[j] = fmaf(full, g1, sg[j]);
+        if (s1) s1[j] = fmaf(bg, hat, s1[j]);
+        static_cast<T*>(p.dy)[at] = from_f<T>(p.post ? fmaf(i1 * bg, g1, -c1 * yv) : bg);
+      }
+    }
+    if (sg && p.cuts == 1)
+      for (int64_t j = t; j < p.cols; j += THREADS) static_cast<T*>(p.dgate)[group * p.cols + j] = from_f<T>(sg[j]);
+  }
+}
+
+// Column sums of partial rows in a fixed order: blockIdx.y 0 and 1 fold dgamma_post and
+// dgamma_pre over the blocks' rows, the others a gate row each over its units.  A block owns a strip of 8
+// columns (one 32-byte sector per partial row); its 256 threads take 32 rows per step.
+struct JoinFoldParams {
+  float* out1;
+  float* out2;
+  void* dgate;
+  const float* ws1;
+  const float* ws2;
+  const float* ws_gate;
+  int64_t cols, parts, cuts, gates;
+  int first;  // what blockIdx.y == 0 stands for
+};
+template <class T>
+__global__ void __launch_bounds__(256) residual_norm_fold_kernel(const __grid_constant__ JoinFoldParams p) {
+  __shared__ float sm[8][8];
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x & 7);
+  for (int64_t what = blockIdx.y + p.first; what < p.gates + 2; what += gridDim.y) {
+    if ((what == 0 && !p.out1) || (what == 1 && !p.out2)) continue;
+    const float* src = what == 0 ? p.ws1 : what == 1 ? p.ws2 : p.ws_gate + (what - 2) * p.cuts * p.cols;
+    const int64_t n = what < 2 ? p.parts : p.cuts;
+    const float s = strip_sum(src, n, p.cols, sm);
+    if (threadIdx.x < 8 && c < p.cols) {
+      if (what == 0) p.out1[c] = s;
+      else if (what == 1) p.out2[c] = s;
+      else static_cast<T*>(p.dgate)[(what - 2) * p.cols + c] = from_f<T>(s);
+    }
+    __syncthreads();
+  }
+}
+
+// How the backward runs: `tpr` lanes of a warp share a row, or (0) a block of `threads` does; what does
+// not fit a block's shared memory takes the stream kernel (threads == 0).
+struct JoinShape {
+  int tpr, threads, stages, smem, per_sm;
+  int workers() const { return tpr ? threads / 32 : 1; }
+};
+constexpr int kSmemPerSm = 227 * 1024;
+inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row) {
+  JoinShape h{0, 0, 0, 0, 4};
+  const int64_t lanes = (cols + kRowElts - 1) / kRowElts;
+  if (lanes > 512) return h;
+  h.tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
+  h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
+  const int factors = 2 * kRowElts * 4, row = (gate_row ? 5 : 4) * kRowElts * elt;
+  h.stages = h.threads * (factors + 2 * row) <= kSmemPerSm - 2048 ? 2 : 1;
+  h.smem = h.threads * (factors + h.stages * row);
+  if (h.smem > kSmemPerSm - 2048) return JoinShape{0, 0, 0, 0, 4};
+  // registers allow 512 threads per SM (128 each)
+  h.per_sm = std::max(1, std::min(512 / h.threads, kSmemPerSm / (h.smem + 2048)));
+  return h;
+}
+// How the rows are cut: units of `chunk` rows, `cuts` of them per gate row.  As many units as there
+// are workers on the card, unless that leaves a worker's unit less than its rows at a time.
+struct JoinCut {
+  int64_t chunk, cuts, units, blocks, workers;
+};
+inline JoinCut join_cut(int64_t rows, int64_t per, const JoinShape& h, int sms) {
+  const int per_block = h.threads ? h.workers() : 1;
+  const int64_t groups = rows / per, most = int64_t{sms} * h.per_sm * per_block;
+  const int64_t at_once = h.tpr ? 32 / h.tpr : 1;
+  JoinCut c;
+  c.cuts = std::max<int64_t>(1, std::min<int64_t>((per + at_once - 1) / at_once, (most + groups - 1) / groups));
+  c.chunk = (per + c.cuts - 1) / c.cuts;
+  c.cuts = (per + c.chunk - 1) / c.chunk;
+  c.units = groups * c.cuts;
+  c.blocks = (std::min<int64_t>(c.units, most) + per_block - 1) / per_block;
+  c.workers = c.blocks * per_block;
+  return c;
+}
+inline size_t join_bwd_floats(const JoinCut& c, const JoinShape& h) {
+  // dgamma_post, dgamma_pre, and the gate's: a row per unit where a gate row is cut, else one per block of
+  // the stream kernel
+  return static_cast<size_t>(2 * c.workers + (c.cuts > 1 ? c.units : h.threads ? 0 : c.blocks));
+}
+
+template <class T, int V, int TPR, int MODE>
+vbt_b200_status go_join_bwd(const JoinBwdParams& p, const JoinShape& h, unsigned grid, cudaStream_t s, int device) {
+  static std::atomic<uint64_t> done{0};
+  VB_CUDA(allow_shared(residual_norm_bwd_kernel<T, V, TPR, MODE>, device, done));
+  residual_norm_bwd_kernel<T, V, TPR, MODE><<<grid, h.threads, h.smem, s>>>(p);
+  return VBT_B200_OK;
+}
+
+template <class T>
+vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg2, float* ws, cudaStream_t s, int device) {
+  constexpr int VW = 16 / sizeof(T);
+  const JoinShape h = join_bwd_shape(p.cols, sizeof(T), mode == GATE_ROW);
+  const JoinCut cut = join_cut(p.rows, p.per, h, sm_count(device));
+  p.chunk = cut.chunk; p.cuts = cut.cuts; p.units = cut.units; p.stages = h.stages;
+  const unsigned g = static_cast<unsigned>(cut.blocks);
+  float* at = ws;
+  if (dg1) { p.ws_g1 = at; at += cut.workers * p.cols; }
+  if (dg2) { p.ws_g2 = at; at += cut.workers * p.cols; }
+  const bool split_gate = mode == GATE_SHARED && p.dgate != nullptr && cut.cuts > 1;
+  // the stream kernel sums a gate row in memory even where it has all its rows
+  if (split_gate || (mode == GATE_SHARED && p.dgate != nullptr && h.threads == 0)) p.ws_gate = at;
+  const bool vec = p.cols % VW == 0 && p.dr_stride % VW == 0 && p.dn_stride % VW == 0 && p.y_stride % VW == 0 &&
+                   p.r_stride % VW == 0 && p.gate_stride % VW == 0 && a16(p.dr) && a16(p.dn) && a16(p.y) && a16(p.r) &&
+                   a16(p.gate) && a16(p.dx) && a16(p.dy) && a16(p.dgate);
+#define VB_JB(V, MODE)                                                             \
+  (h.tpr == 8    ? go_join_bwd<T, V, 8, MODE>(p, h, g, s, device)                  \
+   : h.tpr == 16 ? go_join_bwd<T, V, 16, MODE>(p, h, g, s, device)                 \
+   : h.tpr == 32 ? go_join_bwd<T, V, 32, MODE>(p, h, g, s, device)                 \
+                 : go_join_bwd<T, V, 0, MODE>(p, h, g, s, device))
+#define VB_JB_MODE(MODE)                                                           \
+  do {                                                                             \
+    if (h.threads == 0) residual_norm_bwd_stream_kernel<T, MODE><<<g, 512, 0, s>>>(p); \
+    else if (vec) VB_TRY(VB_JB(VW, MODE));                                         \
+    else VB_TRY(VB_JB(1, MODE));                                                   \
+  } while (0)
+  if (mode == GATE_NONE) VB_JB_MODE(GATE_NONE);
+  else if (mode == GATE_SHARED) VB_JB_MODE(GATE_SHARED);
+  else VB_JB_MODE(GATE_ROW);
+#undef VB_JB_MODE
+#undef VB_JB
+  VB_LAUNCH_CHECK();
+  const int threads = h.threads ? h.threads : 512;
+  int launches = 1;
+  if (dg1 || dg2 || split_gate) {
+    JoinFoldParams f{};
+    f.out1 = dg1; f.out2 = dg2; f.dgate = p.dgate;
+    f.ws1 = p.ws_g1; f.ws2 = p.ws_g2; f.ws_gate = p.ws_gate;
+    f.cols = p.cols; f.parts = cut.workers; f.cuts = cut.cuts; f.gates = split_gate ? p.rows / p.per : 0;
+    f.first = dg1 ? 0 : dg2 ? 1 : 2;
+    const int64_t ny = f.gates + 2 - f.first;
+    dim3 fg(static_cast<unsigned>((p.cols + 7) / 8), static_cast<unsigned>(std::min<int64_t>(ny, 65535)));
+    residual_norm_fold_kernel<T><<<fg, 256, 0, s>>>(f);
+    VB_LAUNCH_CHECK();
+    ++launches;
+  }
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_RESIDUAL_NORM_BACKWARD, dim3(g), dim3(threads), vec ? VW : 1,
+              static_cast<int>(cut.cuts), 0, launches, p.rows * p.cols, p.cols, 0, s);
+  return VBT_B200_OK;
+}
+
+}  // namespace
+}  // namespace vb
+
+extern "C" {
+
+vbt_b200_status vbt_b200_residual_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int32_t dtype,
+                                                                int64_t rows_per_gate, int32_t device,
+                                                                size_t* bytes) {
+  using namespace vb;
+  const char* name = "residual_norm_backward";
+  VB_ARG(bytes != nullptr, std::string(name) + ": null output");
+  VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
+  VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
+  VB_ARG(rows == 0 || (rows_per_gate > 0 && rows % rows_per_gate == 0),
+         std::string(name) + ": rows_per_gate does not divide rows");
+  *bytes = 0;
+  if (rows == 0) return VBT_B200_OK;
+  // a gate row of its own per row is no sum over rows: the rows are cut as if one gate row served all
+  const int elt = itemsize(dtype);
+  for (int gate_row = 0; gate_row < 2; ++gate_row) {  // whichever form the gate given takes
+    const JoinShape h = join_bwd_shape(cols, elt, gate_row);
+    const JoinCut c = join_cut(rows, rows_per_gate == 1 ? rows : rows_per_gate, h, sm_count(device));
+    *bytes = std::max(*bytes, join_bwd_floats(c, h) * static_cast<size_t>(cols) * 4);
+  }
+  return VBT_B200_OK;
+}
+
+vbt_b200_status vbt_b200_residual_norm_backward(
+    void* dx, void* dy, float* dgamma_post, void* dgate, float* dgamma_pre, const void* dr, const void* dn,
+    const void* y, const void* r, const float* inv_post, const float* inv_pre, const float* gamma_post,
+    const void* gate, const float* gamma_pre, int32_t dtype, int64_t rows, int64_t cols, int64_t dr_row_stride,
+    int64_t dn_row_stride, int64_t y_row_stride, int64_t r_row_stride, int64_t gate_row_stride,
+    int64_t rows_per_gate, float residual_scale, float branch_scale, int32_t flags, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  using namespace vb;
+  const char* name = "residual_norm_backward";
+  VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
+  VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
+  const bool pre = flags & VBT_B200_RESNORM_PRE, post = flags & VBT_B200_RESNORM_POST;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cols == 0) return VBT_B200_OK;
+  VB_ARG(dgate == nullptr || gate != nullptr, std::string(name) + ": dgate without a gate");
+  VB_ARG(dgamma_post == nullptr || post, std::string(name) + ": dgamma_post without the norm behind the branch");
+  VB_ARG(dgamma_pre == nullptr || pre, std::string(name) + ": dgamma_pre without the norm in front of the next block");
+  VB_ARG(gate == nullptr || (rows_per_gate > 0 && rows % rows_per_gate == 0),
+         std::string(name) + ": rows_per_gate does not divide rows");
+  if (rows == 0) {  // sums over no rows; a gate shared by no rows has no gradient rows either
+    for (float* o : {dgamma_post, dgamma_pre})
+      if (o) {
+        DeviceScope scope(o);
+        VB_CUDA(cudaMemsetAsync(o, 0, static_cast<size_t>(cols) * 4, s));
+      }
+    return VBT_B200_OK;
+  }
+  VB_ARG(dx && dy && (dn || dr), std::string(name) + ": null pointer");
+  VB_ARG(!pre || (dn && r && inv_pre), std::string(name) + ": the norm in front of the next block needs dn, r and inv_pre");
+  VB_ARG(!post || (y && inv_post), std::string(name) + ": the norm behind the branch needs y and inv_post");
+  VB_ARG(dgate == nullptr || y != nullptr, std::string(name) + ": dgate needs y");
+  VB_ARG(dr_row_stride >= 0 && dn_row_stride >= 0 && y_row_stride >= 0 && r_row_stride >= 0 && gate_row_stride >= 0,
+         std::string(name) + ": negative row stride");
+  DeviceScope scope(dx);
+  const int mode = gate == nullptr ? GATE_NONE : rows_per_gate == 1 && rows > 1 ? GATE_ROW : GATE_SHARED;
+  size_t need = 0;
+  VB_TRY(vbt_b200_residual_norm_backward_workspace_bytes(rows, cols, dtype, gate ? rows_per_gate : rows, scope.device(), &need));
+  VB_ARG((dgamma_post == nullptr && dgamma_pre == nullptr && dgate == nullptr) ||
+             (workspace != nullptr && workspace_bytes >= need),
+         std::string(name) + ": workspace too small (see vbt_b200_residual_norm_backward_workspace_bytes)");
+  JoinBwdParams p{};
+  p.dr = dr; p.dn = pre ? dn : nullptr; p.y = y; p.r = pre ? r : nullptr;
+  p.inv1 = inv_post; p.inv2 = inv_pre; p.g1 = gamma_post; p.gate = gate; p.g2 = gamma_pre;
+  p.dx = dx; p.dy = dy; p.dgate = dgate;
+  p.rows = rows; p.cols = cols;
+  p.dr_stride = dr ? dr_row_stride : 0; p.dn_stride = pre ? dn_row_stride : 0; p.y_stride = y ? y_row_stride : 0;
+  p.r_stride = pre ? r_row_stride : 0; p.gate_stride = gate ? gate_row_stride : 0;
+  p.per = mode == GATE_SHARED ? rows_per_gate : rows;
+  p.a = residual_scale; p.b = branch_scale; p.post = post; p.pre = pre;
+  float* ws = static_cast<float*>(workspace);
+  switch (dtype) {
+    case VBT_B200_F32: return launch_join_bwd<float>(p, mode, dgamma_post, dgamma_pre, ws, s, scope.device());
+    case VBT_B200_F16: return launch_join_bwd<__half>(p, mode, dgamma_post, dgamma_pre, ws, s, scope.device());
+    default: return launch_join_bwd<__nv_bfloat16>(p, mode, dgamma_post, dgamma_pre, ws, s, scope.device());
+  }
+}
+
+}  // extern "C"
