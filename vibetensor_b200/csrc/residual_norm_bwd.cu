@@ -42,7 +42,6 @@ struct JoinBwdParams {
   int64_t units;
   float a, b;
   int post, pre;
-  int stages;        // rows in flight, 1 or 2
 };
 
 // A worker (a warp when TPR lanes of it share a row, else the block) walks a range of neighbouring
@@ -52,10 +51,13 @@ struct JoinBwdParams {
 // registers between the two passes.  w = b * gate * g1 and g2 lie beside them.
 // The sum over a unit of G * y * i1 gives the gate's gradient (times b * g1) and the unit's part of
 // dgamma_post (times b * gate).  A gate row of its own per row (GATE_ROW) is a factor of the sum.
-template <class T, int V, int TPR, int MODE>
-__global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
-  using A = RowChunks<T, V, TPR>;
-  constexpr int C = A::C, E = kRowElts;
+constexpr int kBwdElts = 16;        // values of a row per thread
+constexpr int kBwdMaxThreads = 512;   // of a block that shares a row
+
+template <class T, int V, int TPR, int MODE, int STAGES>
+__global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
+  using A = RowChunks<T, V, TPR, kBwdElts>;
+  constexpr int C = A::C, E = kBwdElts;
   constexpr int RW = TPR ? 32 / TPR : 1;                 // rows a worker takes at once
   constexpr int ARRAYS = MODE == GATE_ROW ? 5 : 4;       // dr, dn, r, y, gate
   extern __shared__ __align__(16) unsigned char smem[];
@@ -64,11 +66,11 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) residual_norm_bw
   const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
   // a warp's part of the shared memory: w, g2, then `stages` times the arrays
-  unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + p.stages * ARRAYS * A::WARP_ARRAY);
+  unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY);
   unsigned char* gbuf = wbuf + A::WARP_FACTORS;
   unsigned char* ring = gbuf + A::WARP_FACTORS;
   auto buf = [&](int stage, int array) { return ring + stage * (ARRAYS * A::WARP_ARRAY) + array * A::WARP_ARRAY; };
-  for (int st = 0; st < p.stages; ++st)
+  for (int st = 0; st < STAGES; ++st)
 #pragma unroll
     for (int a = 0; a < ARRAYS; ++a) {
       const bool present = a == 0 ? p.dr != nullptr : a == 3 ? p.y != nullptr : a == 4 || p.pre;
@@ -81,46 +83,67 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) residual_norm_bw
 
   const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   const int64_t workers = TPR ? static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) : gridDim.x;
-  // units [u, last) of this worker; rows [row, end) of its unit
+  // the worker's units [u, last) are one run of rows; a unit's rows are taken RW at a time
   struct Walk {
-    int64_t u, last, row, end;
+    int64_t u;
+    int todo, left;  // rows of the worker, rows of the unit still to take
     __device__ __forceinline__ void enter(const JoinBwdParams& q) {
-      if (u >= last) return;
-      const int64_t group = u / q.cuts;
-      row = group * q.per + (u - group * q.cuts) * q.chunk;
-      end = min(row + q.chunk, (group + 1) * q.per);
+      const int64_t cut = u % q.cuts;
+      left = static_cast<int>(min(q.chunk, q.per - cut * q.chunk));
     }
-    __device__ __forceinline__ void next(const JoinBwdParams& q) {
-      row += RW;
-      if (row >= end) { ++u; enter(q); }
+    // takes the next rows; returns how many
+    __device__ __forceinline__ int next(const JoinBwdParams& q) {
+      const int n = RW == 1 ? 1 : min(RW, left);
+      todo -= n;
+      left -= n;
+      if (left == 0 && todo > 0) { ++u; enter(q); }
+      return n;
     }
   };
+  const int64_t u0 = worker * p.units / workers, u1 = (worker + 1) * p.units / workers;
+  auto first_row = [&](int64_t u) {
+    const int64_t group = u / p.cuts;
+    return group * p.per + (u - group * p.cuts) * p.chunk;
+  };
+  const int64_t row0 = first_row(u0) + rl;
   Walk at;
-  at.u = worker * p.units / workers;
-  at.last = (worker + 1) * p.units / workers;
-  at.row = at.end = 0;
-  at.enter(p);
+  at.u = u0;
+  at.left = 0;
+  at.todo = u0 < u1 ? static_cast<int>(first_row(u1) - first_row(u0)) : 0;
+  if (at.todo) at.enter(p);
   Walk ahead = at;
-  float i1_next[2] = {0.f, 0.f}, i2_next[2] = {0.f, 0.f};
+  const T* dr_at = static_cast<const T*>(p.dr) + row0 * p.dr_stride + j0;
+  const T* dn_at = static_cast<const T*>(p.dn) + row0 * p.dn_stride + j0;
+  const T* r_at = static_cast<const T*>(p.r) + row0 * p.r_stride + j0;
+  const T* y_at = static_cast<const T*>(p.y) + row0 * p.y_stride + j0;
+  const T* gate_at = static_cast<const T*>(p.gate) + row0 * p.gate_stride + j0;  // GATE_ROW
+  const float* inv1_at = p.inv1 + row0;
+  const float* inv2_at = p.inv2 + row0;
+  float i1_next[STAGES], i2_next[STAGES];
   auto fetch = [&](int stage, float& i1, float& i2) {
-    const int64_t row = ahead.row + rl;
-    if (ahead.u < ahead.last && row < ahead.end) {
-      if (p.dr) A::copy(buf(stage, 0), static_cast<const T*>(p.dr) + row * p.dr_stride + j0, left);
-      if (p.pre) {
-        A::copy(buf(stage, 1), static_cast<const T*>(p.dn) + row * p.dn_stride + j0, left);
-        A::copy(buf(stage, 2), static_cast<const T*>(p.r) + row * p.r_stride + j0, left);
-        i2 = p.inv2[row];
+    i1 = 1.f;
+    i2 = 0.f;
+    if (ahead.todo > 0) {
+      if (RW == 1 || rl < ahead.left) {
+        if (p.dr) A::copy(buf(stage, 0), dr_at, left);
+        if (p.pre) {
+          A::copy(buf(stage, 1), dn_at, left);
+          A::copy(buf(stage, 2), r_at, left);
+          i2 = *inv2_at;
+        }
+        if (p.y) A::copy(buf(stage, 3), y_at, left);
+        if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), gate_at, left);
+        if (p.post) i1 = *inv1_at;
       }
-      if (p.y) A::copy(buf(stage, 3), static_cast<const T*>(p.y) + row * p.y_stride + j0, left);
-      if constexpr (MODE == GATE_ROW)
-        A::copy(buf(stage, 4), static_cast<const T*>(p.gate) + row * p.gate_stride + j0, left);
-      i1 = p.post ? p.inv1[row] : 1.f;
+      const int n = ahead.next(p);
+      dr_at += n * p.dr_stride; dn_at += n * p.dn_stride; r_at += n * p.r_stride; y_at += n * p.y_stride;
+      if constexpr (MODE == GATE_ROW) gate_at += n * p.gate_stride;
+      inv1_at += n; inv2_at += n;
     }
     copy_commit();
-    if (ahead.u < ahead.last) ahead.next(p);
   };
-  fetch(0, i1_next[0], i2_next[0]);
-  if (p.stages == 2) fetch(1, i1_next[1], i2_next[1]);
+#pragma unroll
+  for (int q = 0; q < STAGES; ++q) fetch(q, i1_next[q], i2_next[q]);
 
   float sum1[E], sum2[E];
 #pragma unroll
@@ -135,19 +158,20 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) residual_norm_bw
     }
   };
   const T* gate = nullptr;
+  T* dx = static_cast<T*>(p.dx) + row0 * p.cols + j0;
+  T* dy = static_cast<T*>(p.dy) + row0 * p.cols + j0;
+  T* dgate = static_cast<T*>(p.dgate) + row0 * p.cols + j0;  // GATE_ROW
   bool first_unit = true, enter = true;
   int phase = 0, stage = 0;
-  while (at.u < at.last) {
+  while (at.todo > 0) {
     if constexpr (MODE == GATE_SHARED) {
       if (enter) {
         gate = static_cast<const T*>(p.gate) + at.u / p.cuts * p.gate_stride + j0;
         A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
       }
     }
-    if (p.stages == 2) copy_wait<1>();
-    else copy_wait<0>();
-    const bool live = at.row + rl < at.end;
-    const int64_t row = at.row + rl;
+    copy_wait<STAGES - 1>();
+    const bool live = RW == 1 || rl < at.left;
     const float i1 = i1_next[0], i2 = i2_next[0];
     float s[3] = {0.f, 0.f, 0.f};
     float up[E];  // dr + i2 dn g2, kept for the second pass
@@ -183,8 +207,6 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) residual_norm_bw
     const float c2 = i2 * i2 * i2 * s[0] * inv_cols;
     const float c1 = p.post ? i1 * i1 * i1 * (s[1] - c2 * s[2]) * inv_cols : 0.f;
     if (live) {
-      T* dx = static_cast<T*>(p.dx) + row * p.cols + j0;
-      T* dy = static_cast<T*>(p.dy) + row * p.cols + j0;
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float r[C], y[C], w[C], gt[C], ox[C], oy[C], og[C];
@@ -211,21 +233,21 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) residual_norm_bw
         A::write(dx, c, left, ox);
         A::write(dy, c, left, oy);
         if constexpr (MODE == GATE_ROW) {
-          if (p.dgate) A::write(static_cast<T*>(p.dgate) + row * p.cols + j0, c, left, og);
+          if (p.dgate) A::write(dgate, c, left, og);
         }
       }
     }
-    if (p.stages == 2) {
-      i1_next[0] = i1_next[1];
-      i2_next[0] = i2_next[1];
-      fetch(stage, i1_next[1], i2_next[1]);
-      stage ^= 1;
-    } else {
-      fetch(0, i1_next[0], i2_next[0]);
+#pragma unroll
+    for (int q = 0; q + 1 < STAGES; ++q) {
+      i1_next[q] = i1_next[q + 1];
+      i2_next[q] = i2_next[q + 1];
     }
+    fetch(stage, i1_next[STAGES - 1], i2_next[STAGES - 1]);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
     const int64_t unit = at.u;
-    at.next(p);
-    enter = at.u != unit;
+    const int n = at.next(p);
+    dx += n * p.cols; dy += n * p.cols; dgate += n * p.cols;
+    enter = at.todo == 0 || at.u != unit;
     if constexpr (MODE == GATE_SHARED) {
       if (!enter) continue;
       over_rows(sum1);
@@ -380,17 +402,18 @@ struct JoinShape {
   int tpr, threads, stages, smem, per_sm;
   int workers() const { return tpr ? threads / 32 : 1; }
 };
-constexpr int kSmemPerSm = 227 * 1024;
+constexpr int kSmemPerSm = 228 * 1024;      // of which every block takes 1 KB for the system
+constexpr int kSmemPerBlock = 226 * 1024;   // beside the reduction's 1 KB
 inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row) {
   JoinShape h{0, 0, 0, 0, 4};
-  const int64_t lanes = (cols + kRowElts - 1) / kRowElts;
-  if (lanes > 512) return h;
+  const int64_t lanes = (cols + kBwdElts - 1) / kBwdElts;
+  if (lanes > kBwdMaxThreads) return h;
   h.tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
   h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
-  const int factors = 2 * kRowElts * 4, row = (gate_row ? 5 : 4) * kRowElts * elt;
-  h.stages = h.threads * (factors + 2 * row) <= kSmemPerSm - 2048 ? 2 : 1;
+  const int factors = 2 * kBwdElts * 4, row = (gate_row ? 5 : 4) * kBwdElts * elt;
+  h.stages = h.threads * (factors + 2 * row) <= kSmemPerBlock ? 2 : 1;
   h.smem = h.threads * (factors + h.stages * row);
-  if (h.smem > kSmemPerSm - 2048) return JoinShape{0, 0, 0, 0, 4};
+  if (h.smem > kSmemPerBlock) return JoinShape{0, 0, 0, 0, 4};
   // registers allow 512 threads per SM (128 each)
   h.per_sm = std::max(1, std::min(512 / h.threads, kSmemPerSm / (h.smem + 2048)));
   return h;
@@ -419,11 +442,11 @@ inline size_t join_bwd_floats(const JoinCut& c, const JoinShape& h) {
   return static_cast<size_t>(2 * c.workers + (c.cuts > 1 ? c.units : h.threads ? 0 : c.blocks));
 }
 
-template <class T, int V, int TPR, int MODE>
+template <class T, int V, int TPR, int MODE, int STAGES>
 vbt_b200_status go_join_bwd(const JoinBwdParams& p, const JoinShape& h, unsigned grid, cudaStream_t s, int device) {
   static std::atomic<uint64_t> done{0};
-  VB_CUDA(allow_shared(residual_norm_bwd_kernel<T, V, TPR, MODE>, device, done));
-  residual_norm_bwd_kernel<T, V, TPR, MODE><<<grid, h.threads, h.smem, s>>>(p);
+  VB_CUDA(allow_shared(residual_norm_bwd_kernel<T, V, TPR, MODE, STAGES>, device, done));
+  residual_norm_bwd_kernel<T, V, TPR, MODE, STAGES><<<grid, h.threads, h.smem, s>>>(p);
   return VBT_B200_OK;
 }
 
@@ -432,7 +455,7 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
   constexpr int VW = 16 / sizeof(T);
   const JoinShape h = join_bwd_shape(p.cols, sizeof(T), mode == GATE_ROW);
   const JoinCut cut = join_cut(p.rows, p.per, h, sm_count(device));
-  p.chunk = cut.chunk; p.cuts = cut.cuts; p.units = cut.units; p.stages = h.stages;
+  p.chunk = cut.chunk; p.cuts = cut.cuts; p.units = cut.units;
   const unsigned g = static_cast<unsigned>(cut.blocks);
   float* at = ws;
   if (dg1) { p.ws_g1 = at; at += cut.workers * p.cols; }
@@ -444,10 +467,11 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
                    p.r_stride % VW == 0 && p.gate_stride % VW == 0 && a16(p.dr) && a16(p.dn) && a16(p.y) && a16(p.r) &&
                    a16(p.gate) && a16(p.dx) && a16(p.dy) && a16(p.dgate);
 #define VB_JB(V, MODE)                                                             \
-  (h.tpr == 8    ? go_join_bwd<T, V, 8, MODE>(p, h, g, s, device)                  \
-   : h.tpr == 16 ? go_join_bwd<T, V, 16, MODE>(p, h, g, s, device)                 \
-   : h.tpr == 32 ? go_join_bwd<T, V, 32, MODE>(p, h, g, s, device)                 \
-                 : go_join_bwd<T, V, 0, MODE>(p, h, g, s, device))
+  (h.tpr == 8      ? go_join_bwd<T, V, 8, MODE, 2>(p, h, g, s, device)             \
+   : h.tpr == 16   ? go_join_bwd<T, V, 16, MODE, 2>(p, h, g, s, device)            \
+   : h.tpr == 32   ? go_join_bwd<T, V, 32, MODE, 2>(p, h, g, s, device)            \
+   : h.stages == 2 ? go_join_bwd<T, V, 0, MODE, 2>(p, h, g, s, device)             \
+                   : go_join_bwd<T, V, 0, MODE, 1>(p, h, g, s, device))
 #define VB_JB_MODE(MODE)                                                           \
   do {                                                                             \
     if (h.threads == 0) residual_norm_bwd_stream_kernel<T, MODE><<<g, 512, 0, s>>>(p); \
@@ -516,6 +540,7 @@ vbt_b200_status vbt_b200_residual_norm_backward(
   using namespace vb;
   const char* name = "residual_norm_backward";
   VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
+  VB_ARG(rows < (int64_t{1} << 36), std::string(name) + ": too many rows");
   VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
   const bool pre = flags & VBT_B200_RESNORM_PRE, post = flags & VBT_B200_RESNORM_POST;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -116,22 +116,21 @@ __device__ __forceinline__ void narrow2(__nv_bfloat16* p, float2 v) {
 }
 __device__ __forceinline__ void narrow2(__half* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
 
-// A thread's 16 values of a row, worked on in chunks of C: V neighbours for V-value vectors, two
+// A thread's E values of a row, worked on in chunks of C: V neighbours for V-value vectors, two
 // single values for V = 1.  TPR lanes of a warp share a row, or (TPR = 0) every warp of the block owns
-// 512 neighbouring values of it; either way the columns of a thread's chunks and their places in
+// 32 E neighbouring values of it; either way the columns of a thread's chunks and their places in
 // shared memory are compile-time offsets from one base.  A thread has slots of its own in every
 // buffer: what it copied it may read after its own wait, without a barrier.
-constexpr int kRowElts = 16;
-template <class T, int V, int TPR> struct RowChunks {
+template <class T, int V, int TPR, int E> struct RowChunks {
   static constexpr int C = V > 1 ? V : 2;
-  static constexpr int N = kRowElts / C;
+  static constexpr int N = E / C;
   static constexpr int STEP = TPR ? TPR : 32;
-  static constexpr int WARP_ARRAY = 32 * kRowElts * static_cast<int>(sizeof(T));  // bytes of one array in a warp's part
-  static constexpr int WARP_FACTORS = 32 * kRowElts * 4;
+  static constexpr int WARP_ARRAY = 32 * E * static_cast<int>(sizeof(T));  // bytes of one array in a warp's part
+  static constexpr int WARP_FACTORS = 32 * E * 4;
   static constexpr int FW = C >= 4 ? 4 : 2;  // fp32 factors per access
   // first column of this thread
   static __device__ __forceinline__ int base() {
-    return TPR ? static_cast<int>(threadIdx.x % STEP) * V : static_cast<int>(threadIdx.x >> 5) * (32 * kRowElts) + static_cast<int>(threadIdx.x & 31) * V;
+    return TPR ? static_cast<int>(threadIdx.x % STEP) * V : static_cast<int>(threadIdx.x >> 5) * (32 * E) + static_cast<int>(threadIdx.x & 31) * V;
   }
   // offset of element e of chunk c from it
   static __device__ __forceinline__ constexpr int off(int c, int e) { return V > 1 ? c * STEP * V + e : (2 * c + e) * STEP; }
@@ -154,12 +153,12 @@ template <class T, int V, int TPR> struct RowChunks {
       }
     }
     if constexpr (V == 1 && sizeof(T) == 2) {
-      T v[kRowElts];
+      T v[E];
 #pragma unroll
-      for (int i = 0; i < kRowElts; ++i)
+      for (int i = 0; i < E; ++i)
         if (i * STEP < left) v[i] = row[i * STEP];
 #pragma unroll
-      for (int i = 0; i < kRowElts; ++i)
+      for (int i = 0; i < E; ++i)
         if (i * STEP < left) *slot(array, i / 2, i & 1) = v[i];
     }
   }
@@ -250,7 +249,7 @@ __device__ __forceinline__ void sum_row(float (&s)[N], float4 (*red)[32], int& p
 template <class Kernel> inline cudaError_t allow_shared(Kernel kernel, int device, std::atomic<uint64_t>& done) {
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 2048);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
