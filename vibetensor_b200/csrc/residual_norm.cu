@@ -26,88 +26,148 @@ struct JoinParams {
   int64_t rows, cols;
   int64_t x_stride, y_stride, gate_stride;  // elements
   int64_t per;                              // rows that share a gate row
-  FastDiv per_div;                          // the same when rows < 2^31
-  int small_rows;
+  int64_t chunk;                            // rows of a worker
   float a, b, eps;
   int post, pre;
 };
 
 __device__ __forceinline__ int64_t gate_row(const JoinParams& p, int64_t row) {
-  return p.small_rows ? static_cast<int64_t>(p.per_div.div(static_cast<uint32_t>(row))) : row / p.per;
+  return row / p.per;
 }
 
-// TPR threads per row, VPL vectors of V elements per thread, rows in registers: x and y are read
-// once, r and n written once.
-template <class T, int V, int VPL, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(const __grid_constant__ JoinParams p) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
-  constexpr int R = THREADS / TPR;
-  __shared__ float red[2][1][THREADS / 32];
-  RowFold<TPR, 1, THREADS> fold{red};
-  const int rl = threadIdx.x / TPR, tl = threadIdx.x % TPR;
-  const int nvec = static_cast<int>(p.cols / V);
-  // every thread of a block makes the same number of rounds (barriers inside)
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * R; r0 < p.rows; r0 += static_cast<int64_t>(gridDim.x) * R) {
-    const bool live = r0 + rl < p.rows;
-    const int64_t row = live ? r0 + rl : 0;
-    const int nv = live ? nvec : 0;
-    Vec<T, V> x[VPL], y[VPL], gt[VPL];
-    load_vecs<T, V, VPL>(static_cast<const T*>(p.y) + row * p.y_stride, tl, TPR, nv, y);
-    load_vecs<T, V, VPL>(static_cast<const T*>(p.x) + row * p.x_stride, tl, TPR, nv, x);
-    if (p.gate != nullptr)
-      load_vecs<T, V, VPL>(static_cast<const T*>(p.gate) + gate_row(p, row) * p.gate_stride, tl, TPR, nv, gt);
-    float s[1];
-    float i1 = 1.f;
+constexpr int kFwdElts = 16;         // values of a row per thread
+constexpr int kFwdMaxThreads = 1024;  // of a block that shares a row
+
+// A worker (a warp when TPR lanes of it share a row, else the block) walks neighbouring rows.  x, y
+// (and a gate row per row) arrive in shared memory by asynchronous copies one or two rows ahead; a
+// thread reads back only what it copied itself, so a row needs no barrier but those of its two
+// reductions.  w = b * g1 (times a shared gate row) and g2 lie beside them.
+template <class T, int V, int TPR, bool GATE_ROW, int STAGES>
+__global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) residual_norm_kernel(const __grid_constant__ JoinParams p) {
+  using A = RowChunks<T, V, TPR, kFwdElts>;
+  constexpr int C = A::C, E = kFwdElts;
+  constexpr int RW = TPR ? 32 / TPR : 1;
+  constexpr int ARRAYS = GATE_ROW ? 3 : 2;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float4 red[2][32];
+  const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
+  const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY);
+  unsigned char* gbuf = wbuf + A::WARP_FACTORS;
+  unsigned char* ring = gbuf + A::WARP_FACTORS;
+  auto buf = [&](int stage, int array) { return ring + stage * (ARRAYS * A::WARP_ARRAY) + array * A::WARP_ARRAY; };
+#pragma unroll
+  for (int st = 0; st < STAGES; ++st)
+#pragma unroll
+    for (int a = 0; a < ARRAYS; ++a) A::zero_rest(buf(st, a), true, left);
+  const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
+  const float* g2 = p.pre && p.g2 ? p.g2 + j0 : nullptr;
+
+  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  const int64_t begin = min(worker * p.chunk, p.rows);
+  const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
+  const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.x_stride + j0;
+  const T* y_at = static_cast<const T*>(p.y) + (begin + rl) * p.y_stride + j0;
+  const T* gate_at = static_cast<const T*>(p.gate) + (begin + rl) * p.gate_stride + j0;  // GATE_ROW
+  int ahead = rl;
+  auto fetch = [&](int stage) {
+    if (ahead < todo) {
+      A::copy(buf(stage, 0), y_at, left);
+      A::copy(buf(stage, 1), x_at, left);
+      if constexpr (GATE_ROW) A::copy(buf(stage, 2), gate_at, left);
+    }
+    x_at += RW * p.x_stride;
+    y_at += RW * p.y_stride;
+    if constexpr (GATE_ROW) gate_at += RW * p.gate_stride;
+    ahead += RW;
+    copy_commit();
+  };
+#pragma unroll
+  for (int st = 0; st < STAGES; ++st) fetch(st);
+  A::fill_factors(gbuf, left, [&](int o) { return g2 ? g2[o] : 1.f; });
+  if (GATE_ROW || p.gate == nullptr) A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f); });
+
+  T* r_out = static_cast<T*>(p.r) + (begin + rl) * p.cols + j0;
+  T* n_out = static_cast<T*>(p.n) + (begin + rl) * p.cols + j0;
+  int64_t group = -1, group_end = -1;  // the shared gate row that w holds, first row behind its rows
+  int phase = 0, stage = 0;
+  for (int r0 = 0; r0 < todo; r0 += RW) {
+    const bool live = RW == 1 || r0 + rl < todo;
+    const int64_t row = begin + r0 + rl;
+    if (!GATE_ROW && p.gate != nullptr && live && row >= group_end) {
+      group = row / p.per;
+      group_end = (group + 1) * p.per;
+      const T* gate = static_cast<const T*>(p.gate) + group * p.gate_stride + j0;
+      A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
+    }
+    copy_wait<STAGES - 1>();
+    float s[1] = {0.f};
+    float i1 = 1.f, i2 = 0.f;
     if (p.post) {
-      s[0] = 0.f;
+      if (live) {
 #pragma unroll
-      for (int k = 0; k < VPL; ++k)
+        for (int c = 0; c < A::N; ++c) {
+          float y[C];
+          A::read(buf(stage, 0), c, y);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[0] = fmaf(to_f(y[k].v[e]), to_f(y[k].v[e]), s[0]);
-      fold(s);
-      i1 = rsqrtf(s[0] / static_cast<float>(p.cols) + p.eps);
+          for (int e = 0; e < C; ++e) s[0] = fmaf(y[e], y[e], s[0]);
+        }
+      }
+      sum_row<TPR, 1>(s, red, phase);
+      i1 = rsqrtf(s[0] * inv_cols + p.eps);
     }
-    const float bi = p.b * i1;
-    float r[VPL][V];
+    float r[E];
     s[0] = 0.f;
+    if (live) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      float g[V];
-      load_floats<V>(p.post ? p.g1 : nullptr, tl + k * TPR, nv, g, 1.f);
+      for (int c = 0; c < A::N; ++c) {
+        float x[C], y[C], w[C];
+        A::read(buf(stage, 0), c, y);
+        A::read(buf(stage, 1), c, x);
+        A::read_factors(wbuf, c, w);
+        if constexpr (GATE_ROW) {
+          float gt[C];
+          A::read(buf(stage, 2), c, gt);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float c = bi * g[e];
-        if (p.gate != nullptr) c *= to_f(gt[k].v[e]);
-        r[k][e] = fmaf(p.a, to_f(x[k].v[e]), c * to_f(y[k].v[e]));
-        s[0] = fmaf(r[k][e], r[k][e], s[0]);
+          for (int e = 0; e < C; ++e) w[e] *= gt[e];
+        }
+#pragma unroll
+        for (int e = 0; e < C; ++e) {
+          const int i = c * C + e;
+          r[i] = fmaf(w[e] * i1, y[e], p.a * x[e]);
+          s[0] = fmaf(r[i], r[i], s[0]);
+        }
       }
     }
-    float i2 = 0.f;
+    fetch(stage);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    if (live) {
+#pragma unroll
+      for (int c = 0; c < A::N; ++c) A::write(r_out, c, left, *reinterpret_cast<const float(*)[C]>(&r[c * C]));
+    }
     if (p.pre) {
-      fold(s);
-      i2 = rsqrtf(s[0] / static_cast<float>(p.cols) + p.eps);
-    }
+      sum_row<TPR, 1>(s, red, phase);
+      i2 = rsqrtf(s[0] * inv_cols + p.eps);
+      if (live) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      const int j = tl + k * TPR;
-      if (j >= nv) continue;
-      Vec<T, V> o;
+        for (int c = 0; c < A::N; ++c) {
+          float g[C];
+          A::read_factors(gbuf, c, g);
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(r[k][e]);
-      *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.r) + row * p.cols + static_cast<int64_t>(j) * V) = o;
-      if (p.pre) {
-        float g[V];
-        load_floats<V>(p.g2, j, nv, g, 1.f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(r[k][e] * i2 * g[e]);
-        *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.n) + row * p.cols + static_cast<int64_t>(j) * V) = o;
+          for (int e = 0; e < C; ++e) g[e] *= r[c * C + e] * i2;
+          A::write(n_out, c, left, g);
+        }
       }
     }
-    if (live && tl == 0) {
+    r_out += RW * p.cols;
+    n_out += RW * p.cols;
+    if (live && j0 == 0) {
       if (p.post && p.inv1) p.inv1[row] = i1;
       if (p.pre && p.inv2) p.inv2[row] = i2;
     }
   }
+  copy_wait<0>();
 }
 
 // rows of any length and alignment: a block per row, scalar accesses, the row read once per sum
@@ -158,43 +218,51 @@ __global__ void __launch_bounds__(512) residual_norm_stream_kernel(const __grid_
   }
 }
 
+template <class T, int V, int TPR, bool GATE_ROW, int STAGES>
+vbt_b200_status go_join(JoinParams& p, int threads, int sms, unsigned& grid, cudaStream_t s, int device) {
+  static std::atomic<uint64_t> done{0};
+  VB_CUDA(allow_shared(residual_norm_kernel<T, V, TPR, GATE_ROW, STAGES>, device, done));
+  const int smem = threads * kFwdElts * (8 + STAGES * (GATE_ROW ? 3 : 2) * static_cast<int>(sizeof(T)));
+  const int per_sm = std::max(1, std::min(1024 / threads, kSmemPerSm / (smem + 2048)));
+  const int workers = TPR ? threads / 32 : 1;
+  // as many workers as fit the card at once, each with a run of rows
+  const int64_t most = int64_t{sms} * per_sm * workers;
+  p.chunk = (p.rows + most - 1) / most;
+  const int64_t used = (p.rows + p.chunk - 1) / p.chunk;
+  grid = static_cast<unsigned>((used + workers - 1) / workers);
+  residual_norm_kernel<T, V, TPR, GATE_ROW, STAGES><<<grid, threads, smem, s>>>(p);
+  return VBT_B200_OK;
+}
+
 template <class T>
-vbt_b200_status launch_join(const JoinParams& p, cudaStream_t s, int device) {
+vbt_b200_status launch_join(JoinParams p, cudaStream_t s, int device) {
   constexpr int VW = 16 / sizeof(T);
-  constexpr int E = 16;  // values of a row per thread and operand
   const int sms = sm_count(device);
   const bool vec = p.cols % VW == 0 && p.x_stride % VW == 0 && p.y_stride % VW == 0 && p.gate_stride % VW == 0 &&
-                   a16(p.x) && a16(p.y) && a16(p.gate) && a16(p.r) && a16(p.n) && a16(p.g1) && a16(p.g2);
-  auto grid = [&](int rows_per_block, int per_sm) {
-    const int64_t units = (p.rows + rows_per_block - 1) / rows_per_block;
-    return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(units, int64_t{sms} * per_sm)));
-  };
+                   a16(p.x) && a16(p.y) && a16(p.gate) && a16(p.r) && a16(p.n);
+  const bool gate_row = p.gate != nullptr && p.per == 1 && p.rows > 1;
+  const int64_t lanes = (p.cols + kFwdElts - 1) / kFwdElts;
+  const int tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
+  int threads = tpr ? 256 : static_cast<int>(std::min<int64_t>((lanes + 31) / 32 * 32, 4096));
+  // two rows ahead where they fit, else one
+  auto smem = [&](int stages) { return threads * kFwdElts * (8 + stages * (gate_row ? 3 : 2) * static_cast<int>(sizeof(T))); };
+  const int stages = smem(2) <= kSmemPerBlock ? 2 : 1;
   unsigned g = 0;
-  int threads = 256;
-#define VB_JOIN(V, TPR)                                                         \
-  do {                                                                          \
-    threads = TPR < 256 ? 256 : TPR;                                            \
-    g = grid(threads / TPR, 2048 / threads);                                    \
-    residual_norm_kernel<T, V, E / V, TPR><<<g, threads, 0, s>>>(p);            \
-  } while (0)
-#define VB_JOIN_LADDER(V)                   \
-  if (p.cols <= 8 * E) VB_JOIN(V, 8);       \
-  else if (p.cols <= 32 * E) VB_JOIN(V, 32);     \
-  else if (p.cols <= 128 * E) VB_JOIN(V, 128);   \
-  else if (p.cols <= 256 * E) VB_JOIN(V, 256);   \
-  else if (p.cols <= 512 * E) VB_JOIN(V, 512);   \
-  else VB_JOIN(V, 1024)
-  if (p.cols > 1024 * E) {
+  if (threads > kFwdMaxThreads || smem(1) > kSmemPerBlock) {
     threads = 512;
-    g = grid(1, 4);
+    g = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{sms} * 4));
     residual_norm_stream_kernel<T><<<g, threads, 0, s>>>(p);
-  } else if (vec) {
-    VB_JOIN_LADDER(VW);
   } else {
-    VB_JOIN_LADDER(1);
-  }
-#undef VB_JOIN_LADDER
+#define VB_JOIN(V, GR)                                                                 \
+  (tpr == 8      ? go_join<T, V, 8, GR, 2>(p, threads, sms, g, s, device)              \
+   : tpr == 16   ? go_join<T, V, 16, GR, 2>(p, threads, sms, g, s, device)             \
+   : tpr == 32   ? go_join<T, V, 32, GR, 2>(p, threads, sms, g, s, device)             \
+   : stages == 2 ? go_join<T, V, 0, GR, 2>(p, threads, sms, g, s, device)              \
+                 : go_join<T, V, 0, GR, 1>(p, threads, sms, g, s, device))
+    if (vec) VB_TRY(gate_row ? VB_JOIN(VW, true) : VB_JOIN(VW, false));
+    else VB_TRY(gate_row ? VB_JOIN(1, true) : VB_JOIN(1, false));
 #undef VB_JOIN
+  }
   VB_LAUNCH_CHECK();
   note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_RESIDUAL_NORM, dim3(g), dim3(threads), vec ? VW : 1, 1, 0, 1,
               p.rows * p.cols, p.cols, 0, s);
@@ -215,6 +283,7 @@ vbt_b200_status vbt_b200_residual_norm(void* r, void* n, float* inv_post, float*
   using namespace vb;
   const char* name = "residual_norm";
   VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
+  VB_ARG(rows < (int64_t{1} << 36), std::string(name) + ": too many rows");
   VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
   if (rows == 0 || cols == 0) return VBT_B200_OK;
   const bool pre = flags & VBT_B200_RESNORM_PRE, post = flags & VBT_B200_RESNORM_POST;
@@ -229,8 +298,6 @@ vbt_b200_status vbt_b200_residual_norm(void* r, void* n, float* inv_post, float*
   p.rows = rows; p.cols = cols; p.x_stride = x_row_stride; p.y_stride = y_row_stride;
   p.gate_stride = gate ? gate_row_stride : 0;
   p.per = gate ? rows_per_gate : rows;
-  p.small_rows = rows < (int64_t{1} << 31);
-  if (p.small_rows) p.per_div = FastDiv(static_cast<uint32_t>(p.per));
   p.a = residual_scale; p.b = branch_scale; p.eps = eps; p.post = post; p.pre = pre;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {

@@ -402,8 +402,6 @@ struct JoinShape {
   int tpr, threads, stages, smem, per_sm;
   int workers() const { return tpr ? threads / 32 : 1; }
 };
-constexpr int kSmemPerSm = 228 * 1024;      // of which every block takes 1 KB for the system
-constexpr int kSmemPerBlock = 226 * 1024;   // beside the reduction's 1 KB
 inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row) {
   JoinShape h{0, 0, 0, 0, 4};
   const int64_t lanes = (cols + kBwdElts - 1) / kBwdElts;

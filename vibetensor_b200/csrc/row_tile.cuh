@@ -245,11 +245,14 @@ __device__ __forceinline__ void sum_row(float (&s)[N], float4 (*red)[32], int& p
   }
 }
 
+constexpr int kSmemPerSm = 228 * 1024;     // of which every block takes 1 KB for the system
+constexpr int kSmemPerBlock = 226 * 1024;  // beside sum_row's 1 KB
+
 // Shared memory beyond the default limit has to be asked for once per kernel and device.
 template <class Kernel> inline cudaError_t allow_shared(Kernel kernel, int device, std::atomic<uint64_t>& done) {
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
