@@ -39,10 +39,12 @@ constexpr int kFwdElts = 16;         // values of a row per thread
 constexpr int kFwdMaxThreads = 1024;  // of a block that shares a row
 
 // A worker (a warp when TPR lanes of it share a row, else the block) walks neighbouring rows.  x, y
-// (and a gate row per row) arrive in shared memory by asynchronous copies one or two rows ahead; a
-// thread reads back only what it copied itself, so a row needs no barrier but those of its two
-// reductions.  w = b * g1 (times a shared gate row) and g2 lie beside them.
-template <class T, int V, int TPR, bool GATE_ROW, int STAGES>
+// (and a gate row per row) arrive in shared memory by asynchronous copies; a thread reads back only
+// what it copied itself, so a row needs no barrier but those of its two reductions, and the next
+// row's copies start as soon as r stands in registers.  w = b * g1 (times a shared gate row) and g2 lie
+// beside them.  One row per block in flight and four blocks per SM; two rows and three blocks (what
+// shared memory holds) ran [32768,4096] bf16 in 198 us against 178, three rows and two blocks in 184.
+template <class T, int V, int TPR, bool GATE_ROW>
 __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) residual_norm_kernel(const __grid_constant__ JoinParams p) {
   using A = RowChunks<T, V, TPR, kFwdElts>;
   constexpr int C = A::C, E = kFwdElts;
@@ -53,14 +55,12 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
   const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
-  unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY);
+  unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + ARRAYS * A::WARP_ARRAY);
   unsigned char* gbuf = wbuf + A::WARP_FACTORS;
   unsigned char* ring = gbuf + A::WARP_FACTORS;
-  auto buf = [&](int stage, int array) { return ring + stage * (ARRAYS * A::WARP_ARRAY) + array * A::WARP_ARRAY; };
+  auto buf = [&](int array) { return ring + array * A::WARP_ARRAY; };
 #pragma unroll
-  for (int st = 0; st < STAGES; ++st)
-#pragma unroll
-    for (int a = 0; a < ARRAYS; ++a) A::zero_rest(buf(st, a), true, left);
+  for (int a = 0; a < ARRAYS; ++a) A::zero_rest(buf(a), true, left);
   const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
   const float* g2 = p.pre && p.g2 ? p.g2 + j0 : nullptr;
 
@@ -71,11 +71,11 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
   const T* y_at = static_cast<const T*>(p.y) + (begin + rl) * p.y_stride + j0;
   const T* gate_at = static_cast<const T*>(p.gate) + (begin + rl) * p.gate_stride + j0;  // GATE_ROW
   int ahead = rl;
-  auto fetch = [&](int stage) {
+  auto fetch = [&] {
     if (ahead < todo) {
-      A::copy(buf(stage, 0), y_at, left);
-      A::copy(buf(stage, 1), x_at, left);
-      if constexpr (GATE_ROW) A::copy(buf(stage, 2), gate_at, left);
+      A::copy(buf(0), y_at, left);
+      A::copy(buf(1), x_at, left);
+      if constexpr (GATE_ROW) A::copy(buf(2), gate_at, left);
     }
     x_at += RW * p.x_stride;
     y_at += RW * p.y_stride;
@@ -83,15 +83,14 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
     ahead += RW;
     copy_commit();
   };
-#pragma unroll
-  for (int st = 0; st < STAGES; ++st) fetch(st);
+  fetch();
   A::fill_factors(gbuf, left, [&](int o) { return g2 ? g2[o] : 1.f; });
   if (GATE_ROW || p.gate == nullptr) A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f); });
 
   T* r_out = static_cast<T*>(p.r) + (begin + rl) * p.cols + j0;
   T* n_out = static_cast<T*>(p.n) + (begin + rl) * p.cols + j0;
   int64_t group = -1, group_end = -1;  // the shared gate row that w holds, first row behind its rows
-  int phase = 0, stage = 0;
+  int phase = 0;
   for (int r0 = 0; r0 < todo; r0 += RW) {
     const bool live = RW == 1 || r0 + rl < todo;
     const int64_t row = begin + r0 + rl;
@@ -101,7 +100,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
       const T* gate = static_cast<const T*>(p.gate) + group * p.gate_stride + j0;
       A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
     }
-    copy_wait<STAGES - 1>();
+    copy_wait<0>();
     float s[1] = {0.f};
     float i1 = 1.f, i2 = 0.f;
     if (p.post) {
@@ -109,7 +108,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
           float y[C];
-          A::read(buf(stage, 0), c, y);
+          A::read(buf(0), c, y);
 #pragma unroll
           for (int e = 0; e < C; ++e) s[0] = fmaf(y[e], y[e], s[0]);
         }
@@ -123,12 +122,12 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float x[C], y[C], w[C];
-        A::read(buf(stage, 0), c, y);
-        A::read(buf(stage, 1), c, x);
+        A::read(buf(0), c, y);
+        A::read(buf(1), c, x);
         A::read_factors(wbuf, c, w);
         if constexpr (GATE_ROW) {
           float gt[C];
-          A::read(buf(stage, 2), c, gt);
+          A::read(buf(2), c, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }
@@ -140,8 +139,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
         }
       }
     }
-    fetch(stage);
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    fetch();
     if (live) {
 #pragma unroll
       for (int c = 0; c < A::N; ++c) A::write(r_out, c, left, *reinterpret_cast<const float(*)[C]>(&r[c * C]));
@@ -218,11 +216,11 @@ __global__ void __launch_bounds__(512) residual_norm_stream_kernel(const __grid_
   }
 }
 
-template <class T, int V, int TPR, bool GATE_ROW, int STAGES>
+template <class T, int V, int TPR, bool GATE_ROW>
 vbt_b200_status go_join(JoinParams& p, int threads, int sms, unsigned& grid, cudaStream_t s, int device) {
   static std::atomic<uint64_t> done{0};
-  VB_CUDA(allow_shared(residual_norm_kernel<T, V, TPR, GATE_ROW, STAGES>, device, done));
-  const int smem = threads * kFwdElts * (8 + STAGES * (GATE_ROW ? 3 : 2) * static_cast<int>(sizeof(T)));
+  VB_CUDA(allow_shared(residual_norm_kernel<T, V, TPR, GATE_ROW>, device, done));
+  const int smem = threads * kFwdElts * (8 + (GATE_ROW ? 3 : 2) * static_cast<int>(sizeof(T)));
   const int per_sm = std::max(1, std::min(1024 / threads, kSmemPerSm / (smem + 2048)));
   const int workers = TPR ? threads / 32 : 1;
   // as many workers as fit the card at once, each with a run of rows
@@ -230,7 +228,7 @@ vbt_b200_status go_join(JoinParams& p, int threads, int sms, unsigned& grid, cud
   p.chunk = (p.rows + most - 1) / most;
   const int64_t used = (p.rows + p.chunk - 1) / p.chunk;
   grid = static_cast<unsigned>((used + workers - 1) / workers);
-  residual_norm_kernel<T, V, TPR, GATE_ROW, STAGES><<<grid, threads, smem, s>>>(p);
+  residual_norm_kernel<T, V, TPR, GATE_ROW><<<grid, threads, smem, s>>>(p);
   return VBT_B200_OK;
 }
 
@@ -244,21 +242,18 @@ vbt_b200_status launch_join(JoinParams p, cudaStream_t s, int device) {
   const int64_t lanes = (p.cols + kFwdElts - 1) / kFwdElts;
   const int tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
   int threads = tpr ? 256 : static_cast<int>(std::min<int64_t>((lanes + 31) / 32 * 32, 4096));
-  // two rows ahead where they fit, else one
-  auto smem = [&](int stages) { return threads * kFwdElts * (8 + stages * (gate_row ? 3 : 2) * static_cast<int>(sizeof(T))); };
-  const int stages = smem(2) <= kSmemPerBlock ? 2 : 1;
+  const int smem = threads * kFwdElts * (8 + (gate_row ? 3 : 2) * static_cast<int>(sizeof(T)));
   unsigned g = 0;
-  if (threads > kFwdMaxThreads || smem(1) > kSmemPerBlock) {
+  if (threads > kFwdMaxThreads || smem > kSmemPerBlock) {
     threads = 512;
     g = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{sms} * 4));
     residual_norm_stream_kernel<T><<<g, threads, 0, s>>>(p);
   } else {
-#define VB_JOIN(V, GR)                                                                 \
-  (tpr == 8      ? go_join<T, V, 8, GR, 2>(p, threads, sms, g, s, device)              \
-   : tpr == 16   ? go_join<T, V, 16, GR, 2>(p, threads, sms, g, s, device)             \
-   : tpr == 32   ? go_join<T, V, 32, GR, 2>(p, threads, sms, g, s, device)             \
-   : stages == 2 ? go_join<T, V, 0, GR, 2>(p, threads, sms, g, s, device)              \
-                 : go_join<T, V, 0, GR, 1>(p, threads, sms, g, s, device))
+#define VB_JOIN(V, GR)                                                           \
+  (tpr == 8    ? go_join<T, V, 8, GR>(p, threads, sms, g, s, device)             \
+   : tpr == 16 ? go_join<T, V, 16, GR>(p, threads, sms, g, s, device)            \
+   : tpr == 32 ? go_join<T, V, 32, GR>(p, threads, sms, g, s, device)            \
+               : go_join<T, V, 0, GR>(p, threads, sms, g, s, device))
     if (vec) VB_TRY(gate_row ? VB_JOIN(VW, true) : VB_JOIN(VW, false));
     else VB_TRY(gate_row ? VB_JOIN(1, true) : VB_JOIN(1, false));
 #undef VB_JOIN
