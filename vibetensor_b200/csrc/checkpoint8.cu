@@ -68,11 +68,9 @@ template <class T, bool VEC> struct Lanes {
   }
   // quantises the group: returns its stored scale
   template <int F>
-  static __device__ __forceinline__ float store_q(uint8_t* group, int lane, int len, const float (&v)[N]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) m = max(m, mag_bits(v[e]));
-    const Q8Scale s = q8_scale<F>(lanes_max<L>(m));
+  static __device__ __forceinline__ float store_q(uint8_t* group, int lane, int len, const Raw& raw, const float (&v)[N]) {
+    const Raw one[1] = {raw};
+    const Q8Scale s = q8_scale<F>(group_mag<T, N, 1, L>(one));
     if constexpr (VEC) {
       if (lane * V < len) q8_store<F, N>(group + lane * V, v, s.up);
     } else {
@@ -142,7 +140,7 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint8_kernel(const __grid_co
     float v[A::N];
 #pragma unroll
     for (int e = 0; e < A::N; ++e) v[e] = to_f(x[u].v[e]);
-    const float s = A::template store_q<F>(p.q + row[u] * p.g.cols + col[u], lane, len[u], v);
+    const float s = A::template store_q<F>(p.q + row[u] * p.g.cols + col[u], lane, len[u], x[u], v);
     if (lane == 0 && len[u]) p.scale[first + u * S] = s;
   }
 }
@@ -178,6 +176,17 @@ __global__ void __launch_bounds__(kCkThreads) restore8_kernel(const __grid_const
 // ---------------------------------------------------------------------------------------
 // gated activation
 // ---------------------------------------------------------------------------------------
+// 1 / (1 + exp(-x)).  For 16-bit storage exp(-x) is 2^(-x log2 e) on the special-function unit: the
+// rounded product is off by at most |x| 2^-23 in the exponent, 2^-18 of the value where that is
+// smallest (|x| < 40; further out the sigmoid itself is below 2^-57 or rounds to one).
+template <class T> __device__ __forceinline__ float sigmoid(float x) {
+  float e, r;
+  if constexpr (sizeof(T) == 2) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  else e = expf(-x);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
+
 struct GluParams {
   const void* dout;    // backward
   const void* gate;    // storage type, or levels
@@ -220,13 +229,13 @@ __global__ void __launch_bounds__(kCkThreads) silu_mul_kernel(const __grid_const
     for (int e = 0; e < A::N; ++e) {
       a[e] = to_f(ga[u].v[e]);
       b[e] = to_f(up[u].v[e]);
-      h[e] = a[e] / (1.f + expf(-a[e])) * b[e];
+      h[e] = a[e] * sigmoid<T>(a[e]) * b[e];
     }
     const int64_t at = row[u] * p.g.cols + col[u];
     A::store(static_cast<T*>(p.out) + at, lane, len[u], h);
     if constexpr (KEEP) {
-      const float sa = A::template store_q<F>(p.q_gate + at, lane, len[u], a);
-      const float sb = A::template store_q<F>(p.q_up + at, lane, len[u], b);
+      const float sa = A::template store_q<F>(p.q_gate + at, lane, len[u], ga[u], a);
+      const float sb = A::template store_q<F>(p.q_up + at, lane, len[u], up[u], b);
       if (lane == 0 && len[u]) {
         p.s_gate[first + u * S] = sa;
         p.s_up[first + u * S] = sb;
@@ -281,7 +290,7 @@ __global__ void __launch_bounds__(kCkThreads) silu_mul_bwd_kernel(const __grid_c
     }
 #pragma unroll
     for (int e = 0; e < A::N; ++e) {
-      const float s = 1.f / (1.f + expf(-a[e])), dv = to_f(d[u].v[e]);
+      const float s = sigmoid<T>(a[e]), dv = to_f(d[u].v[e]);
       da[e] = dv * b[e] * s * (1.f + a[e] * (1.f - s));
       db[e] = dv * a[e] * s;
     }
@@ -334,14 +343,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rmsnorm8_kernel(const _
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
       const int j = tl + k * TPR;
+      const Vec<T, V> one[1] = {x[k]};
+      const Q8Scale sc = q8_scale<F>(group_mag<T, V, 1, L>(one));
       float v[V];
-      uint32_t m = 0;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[e] = to_f(x[k].v[e]);
-        m = max(m, mag_bits(v[e]));
-      }
-      const Q8Scale sc = q8_scale<F>(lanes_max<L>(m));
+      for (int e = 0; e < V; ++e) v[e] = to_f(x[k].v[e]);
       if (j < nv) {
         q8_store<F, V>(p.q + row * p.cols + static_cast<int64_t>(j) * V, v, sc.up);
         if (tl % L == 0) p.scale[row * p.groups + j / L] = sc.down;
@@ -383,7 +389,7 @@ __global__ void __launch_bounds__(256) rmsnorm8_stream_kernel(const __grid_const
         v[e] = to_f(raw.v[e]);
         s[0] = fmaf(v[e], v[e], s[0]);
       }
-      const float sc = A::template store_q<F>(p.q + row * p.cols + g * kQ8Group, lane, len, v);
+      const float sc = A::template store_q<F>(p.q + row * p.cols + g * kQ8Group, lane, len, raw, v);
       if (lane == 0) p.scale[row * p.groups + g] = sc;
     }
     fold(s);

@@ -12,6 +12,7 @@
 #include <algorithm>
 
 #include "quant8.cuh"
+#include "row_tile.cuh"
 
 namespace vb {
 namespace {
@@ -93,31 +94,24 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const __grid_const
     const T* src = static_cast<const T*>(p.src[kv]) + (first + tok) * p.src_t[kv] + static_cast<int64_t>(h) * p.src_h[kv];
     const int64_t row = live ? slot * p.heads + h : 0;
     uint8_t* dst = p.cache[kv] + row * p.dim;
-    uint32_t m = 0;
     if constexpr (VEC) {
       const int nv = live ? p.dim / V : 0;
-      float v[VPL][V];
+      Vec<T, V> raw[VPL];
+      load_vecs<T, V, VPL>(src, lane, L, nv, raw);
+      const Q8Scale s = q8_scale<F>(group_mag<T, V, VPL, L>(raw));
 #pragma unroll
       for (int k = 0; k < VPL; ++k) {
         const int j = lane + k * L;
-        if (j < nv) {
-          const Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(src + j * V);
+        if (j >= nv) continue;
+        float v[V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            v[k][e] = to_f(raw.v[e]);
-            m = max(m, mag_bits(v[k][e]));
-          }
-        }
-      }
-      const Q8Scale s = q8_scale<F>(lanes_max<L>(m));
-#pragma unroll
-      for (int k = 0; k < VPL; ++k) {
-        const int j = lane + k * L;
-        if (j < nv) q8_store<F, V>(dst + j * V, v[k], s.up);
+        for (int e = 0; e < V; ++e) v[e] = to_f(raw[k].v[e]);
+        q8_store<F, V>(dst + j * V, v, s.up);
       }
       if (live && lane == 0) p.scale[kv][row] = s.down;
     } else {
       const int n = live ? p.dim : 0;
+      uint32_t m = 0;
       for (int j = lane; j < n; j += L) m = max(m, mag_bits(to_f(src[j])));
       const Q8Scale s = q8_scale<F>(lanes_max<L>(m));
       for (int j = lane; j < n; j += L) dst[j] = q8_pack1<F>(to_f(src[j]), s.up);
@@ -148,17 +142,35 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const __grid_consta
   __shared__ int64_t slot_of[kKvMaxTokens];  // >= 0 slot, -1 zeros, -2 leave alone
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tb;
   const int tb = static_cast<int>(min(static_cast<int64_t>(p.tb), p.rows - first));
-  if (threadIdx.x < tb) {
-    const int64_t i = first + threadIdx.x;
-    int64_t lo = 0, hi = p.seqs;  // the last s with starts[s] <= i
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (p.starts[mid] <= i) lo = mid + 1;
-      else hi = mid;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    // the sequence of the block's first row, the last s with starts[s] <= first: 32 probes at a time
+    int64_t lo = 0, n = p.seqs;  // it lies in [lo - 1, lo + n)
+    while (n > 0) {
+      const int64_t hop = (n + 31) / 32;
+      const int64_t probe = min(lo + (lane + 1) * hop, lo + n) - 1;
+      const int below = __popc(__ballot_sync(0xffffffffu, p.starts[probe] <= first));  // ascending
+      if (hop == 1) {
+        lo += min(static_cast<int64_t>(below), n);
+        break;
+      }
+      const int64_t from = below * hop;
+      lo += min(from, n);
+      n = from >= n ? 0 : min(hop, n - from) - 1;  // the last of the piece is known to lie above
     }
-    const int64_t s = lo - 1;
+    const int64_t i = first + lane;
+    int64_t s = lo - 1;
+    if (lane < tb && s + 1 < p.seqs && p.starts[s + 1] <= i) {  // a later row's own sequence
+      int64_t a = s + 1, b = p.seqs;
+      while (a < b) {
+        const int64_t mid = (a + b) >> 1;
+        if (p.starts[mid] <= i) a = mid + 1;
+        else b = mid;
+      }
+      s = a - 1;
+    }
     int64_t slot = p.fill ? -1 : -2;
-    if (s >= 0 && i < p.starts[s + 1]) {
+    if (lane < tb && s >= 0 && i < p.starts[s + 1]) {
       const int64_t pos = i - p.starts[s], pg = pos / p.page_size;
       int64_t page = -1;
       if (pg < p.pages_per_seq) page = load_index(p.table, p.table_dtype, s * p.table_stride + pg);
@@ -169,7 +181,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const __grid_consta
         count_bad(p.status, page);
       }
     }
-    slot_of[threadIdx.x] = slot;
+    if (lane < tb) slot_of[lane] = slot;
   }
   __syncthreads();
   const int total = tb * 2 * p.chunks;

@@ -11,8 +11,12 @@
 // One division per group and one multiply per value; every step is a correctly rounded fp32
 // operation, so the levels are a function of the inputs alone.  |x * fl(top / amax)| is at most
 // top * (1 + 2^-23), which rounds to top in both formats: no clamp.  A group whose amax is below
-// 2^-119 is held as zeros (top / amax would overflow).  A group that holds a NaN or an infinity has
-// a scale that is one too and zero (or NaN) levels: the whole group reads back as NaN.
+// 2^-119 is held as zeros (top / amax would overflow).  A group that holds a NaN or an infinity is
+// held as zeros with a NaN for its scale: the whole group reads back as NaN.
+//
+// The conversions between integers and floats that the hardware has run at a quarter of the rate of an
+// add, and a gated activation's pass with its two 8-bit copies was bound by them: here they are adds
+// of 1.5 * 2^23 (whose low byte is the rounded level) and byte permutes.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -36,26 +40,29 @@ struct Q8Scale {
 template <int F> __device__ __forceinline__ Q8Scale q8_scale(uint32_t amax_bits) {
   const float amax = __uint_as_float(amax_bits);
   if (amax < 0x1p-119f) return {0.0f, 0.0f};
+  if (amax_bits >= 0x7f800000u) return {0.0f, __uint_as_float(0x7fffffffu)};
   return {__fdiv_rn(q8_top<F>(), amax), __fmul_rn(amax, 1.0f / q8_top<F>())};
 }
 __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// N values (N = 1, 2, 4, 8) -> N bytes, packed little-endian in words of up to four
+// four values -> four bytes
 template <int F> __device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d, float up) {
   a = __fmul_rn(a, up); b = __fmul_rn(b, up); c = __fmul_rn(c, up); d = __fmul_rn(d, up);
+  uint32_t w;
   if constexpr (F == VBT_B200_Q8_INT8) {
-    const uint32_t ia = __float2int_rn(a), ib = __float2int_rn(b), ic = __float2int_rn(c), id = __float2int_rn(d);
-    return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's last place is 1
+    const uint32_t ia = __float_as_uint(__fadd_rn(a, kRound)), ib = __float_as_uint(__fadd_rn(b, kRound));
+    const uint32_t ic = __float_as_uint(__fadd_rn(c, kRound)), id = __float_as_uint(__fadd_rn(d, kRound));
+    w = __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
   } else {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
+    w = lo | (hi << 16);
   }
+  return up == 0.0f ? 0u : w;  // a group with a NaN or an infinity
 }
 template <int F> __device__ __forceinline__ uint8_t q8_pack1(float a, float up) {
-  a = __fmul_rn(a, up);
-  if constexpr (F == VBT_B200_Q8_INT8) return static_cast<uint8_t>(__float2int_rn(a));
-  else return static_cast<uint8_t>(__nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3));
+  return static_cast<uint8_t>(q8_pack4<F>(a, 0.f, 0.f, 0.f, up));
 }
 // four bytes -> four levels (not yet multiplied by the scale)
 template <int F> __device__ __forceinline__ void q8_levels4(uint32_t w, float (&v)[4]) {
@@ -123,6 +130,35 @@ template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t b) {
 #pragma unroll
   for (int d = LANES / 2; d > 0; d >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, d));
   return b;
+}
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+// The same from the stored values of a lane, W vectors of N.  16-bit types are compared two at a
+// time in their own bit patterns, which are ordered like the values.
+template <class T, int N, int W, int LANES>
+__device__ __forceinline__ uint32_t group_mag(const Vec<T, N> (&v)[W]) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int e = 0; e < N; e += 2) m = max_halves(m, *reinterpret_cast<const uint32_t*>(&v[k].v[e]) & 0x7fff7fffu);
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) m = max_halves(m, __shfl_xor_sync(0xffffffffu, m, d));
+    m = max(m & 0xffffu, m >> 16);
+    const uint16_t h = static_cast<uint16_t>(m);
+    return __float_as_uint(to_f(*reinterpret_cast<const T*>(&h)));
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) m = max(m, mag_bits(to_f(v[k].v[e])));
+    return lanes_max<LANES>(m);
+  }
 }
 
 }  // namespace vb
