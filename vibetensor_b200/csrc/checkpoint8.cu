@@ -87,14 +87,23 @@ struct Groups {
   int64_t total, per_row, cols;
   FastDiv div;
   int small;
-  void fill(int64_t rows, int64_t c) {
+  int flat;  // dense rows of whole groups: the groups lie one behind the other
+  // dense: every operand's row stride is the row length
+  void fill(int64_t rows, int64_t c, bool dense) {
     cols = c;
     per_row = (c + kQ8Group - 1) / kQ8Group;
     total = rows * per_row;
     small = total < (int64_t{1} << 31);
+    flat = dense && c % kQ8Group == 0;
     if (small) div = FastDiv(static_cast<uint32_t>(per_row));
   }
   __device__ __forceinline__ void find(int64_t i, int64_t& row, int64_t& col, int& len) const {
+    if (flat) {
+      row = 0;
+      col = i * kQ8Group;
+      len = kQ8Group;
+      return;
+    }
     int64_t g;
     if (small) {
       uint32_t q, r;
@@ -117,7 +126,10 @@ struct CkParams {
   Groups g;
 };
 
-constexpr int kCkThreads = 256;
+// Short blocks of one or two groups per thread: with four groups per thread (more registers, fewer
+// threads per SM) and 256 threads the 8-bit copy and its way back took 222 us for [16384,8192] bf16
+// against 152, the gated activation's two passes 409 against 376.
+constexpr int kCkThreads = 128;
 
 template <class T, bool VEC, int F, int U>
 __global__ void __launch_bounds__(kCkThreads) checkpoint8_kernel(const __grid_constant__ CkParams p) {
@@ -311,63 +323,99 @@ struct Norm8Params {
   uint8_t* q;
   float* scale;
   float* inv;
-  float* ws;           // backward: [gridDim.x][cols] partial sums of dgamma, or null
+  float* ws;           // backward: [workers][cols] partial sums of dgamma, or null
   int64_t rows, cols, groups;
+  int64_t chunk;       // rows of a worker
   int64_t stride;      // of x or dy
   float eps;
 };
 
-template <class T, int F, int VPL, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rmsnorm8_kernel(const __grid_constant__ Norm8Params p) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
-  constexpr int R = THREADS / TPR;
-  constexpr int V = 16 / sizeof(T);
-  constexpr int L = kQ8Group / V;
-  static_assert(TPR % L == 0, "a group's lanes are neighbours");
-  __shared__ float red[2][1][THREADS / 32];
-  RowFold<TPR, 1, THREADS> fold{red};
-  const int rl = threadIdx.x / TPR, tl = threadIdx.x % TPR;
-  const int nvec = static_cast<int>(p.cols / V);
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * R; r0 < p.rows; r0 += static_cast<int64_t>(gridDim.x) * R) {
-    const bool live = r0 + rl < p.rows;
-    const int64_t row = live ? r0 + rl : 0;
-    const int nv = live ? nvec : 0;
-    Vec<T, V> x[VPL];
-    load_vecs<T, V, VPL>(static_cast<const T*>(p.x) + row * p.stride, tl, TPR, nv, x);
+// Rows staged in shared memory as in residual_norm: a worker (a warp when TPR lanes of it share a row,
+// else the block) walks neighbouring rows, a thread reads back only what it copied itself.
+constexpr int kNormElts = 16;
+constexpr int kBwd8Stages = 1;  // rows in flight of the backward
+// group of 128 values that chunk c of this thread belongs to, counted from the row's start
+template <class A> __device__ __forceinline__ int chunk_group(int j0, int c) { return (j0 + A::off(c, 0)) / kQ8Group; }
+
+template <class T, int V, int TPR, int F>
+__global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel(const __grid_constant__ Norm8Params p) {
+  using A = RowChunks<T, V, TPR, kNormElts>;
+  constexpr int C = A::C;
+  constexpr int RW = TPR ? 32 / TPR : 1;
+  // chunks (of this thread) and lanes that hold one group together
+  constexpr int GC = V > 1 ? 1 : 2, GL = V > 1 ? kQ8Group / V : 32;
+  static_assert(A::STEP % GL == 0, "a group's lanes are neighbours");
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float4 red[2][32];
+  const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
+  const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  unsigned char* gbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (A::WARP_FACTORS + A::WARP_ARRAY);
+  unsigned char* xbuf = gbuf + A::WARP_FACTORS;
+  A::zero_rest(xbuf, true, left);
+  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  const int64_t begin = min(worker * p.chunk, p.rows);
+  const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
+  const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.stride + j0;
+  if (rl < todo) A::copy(xbuf, x_at, left);
+  copy_commit();
+  A::fill_factors(gbuf, left, [&](int o) { return p.gamma ? p.gamma[j0 + o] : 1.f; });
+  T* out = static_cast<T*>(p.out) + (begin + rl) * p.cols + j0;
+  uint8_t* q = p.q + (begin + rl) * p.cols + j0;
+  float* scale = p.scale + (begin + rl) * p.groups;
+  int phase = 0;
+  for (int r0 = 0; r0 < todo; r0 += RW) {
+    const bool live = RW == 1 || r0 + rl < todo;
+    copy_wait<0>();
+    float x[kNormElts];
     float s[1] = {0.f};
 #pragma unroll
-    for (int k = 0; k < VPL; ++k)
+    for (int c0 = 0; c0 < A::N; c0 += GC) {
+      Vec<T, C> raw[GC];
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[0] = fmaf(to_f(x[k].v[e]), to_f(x[k].v[e]), s[0]);
-    // the 8-bit copy needs nothing of the row's sum: its shuffles hide the wait for it
+      for (int k = 0; k < GC; ++k) {
+        A::read_raw(xbuf, c0 + k, raw[k]);
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      const int j = tl + k * TPR;
-      const Vec<T, V> one[1] = {x[k]};
-      const Q8Scale sc = q8_scale<F>(group_mag<T, V, 1, L>(one));
-      float v[V];
+        for (int e = 0; e < C; ++e) {
+          x[(c0 + k) * C + e] = to_f(raw[k].v[e]);
+          s[0] = fmaf(x[(c0 + k) * C + e], x[(c0 + k) * C + e], s[0]);
+        }
+      }
+      // the 8-bit copy needs nothing of the row's sum
+      const Q8Scale sc = q8_scale<F>(group_mag<T, C, GC, GL>(raw));
+      if (live && A::off(c0, 0) < left) {
+        if constexpr (V > 1) {
+          q8_store<F, V>(q + A::off(c0, 0), *reinterpret_cast<const float(*)[V]>(&x[c0 * C]), sc.up);
+        } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = to_f(x[k].v[e]);
-      if (j < nv) {
-        q8_store<F, V>(p.q + row * p.cols + static_cast<int64_t>(j) * V, v, sc.up);
-        if (tl % L == 0) p.scale[row * p.groups + j / L] = sc.down;
+          for (int i = 0; i < GC * C; ++i)
+            if (A::off(c0 + i / C, i % C) < left) q[A::off(c0 + i / C, i % C)] = q8_pack1<F>(x[c0 * C + i], sc.up);
+        }
+        if ((threadIdx.x & 31) % GL == 0) scale[chunk_group<A>(j0, c0)] = sc.down;
       }
     }
-    fold(s);
-    const float inv = rsqrtf(s[0] / static_cast<float>(p.cols) + p.eps);
+    x_at += RW * p.stride;
+    if (r0 + RW + rl < todo) A::copy(xbuf, x_at, left);
+    copy_commit();
+    if (!live) s[0] = 0.f;
+    sum_row<TPR, 1>(s, red, phase);
+    const float inv = rsqrtf(s[0] * inv_cols + p.eps);
+    if (live) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      const int j = tl + k * TPR;
-      if (j >= nv) continue;
-      float g[V];
-      load_floats<V>(p.gamma, j, nv, g, 1.f);
-      Vec<T, V> o;
+      for (int c = 0; c < A::N; ++c) {
+        float g[C];
+        A::read_factors(gbuf, c, g);
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(to_f(x[k].v[e]) * inv * g[e]);
-      *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.out) + row * p.cols + static_cast<int64_t>(j) * V) = o;
+        for (int e = 0; e < C; ++e) g[e] *= x[c * C + e] * inv;
+        A::write(out, c, left, g);
+      }
+      if (j0 == 0 && p.inv) p.inv[begin + r0 + rl] = inv;
     }
-    if (live && tl == 0 && p.inv) p.inv[row] = inv;
+    out += RW * p.cols;
+    q += RW * p.cols;
+    scale += RW * p.groups;
   }
+  copy_wait<0>();
 }
 
 // any length and alignment: a block per row, a warp per group
@@ -400,90 +448,133 @@ __global__ void __launch_bounds__(256) rmsnorm8_stream_kernel(const __grid_const
   }
 }
 
-template <class T, int F, int VPL, int TPR>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_bwd8_kernel(const __grid_constant__ Norm8Params p) {
-  constexpr int THREADS = TPR < 128 ? 128 : TPR;
-  constexpr int R = THREADS / TPR;
-  constexpr int V = 16 / sizeof(T);
-  constexpr int E = V * VPL;
-  __shared__ float red[2][1][THREADS / 32];
-  __shared__ float slots[R > 1 ? E * (THREADS + TPR) : 1];
-  RowFold<TPR, 1, THREADS> fold{red};
-  const int rl = threadIdx.x / TPR, tl = threadIdx.x % TPR;
-  const int nvec = static_cast<int>(p.cols / V);
+template <class T, int V, int TPR, int F>
+__global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_kernel(const __grid_constant__ Norm8Params p) {
+  using A = RowChunks<T, V, TPR, kNormElts>;
+  using Q = RowChunks<uint8_t, V, TPR, kNormElts>;
+  constexpr int C = A::C, E = kNormElts;
+  constexpr int RW = TPR ? 32 / TPR : 1;
+  constexpr int GC = V > 1 ? 1 : 2;    // chunks of this thread in one group
+  constexpr int NS = A::N / GC;        // scales of this thread
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float4 red[2][32];
+  const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
+  const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  constexpr int STAGE = A::WARP_ARRAY + Q::WARP_ARRAY;
+  unsigned char* gbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (A::WARP_FACTORS + kBwd8Stages * STAGE);
+  unsigned char* ring = gbuf + A::WARP_FACTORS;
+#pragma unroll
+  for (int st = 0; st < kBwd8Stages; ++st) {
+    A::zero_rest(ring + st * STAGE, true, left);
+    Q::zero_rest(ring + st * STAGE + A::WARP_ARRAY, true, left);
+  }
+  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  const int64_t begin = min(worker * p.chunk, p.rows);
+  const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
+  const T* dy_at = static_cast<const T*>(p.dy) + (begin + rl) * p.stride + j0;
+  const uint8_t* q_at = p.q + (begin + rl) * p.cols + j0;
+  const float* scale_at = p.scale + (begin + rl) * p.groups;
+  const float* inv_at = p.inv + begin + rl;
+  int ahead = rl;
+  float sc_next[kBwd8Stages][NS], inv_next[kBwd8Stages];
+  auto fetch = [&](int stage, float (&sc)[NS], float& inv) {
+    inv = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) sc[i] = 0.f;
+    if (ahead < todo) {
+      A::copy(ring + stage * STAGE, dy_at, left);
+      Q::copy(ring + stage * STAGE + A::WARP_ARRAY, q_at, left);
+      inv = *inv_at;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (A::off(i * GC, 0) < left) sc[i] = __ldg(scale_at + chunk_group<A>(j0, i * GC));
+    }
+    ahead += RW;
+    dy_at += RW * p.stride;
+    q_at += RW * p.cols;
+    scale_at += RW * p.groups;
+    inv_at += RW;
+    copy_commit();
+  };
+#pragma unroll
+  for (int st = 0; st < kBwd8Stages; ++st) fetch(st, sc_next[st], inv_next[st]);
+  A::fill_factors(gbuf, left, [&](int o) { return p.gamma ? p.gamma[j0 + o] : 1.f; });
+  T* dx = static_cast<T*>(p.out) + (begin + rl) * p.cols + j0;
   float sum[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) sum[e] = 0.f;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * R; r0 < p.rows; r0 += static_cast<int64_t>(gridDim.x) * R) {
-    const bool live = r0 + rl < p.rows;
-    const int64_t row = live ? r0 + rl : 0;
-    const int nv = live ? nvec : 0;
-    Vec<T, V> dy[VPL];
-    typename Q8Raw<V>::type q[VPL];
-    float sc[VPL];
-    load_vecs<T, V, VPL>(static_cast<const T*>(p.dy) + row * p.stride, tl, TPR, nv, dy);
-#pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      const int j = tl + k * TPR;
-      q[k] = {};
-      sc[k] = 0.f;
-      if (j < nv) {
-        q[k] = *reinterpret_cast<const typename Q8Raw<V>::type*>(p.q + row * p.cols + static_cast<int64_t>(j) * V);
-        sc[k] = __ldg(p.scale + row * p.groups + j / (kQ8Group / V));
-      }
-    }
-    const float inv = live ? p.inv[row] : 0.f;
+  for (int i = 0; i < E; ++i) sum[i] = 0.f;
+  int phase = 0, stage = 0;
+  for (int r0 = 0; r0 < todo; r0 += RW) {
+    const bool live = RW == 1 || r0 + rl < todo;
+    copy_wait<kBwd8Stages - 1>();
+    unsigned char* dbuf = ring + stage * STAGE;
+    unsigned char* qbuf = dbuf + A::WARP_ARRAY;
+    const float inv = inv_next[0];
+    float x[E];
     float s[1] = {0.f};
+    if (live) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      float x[V], g[V];
-      q8_widen<F, V>(q[k], sc[k], x);
-      load_floats<V>(p.gamma, tl + k * TPR, nv, g, 1.f);
+      for (int c = 0; c < A::N; ++c) {
+        float d[C], g[C];
+        A::read(dbuf, c, d);
+        A::read_factors(gbuf, c, g);
+        Vec<uint8_t, C> lv;
+        Q::read_raw(qbuf, c, lv);
+        const float sc = sc_next[0][c / GC];
+        if constexpr (V > 1) {
+          q8_widen<F, V>(*reinterpret_cast<const typename Q8Raw<V>::type*>(&lv), sc, *reinterpret_cast<float(*)[V]>(&x[c * C]));
+        } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float t = to_f(dy[k].v[e]) * x[e];
-        sum[k * V + e] = fmaf(t, inv, sum[k * V + e]);
-        s[0] = fmaf(t, g[e], s[0]);
+          for (int e = 0; e < C; ++e) x[c * C + e] = __fmul_rn(q8_level1<F>(lv.v[e]), sc);
+        }
+#pragma unroll
+        for (int e = 0; e < C; ++e) {
+          const int i = c * C + e;
+          const float t = d[e] * x[i];
+          sum[i] = fmaf(t, inv, sum[i]);
+          s[0] = fmaf(t, g[e], s[0]);
+        }
       }
     }
-    fold(s);
-    const float c = inv * inv * (s[0] * inv / static_cast<float>(p.cols));
+    sum_row<TPR, 1>(s, red, phase);
+    const float k = inv * inv * inv * s[0] * inv_cols;
+    if (live) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      const int j = tl + k * TPR;
-      if (j >= nv) continue;
-      float x[V], g[V];
-      q8_widen<F, V>(q[k], sc[k], x);
-      load_floats<V>(p.gamma, j, nv, g, 1.f);
-      Vec<T, V> o;
+      for (int c = 0; c < A::N; ++c) {
+        float d[C], g[C];
+        A::read(dbuf, c, d);
+        A::read_factors(gbuf, c, g);
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(fmaf(inv * to_f(dy[k].v[e]), g[e], -c * x[e]));
-      *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.out) + row * p.cols + static_cast<int64_t>(j) * V) = o;
+        for (int e = 0; e < C; ++e) d[e] = fmaf(inv * d[e], g[e], -k * x[c * C + e]);
+        A::write(dx, c, left, d);
+      }
     }
+    dx += RW * p.cols;
+#pragma unroll
+    for (int st = 0; st + 1 < kBwd8Stages; ++st) {
+      inv_next[st] = inv_next[st + 1];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) sc_next[st][i] = sc_next[st + 1][i];
+    }
+    fetch(stage, sc_next[kBwd8Stages - 1], inv_next[kBwd8Stages - 1]);
+    stage = stage + 1 == kBwd8Stages ? 0 : stage + 1;
   }
+  copy_wait<0>();
   if (p.ws == nullptr) return;
-  if constexpr (R > 1) {  // the row slots' sums, in slot order
-    __syncthreads();
+  if constexpr (RW > 1) {  // the worker's rows at a time
 #pragma unroll
-    for (int e = 0; e < E; ++e) slots[e * (THREADS + TPR) + threadIdx.x] = sum[e];
-    __syncthreads();
+    for (int i = 0; i < E; ++i)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float t = 0.f;
-#pragma unroll
-      for (int k = 0; k < R; ++k) t += slots[e * (THREADS + TPR) + k * TPR + tl];
-      sum[e] = t;
-    }
+      for (int d = TPR; d < 32; d <<= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
   }
   if (rl == 0) {
+    float* w = p.ws + worker * p.cols + j0;
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-      const int j = tl + k * TPR;
-      if (j >= nvec) continue;
+    for (int c = 0; c < A::N; ++c)
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        p.ws[static_cast<int64_t>(blockIdx.x) * p.cols + static_cast<int64_t>(j) * V + e] = sum[k * V + e];
-    }
+      for (int e = 0; e < C; ++e)
+        if (A::off(c, e) < left) w[A::off(c, e)] = sum[c * C + e];
   }
 }
 
@@ -542,7 +633,7 @@ void launch_checkpoint(const CkParams& p, int format, bool restore, cudaStream_t
   constexpr int VW = 16 / sizeof(T);
   const bool vec = p.g.cols % VW == 0 && p.x_stride % VW == 0 && a16(p.x) && a16(p.out) &&
                    reinterpret_cast<uintptr_t>(p.q) % VW == 0;
-  constexpr int U = 4;
+  constexpr int U = 2;
   unsigned grid = 0;
 #define VB_CK(VEC)                                                                   \
   do {                                                                               \
@@ -565,7 +656,7 @@ void launch_glu(const GluParams& p, int format, bool backward, bool kept, cudaSt
              p.dout_stride % VW == 0 && q_ok(p.q_gate) && q_ok(p.q_up);
   if (backward && kept) vec = vec && q_ok(p.gate) && q_ok(p.up);
   else vec = vec && a16(p.gate) && a16(p.up) && p.gate_stride % VW == 0 && p.up_stride % VW == 0;
-  constexpr int U = 2;
+  constexpr int U = 1;
   unsigned grid = 0;
 #define VB_GLU(VEC)                                                                                             \
   do {                                                                                                          \
@@ -582,72 +673,105 @@ void launch_glu(const GluParams& p, int format, bool backward, bool kept, cudaSt
               p.g.total / p.g.per_row * p.g.cols, p.g.cols, 0, s);
 }
 
+// How a row kernel of this file runs: TPR lanes of a warp share a row (0: the block does), `workers`
+// of them with a run of `chunk` rows each; threads == 0: the stream kernel.
+struct NormShape {
+  int tpr, threads, smem;
+  int64_t chunk, workers;
+  unsigned grid;
+};
+inline NormShape norm_shape(int64_t rows, int64_t cols, int elt, int bytes_per_thread, int sms) {
+  NormShape h{};
+  const int64_t lanes = (cols + kNormElts - 1) / kNormElts;
+  if (lanes > 1024) return h;
+  // a group of 128 values lies in 16 lanes of 16-bit values, 32 of 32-bit ones
+  h.tpr = lanes <= 16 && elt == 2 ? 16 : lanes <= 32 ? 32 : 0;
+  h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
+  h.smem = h.threads * bytes_per_thread;
+  if (h.smem > kSmemPerBlock) return NormShape{};
+  const int per_block = h.tpr ? h.threads / 32 : 1;
+  const int per_sm = std::max(1, std::min(1024 / h.threads, kSmemPerSm / (h.smem + 2048)));
+  const int64_t most = int64_t{sms} * per_sm * per_block;
+  h.chunk = (rows + most - 1) / most;
+  h.grid = static_cast<unsigned>(((rows + h.chunk - 1) / h.chunk + per_block - 1) / per_block);
+  h.workers = int64_t{h.grid} * per_block;
+  return h;
+}
+constexpr int norm8_bytes(int elt) { return kNormElts * (4 + elt); }
+constexpr int bwd8_bytes(int elt) { return kNormElts * (4 + kBwd8Stages * (elt + 1)); }
+
+#define VB_ROW8(KERNEL, V, TPR)                                                       \
+  VB_FORMAT(format, F, do {                                                           \
+    static std::atomic<uint64_t> done{0};                                             \
+    VB_CUDA(allow_shared(KERNEL<T, V, TPR, F>, device, done));                        \
+    KERNEL<T, V, TPR, F><<<h.grid, h.threads, h.smem, s>>>(p);                        \
+  } while (0))
+// single values of 16 bits may share a row between 32 lanes only (a group lies in 32 of them)
+#define VB_ROW8_ALL(KERNEL)                                                           \
+  do {                                                                                \
+    if (vec) {                                                                        \
+      if constexpr (VW == 8) {                                                        \
+        if (h.tpr == 16) { VB_ROW8(KERNEL, VW, 16); break; }                          \
+      }                                                                               \
+      if (h.tpr == 32) VB_ROW8(KERNEL, VW, 32);                                       \
+      else VB_ROW8(KERNEL, VW, 0);                                                    \
+    } else if (h.tpr == 32) VB_ROW8(KERNEL, 1, 32);                                   \
+    else VB_ROW8(KERNEL, 1, 0);                                                       \
+  } while (0)
+
 template <class T>
-void launch_norm8(const Norm8Params& p, int format, cudaStream_t s, int device) {
+vbt_b200_status launch_norm8(Norm8Params p, int format, cudaStream_t s, int device) {
   constexpr int VW = 16 / sizeof(T);
-  constexpr int E = 16;
   const int sms = sm_count(device);
-  const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.x) && a16(p.out) && a16(p.gamma) &&
+  const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.x) && a16(p.out) &&
                    reinterpret_cast<uintptr_t>(p.q) % VW == 0;
-  unsigned g = 0;
-  int threads = 256;
-  auto grid = [&](int per_block, int per_sm) {
-    return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((p.rows + per_block - 1) / per_block, int64_t{sms} * per_sm)));
-  };
-#define VB_N8(TPR)                                                                                      \
-  do {                                                                                                  \
-    threads = TPR < 256 ? 256 : TPR;                                                                    \
-    g = grid(threads / TPR, 2048 / threads);                                                            \
-    VB_FORMAT(format, F, (rmsnorm8_kernel<T, F, E / VW, TPR><<<g, threads, 0, s>>>(p)));                \
-  } while (0)
-  if (!vec || p.cols > 1024 * E) {
-    g = grid(1, 8);
-    VB_FORMAT(format, F, (rmsnorm8_stream_kernel<T, F><<<g, threads, 0, s>>>(p)));
-  } else if (p.cols <= 32 * E) VB_N8(32);
-  else if (p.cols <= 128 * E) VB_N8(128);
-  else if (p.cols <= 256 * E) VB_N8(256);
-  else if (p.cols <= 512 * E) VB_N8(512);
-  else VB_N8(1024);
-#undef VB_N8
-  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_CHECKPOINT8, dim3(g), dim3(threads), vec ? VW : 1, 1, 0, 1,
-              p.rows * p.cols, p.cols, 0, s);
+  const NormShape h = norm_shape(p.rows, p.cols, vec ? static_cast<int>(sizeof(T)) : 4, norm8_bytes(sizeof(T)), sms);
+  unsigned g = h.grid;
+  p.chunk = h.chunk;
+  if (h.threads == 0) {
+    g = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{sms} * 8));
+    VB_FORMAT(format, F, (rmsnorm8_stream_kernel<T, F><<<g, 256, 0, s>>>(p)));
+  } else {
+    VB_ROW8_ALL(rmsnorm8_kernel);
+  }
+  VB_LAUNCH_CHECK();
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_CHECKPOINT8, dim3(g), dim3(h.threads ? h.threads : 256), vec ? VW : 1, 1,
+              0, 1, p.rows * p.cols, p.cols, 0, s);
+  return VBT_B200_OK;
 }
 
-constexpr int bwd8_elts(int elt) { return elt == 2 ? 16 : 8; }
-inline unsigned bwd8_grid(int64_t rows, int sms) {
-  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(rows, int64_t{sms} * 6)));
-}
+inline int64_t bwd8_stream_blocks(int64_t rows, int sms) { return std::min<int64_t>(rows, int64_t{sms} * 6); }
 
 template <class T>
-int launch_norm_bwd8(const Norm8Params& p, float* dgamma, int format, cudaStream_t s, int device) {
+vbt_b200_status launch_norm_bwd8(Norm8Params p, float* dgamma, int format, cudaStream_t s, int device) {
   constexpr int VW = 16 / sizeof(T);
-  constexpr int E = bwd8_elts(sizeof(T));
-  const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.dy) && a16(p.out) && a16(p.gamma) &&
+  const int sms = sm_count(device);
+  const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.dy) && a16(p.out) &&
                    reinterpret_cast<uintptr_t>(p.q) % VW == 0;
-  const unsigned most = bwd8_grid(p.rows, sm_count(device));
-  unsigned g = most;
-  int threads = 256;
-#define VB_B8(TPR)                                                                                      \
-  do {                                                                                                  \
-    threads = TPR < 128 ? 128 : TPR;                                                                    \
-    g = static_cast<unsigned>(std::min<int64_t>(most, (p.rows + threads / TPR - 1) / (threads / TPR))); \
-    VB_FORMAT(format, F, (rmsnorm_bwd8_kernel<T, F, E / VW, TPR><<<g, threads, 0, s>>>(p)));            \
-  } while (0)
-  if (!vec || p.cols > 512 * E) VB_FORMAT(format, F, (rmsnorm_bwd8_stream_kernel<T, F><<<g, threads, 0, s>>>(p)));
-  else if (p.cols <= 8 * E) VB_B8(8);
-  else if (p.cols <= 32 * E) VB_B8(32);
-  else if (p.cols <= 128 * E) VB_B8(128);
-  else if (p.cols <= 256 * E) VB_B8(256);
-  else VB_B8(512);
-#undef VB_B8
-  if (p.ws) rmsnorm_bwd8_fold_kernel<<<static_cast<unsigned>((p.cols + 7) / 8), 256, 0, s>>>(dgamma, p.ws, g, p.cols);
-  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_RMSNORM_BACKWARD8, dim3(g), dim3(threads), vec ? VW : 1, 1, 0,
-              p.ws ? 2 : 1, p.rows * p.cols, p.cols, p.ws ? static_cast<size_t>(g) * p.cols * 4 : 0, s);
-  return 0;
+  const NormShape h = norm_shape(p.rows, p.cols, vec ? static_cast<int>(sizeof(T)) : 4, bwd8_bytes(sizeof(T)), sms);
+  int64_t parts = h.workers;
+  unsigned g = h.grid;
+  p.chunk = h.chunk;
+  if (h.threads == 0) {
+    parts = bwd8_stream_blocks(p.rows, sms);
+    g = static_cast<unsigned>(parts);
+    VB_FORMAT(format, F, (rmsnorm_bwd8_stream_kernel<T, F><<<g, 256, 0, s>>>(p)));
+  } else {
+    VB_ROW8_ALL(rmsnorm_bwd8_kernel);
+  }
+  VB_LAUNCH_CHECK();
+  if (p.ws) rmsnorm_bwd8_fold_kernel<<<static_cast<unsigned>((p.cols + 7) / 8), 256, 0, s>>>(dgamma, p.ws, parts, p.cols);
+  VB_LAUNCH_CHECK();
+  note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_RMSNORM_BACKWARD8, dim3(g), dim3(h.threads ? h.threads : 256), vec ? VW : 1,
+              1, 0, p.ws ? 2 : 1, p.rows * p.cols, p.cols, p.ws ? static_cast<size_t>(parts) * p.cols * 4 : 0, s);
+  return VBT_B200_OK;
 }
+#undef VB_ROW8_ALL
+#undef VB_ROW8
 
 vbt_b200_status check_common(const char* name, int32_t dtype, int32_t format, int64_t rows, int64_t cols) {
   VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
+  VB_ARG(rows < (int64_t{1} << 36), std::string(name) + ": too many rows");
   VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
   VB_ARG(format == VBT_B200_Q8_INT8 || format == VBT_B200_Q8_E4M3, std::string(name) + ": unknown 8-bit format");
   VB_ARG(cols == 0 || rows_fit(rows * ((cols + kQ8Group - 1) / kQ8Group)), std::string(name) + ": too many groups");
@@ -676,7 +800,7 @@ vbt_b200_status vbt_b200_checkpoint8(void* q, float* scale, const void* x, int32
   DeviceScope scope(q);
   CkParams p{};
   p.x = x; p.q = static_cast<uint8_t*>(q); p.scale = scale; p.x_stride = x_row_stride;
-  p.g.fill(rows, cols);
+  p.g.fill(rows, cols, x_row_stride == cols);
   VB_BY_DTYPE(dtype, T, launch_checkpoint<T>(p, format, false, static_cast<cudaStream_t>(stream)));
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;
@@ -691,7 +815,7 @@ vbt_b200_status vbt_b200_checkpoint8_restore(void* out, const void* q, const flo
   DeviceScope scope(out);
   CkParams p{};
   p.out = out; p.q = static_cast<uint8_t*>(const_cast<void*>(q)); p.scale = const_cast<float*>(scale);
-  p.g.fill(rows, cols);
+  p.g.fill(rows, cols, true);
   VB_BY_DTYPE(dtype, T, launch_checkpoint<T>(p, format, true, static_cast<cudaStream_t>(stream)));
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;
@@ -709,7 +833,7 @@ vbt_b200_status vbt_b200_rmsnorm_checkpoint8(void* out, float* inv_rms, void* q,
   Norm8Params p{};
   p.x = x; p.gamma = gamma; p.out = out; p.q = static_cast<uint8_t*>(q); p.scale = scale; p.inv = inv_rms;
   p.rows = rows; p.cols = cols; p.groups = (cols + kQ8Group - 1) / kQ8Group; p.stride = x_row_stride; p.eps = eps;
-  VB_BY_DTYPE(dtype, T, launch_norm8<T>(p, format, static_cast<cudaStream_t>(stream), scope.device()));
+  VB_BY_DTYPE(dtype, T, VB_TRY(launch_norm8<T>(p, format, static_cast<cudaStream_t>(stream), scope.device())));
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;
 }
@@ -719,7 +843,12 @@ vbt_b200_status vbt_b200_rmsnorm_backward8_workspace_bytes(int64_t rows, int64_t
   using namespace vb;
   VB_ARG(bytes != nullptr, "rmsnorm_backward8: null output");
   VB_TRY(check_common("rmsnorm_backward8", dtype, VBT_B200_Q8_INT8, rows, cols));
-  *bytes = static_cast<size_t>(bwd8_grid(rows, sm_count(device))) * static_cast<size_t>(cols) * 4;
+  // whichever form the pointers' alignment takes
+  const int sms = sm_count(device), elt = itemsize(dtype);
+  int64_t parts = bwd8_stream_blocks(rows, sms);
+  for (int lanes_of : {elt, 4})
+    if (rows > 0 && cols > 0) parts = std::max(parts, norm_shape(rows, cols, lanes_of, bwd8_bytes(elt), sms).workers);
+  *bytes = static_cast<size_t>(parts) * static_cast<size_t>(cols) * 4;
   return VBT_B200_OK;
 }
 
@@ -752,7 +881,7 @@ vbt_b200_status vbt_b200_rmsnorm_backward8(void* dx, float* dgamma, const void* 
            "rmsnorm_backward8: workspace too small (see vbt_b200_rmsnorm_backward8_workspace_bytes)");
     p.ws = static_cast<float*>(workspace);
   }
-  VB_BY_DTYPE(dtype, T, launch_norm_bwd8<T>(p, dgamma, format, s, scope.device()));
+  VB_BY_DTYPE(dtype, T, VB_TRY(launch_norm_bwd8<T>(p, dgamma, format, s, scope.device())));
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;
 }
@@ -771,7 +900,7 @@ vbt_b200_status vbt_b200_silu_mul(void* out, void* q_gate, float* scale_gate, vo
   p.gate = gate; p.up = up; p.out = out; p.gate_stride = gate_row_stride; p.up_stride = up_row_stride;
   p.q_gate = static_cast<uint8_t*>(q_gate); p.s_gate = scale_gate;
   p.q_up = static_cast<uint8_t*>(q_up); p.s_up = scale_up;
-  p.g.fill(rows, cols);
+  p.g.fill(rows, cols, gate_row_stride == cols && up_row_stride == cols);
   VB_BY_DTYPE(dtype, T, launch_glu<T>(p, format, false, q_gate != nullptr, static_cast<cudaStream_t>(stream)));
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;
@@ -793,7 +922,7 @@ vbt_b200_status vbt_b200_silu_mul_backward(void* dgate, void* dup, const void* d
   p.dout = dout; p.gate = gate; p.up = up; p.gate_scale = scale_gate; p.up_scale = scale_up;
   p.dgate = dgate; p.dup = dup;
   p.dout_stride = dout_row_stride; p.gate_stride = gate_row_stride; p.up_stride = up_row_stride;
-  p.g.fill(rows, cols);
+  p.g.fill(rows, cols, dout_row_stride == cols && (scale_gate || (gate_row_stride == cols && up_row_stride == cols)));
   VB_BY_DTYPE(dtype, T, launch_glu<T>(p, format, true, scale_gate != nullptr, static_cast<cudaStream_t>(stream)));
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;

@@ -139,8 +139,8 @@ template <class T, int V, int TPR, int E> struct RowChunks {
     return reinterpret_cast<T*>(array) + (V > 1 ? c : 2 * c + e) * (32 * V) + static_cast<int>(threadIdx.x & 31) * V;
   }
   // starts the copies of the thread's part of a row; `row` points at the thread's first column, `left`
-  // values of the row lie from there on (16-bit single values are copied at once: they are smaller
-  // than the smallest asynchronous copy)
+  // values of the row lie from there on (single values of less than four bytes are copied at once: they
+  // are smaller than the smallest asynchronous copy)
   static __device__ __forceinline__ void copy(unsigned char* array, const T* row, int left) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
@@ -152,7 +152,7 @@ template <class T, int V, int TPR, int E> struct RowChunks {
           if (off(c, e) < left) copy_async<4>(slot(array, c, e), row + off(c, e));
       }
     }
-    if constexpr (V == 1 && sizeof(T) == 2) {
+    if constexpr (V == 1 && sizeof(T) < 4) {
       T v[E];
 #pragma unroll
       for (int i = 0; i < E; ++i)
@@ -168,7 +168,7 @@ template <class T, int V, int TPR, int E> struct RowChunks {
     for (int c = 0; c < N; ++c)
 #pragma unroll
       for (int e = 0; e < C; ++e)
-        if (!present || off(c, e) >= left) (V > 1 ? slot(array, c, 0)[e] : *slot(array, c, e)) = from_f<T>(0.f);
+        if (!present || off(c, e) >= left) (V > 1 ? slot(array, c, 0)[e] : *slot(array, c, e)) = T{};
   }
   static __device__ __forceinline__ void read(unsigned char* array, int c, float (&v)[C]) {
     if constexpr (V > 1) {
@@ -178,6 +178,15 @@ template <class T, int V, int TPR, int E> struct RowChunks {
     } else {
       v[0] = to_f(*slot(array, c, 0));
       v[1] = to_f(*slot(array, c, 1));
+    }
+  }
+  // the same without the conversion
+  static __device__ __forceinline__ void read_raw(unsigned char* array, int c, Vec<T, C>& v) {
+    if constexpr (V > 1) {
+      v = *reinterpret_cast<const Vec<T, V>*>(slot(array, c, 0));
+    } else {
+      v.v[0] = *slot(array, c, 0);
+      v.v[1] = *slot(array, c, 1);
     }
   }
   static __device__ __forceinline__ void write(T* row, int c, int left, const float (&v)[C]) {
