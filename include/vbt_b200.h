@@ -566,19 +566,16 @@ VBT_B200_API vbt_b200_status vbt_b200_silu_mul_backward(void* dgate, void* dup, 
  * (2i, 2i + 1) with interleaved != 0; values behind 2 * half are copied.
  *   a' = a cos - b sin,  b' = b cos + a sin;  inverse != 0 turns back, which is the backward pass.
  * The angle is formed in 64 bits and reduced to a part of a turn there, so positions far into a long
- * sequence lose nothing.  q and k: [batch, tokens, heads, dim], last stride 1, other strides (in
- * elements) given as {batch, token, head}; q_out, k_out likewise (an output may be its own input).
- * k may be NULL.  positions: I64, I32 or F32 with strides {axis, batch, token}; inv_freq: F32 [half].
- * The stride and section arrays are host memory, read before the call returns. */
+ * sequence lose nothing.  q and k: [batch, tokens, heads, dim], last stride 1; q_out, k_out likewise (an
+ * output may be its own input).  k may be NULL.  positions: I64, I32 or F32 [naxes, batch, tokens];
+ * inv_freq: F32 [half].  strides (in elements): {batch, token, head} of q_out, q, k_out and k, then
+ * {axis, batch, token} of positions.  It and `sections` are host memory, read before the call returns. */
 #define VBT_B200_ROTARY_MAX_AXES 4
-VBT_B200_API vbt_b200_status vbt_b200_rotary(void* q_out, const int64_t* q_out_strides, const void* q,
-                                const int64_t* q_strides, int64_t q_heads, void* k_out,
-                                const int64_t* k_out_strides, const void* k, const int64_t* k_strides,
-                                int64_t k_heads, int32_t dtype, int64_t batch, int64_t tokens, int64_t dim,
-                                const void* positions, int32_t positions_dtype,
-                                const int64_t* positions_strides, const float* inv_freq, int64_t half,
-                                const int64_t* sections, int32_t naxes, int32_t interleaved, int32_t inverse,
-                                void* stream);
+VBT_B200_API vbt_b200_status vbt_b200_rotary(void* q_out, const void* q, int64_t q_heads, void* k_out, const void* k,
+                                int64_t k_heads, const int64_t* strides, int32_t dtype, int64_t batch,
+                                int64_t tokens, int64_t dim, const void* positions, int32_t positions_dtype,
+                                const float* inv_freq, int64_t half, const int64_t* sections, int32_t naxes,
+                                int32_t interleaved, int32_t inverse, void* stream);
 
 /* A paged key/value cache in 8 bits (the format above, one scale per slot and head).  k_cache and
  * v_cache: dense [num_slots, heads, dim] bytes, num_slots = pages * page_size; k_scale, v_scale: F32

@@ -103,8 +103,8 @@ SIGNATURES = {
     "vbt_b200_rmsnorm_backward8": (_i32, [_vp] * 7 + [_i32] * 2 + [_i64] * 3 + [_vp, ctypes.c_size_t, _vp]),
     "vbt_b200_silu_mul": (_i32, [_vp] * 7 + [_i32] * 2 + [_i64] * 4 + [_vp]),
     "vbt_b200_silu_mul_backward": (_i32, [_vp] * 7 + [_i32] * 2 + [_i64] * 5 + [_vp]),
-    "vbt_b200_rotary": (_i32, [_vp, _i64p, _vp, _i64p, _i64] * 2 + [_i32] + [_i64] * 3 + [_vp, _i32, _i64p, _vp, _i64,
-                               _i64p, _i32, _i32, _i32, _vp]),
+    "vbt_b200_rotary": (_i32, [_vp, _vp, _i64] * 2 + [_i64p, _i32] + [_i64] * 3 + [_vp, _i32, _vp, _i64, _i64p] +
+                        [_i32] * 3 + [_vp]),
     "vbt_b200_kv_cache_write": (_i32, [_vp] * 4 + [_i64] * 3 + [_i32] + [_vp, _i64p] * 2 +
                                 [_i32, _vp, _i32, _i64, _vp, _vp, _vp]),
     "vbt_b200_kv_cache_read": (_i32, [_vp] * 2 + [_i32, _i64] + [_vp] * 4 + [_i64] * 4 + [_i32, _vp, _i32] + [_i64] * 2 +

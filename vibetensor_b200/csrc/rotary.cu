@@ -200,13 +200,11 @@ vbt_b200_status launch_rotary(RotParams p, int interleaved, cudaStream_t s) {
 
 extern "C" {
 
-vbt_b200_status vbt_b200_rotary(void* q_out, const int64_t* q_out_strides, const void* q, const int64_t* q_strides,
-                                int64_t q_heads, void* k_out, const int64_t* k_out_strides, const void* k,
-                                const int64_t* k_strides, int64_t k_heads, int32_t dtype, int64_t batch, int64_t tokens,
-                                int64_t dim, const void* positions, int32_t positions_dtype,
-                                const int64_t* positions_strides, const float* inv_freq, int64_t half,
-                                const int64_t* sections, int32_t naxes, int32_t interleaved, int32_t inverse,
-                                void* stream) {
+vbt_b200_status vbt_b200_rotary(void* q_out, const void* q, int64_t q_heads, void* k_out, const void* k,
+                                int64_t k_heads, const int64_t* strides, int32_t dtype, int64_t batch, int64_t tokens,
+                                int64_t dim, const void* positions, int32_t positions_dtype, const float* inv_freq,
+                                int64_t half, const int64_t* sections, int32_t naxes, int32_t interleaved,
+                                int32_t inverse, void* stream) {
   using namespace vb;
   VB_ARG(is_float_dtype(dtype), "rotary: expected a floating dtype");
   VB_ARG(batch >= 0 && tokens >= 0 && dim >= 0 && q_heads >= 0 && k_heads >= 0 && half >= 0, "rotary: negative size");
@@ -224,9 +222,9 @@ vbt_b200_status vbt_b200_rotary(void* q_out, const int64_t* q_out_strides, const
   if (batch == 0 || tokens == 0 || dim == 0 || q_heads + k_heads == 0) return VBT_B200_OK;
   VB_ARG(half <= 4096 && q_heads <= 16384 && k_heads <= 16384 && dim <= (int64_t{1} << 28) / (q_heads + k_heads),
          "rotary: head too wide or too many heads");
-  VB_ARG(q_heads == 0 || (q && q_out && q_strides && q_out_strides), "rotary: null pointer");
-  VB_ARG(k_heads == 0 || (k && k_out && k_strides && k_out_strides), "rotary: null pointer");
-  VB_ARG(positions_strides && (half == 0 || (positions && inv_freq)), "rotary: null pointer");
+  VB_ARG(q_heads == 0 || (q && q_out), "rotary: null pointer");
+  VB_ARG(k_heads == 0 || (k && k_out), "rotary: null pointer");
+  VB_ARG(strides && (half == 0 || (positions && inv_freq)), "rotary: null pointer");
   VB_ARG(batch <= (int64_t{1} << 31) / tokens, "rotary: too many tokens");
   DeviceScope scope(q_heads ? q_out : k_out);
   RotParams p{};
@@ -234,10 +232,10 @@ vbt_b200_status vbt_b200_rotary(void* q_out, const int64_t* q_out_strides, const
     s.in = in; s.in_b = is[0]; s.in_t = is[1]; s.in_h = is[2];
     s.out = out; s.out_b = os[0]; s.out_t = os[1]; s.out_h = os[2];
   };
-  if (q_heads) side(p.q, q, q_strides, q_out, q_out_strides);
-  if (k_heads) side(p.k, k, k_strides, k_out, k_out_strides);
+  if (q_heads) side(p.q, q, strides + 3, q_out, strides);
+  if (k_heads) side(p.k, k, strides + 9, k_out, strides + 6);
   p.pos = positions; p.pos_dtype = positions_dtype;
-  p.pos_a = positions_strides[0]; p.pos_b = positions_strides[1]; p.pos_t = positions_strides[2];
+  p.pos_a = strides[12]; p.pos_b = strides[13]; p.pos_t = strides[14];
   p.freq = inv_freq;
   p.count = batch * tokens; p.tokens = tokens;
   p.q_heads = static_cast<int>(q_heads); p.heads = static_cast<int>(q_heads + k_heads);

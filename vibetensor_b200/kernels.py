@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import builtins
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -249,6 +250,14 @@ def _like(what: str, name: str, t: torch.Tensor, x: torch.Tensor) -> None:
         raise TypeError(f"{what}: {name} is {t.dtype}, expected {x.dtype}")
 
 
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(entry: str, *sizes: int) -> int:
+    """What a ``*_workspace_bytes`` entry answers, a function of its arguments alone."""
+    need = ctypes.c_size_t()
+    check(getattr(lib(), entry)(*sizes, ctypes.byref(need)))
+    return need.value
+
+
 def _gamma(name: str, g: Optional[torch.Tensor], cols: int) -> Optional[torch.Tensor]:
     if g is None:
         return None
@@ -311,8 +320,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gamma_post: Optional[torch.T
     gv, rs_g, per = _gate_rows(what, gate, x, rows)
     r = _dense_like(x)
     n = _dense_like(x) if pre_norm else None
-    inv_post = _floats(x, rows) if post_norm else None
-    inv_pre = _floats(x, rows) if pre_norm else None
+    if post_norm and pre_norm:
+        inv_post, inv_pre = x.new_empty((2, rows), dtype=torch.float32).unbind()
+    else:
+        inv_post, inv_pre = (_floats(x, rows) if on else None for on in (post_norm, pre_norm))
     if rows and cols:
         check(lib().vbt_b200_residual_norm(
             _ptr(r), _ptr(n), _ptr(inv_post), _ptr(inv_pre), _ptr(xv), _ptr(yv), _ptr(gamma_post), _ptr(gv),
@@ -368,11 +379,9 @@ def residual_norm_backward(grad_r: Optional[torch.Tensor], grad_n: Optional[torc
         return dx, dy, dg1, dgate, dg2
     ws, ws_bytes = None, 0
     if rows and (dg1 is not None or dg2 is not None or dgate is not None):
-        need = ctypes.c_size_t()
-        check(lib().vbt_b200_residual_norm_backward_workspace_bytes(rows, cols, dtype_code(first.dtype), per,
-                                                                    first.device.index, ctypes.byref(need)))
-        ws = first.new_empty((need.value,), dtype=torch.uint8)
-        ws_bytes = need.value
+        ws_bytes = _scratch_bytes("vbt_b200_residual_norm_backward_workspace_bytes", rows, cols, dtype_code(first.dtype),
+                                  per, first.get_device())
+        ws = first.new_empty((ws_bytes,), dtype=torch.uint8)
     (drv, rs_dr), (dnv, rs_dn), (yv, rs_y), (rv, rs_r) = views
     check(lib().vbt_b200_residual_norm_backward(
         _ptr(dx), _ptr(dy), _ptr(dg1), _ptr(dgate), _ptr(dg2), _ptr(drv), _ptr(dnv), _ptr(yv), _ptr(rv),
@@ -495,11 +504,9 @@ def _rmsnorm_backward8(grad_output: torch.Tensor, c: Checkpoint8, inv_rms: torch
         return dx, dgamma
     ws, ws_bytes = None, 0
     if rows and dgamma is not None:
-        need = ctypes.c_size_t()
-        check(lib().vbt_b200_rmsnorm_backward8_workspace_bytes(rows, cols, dtype_code(c.dtype), c.device.index,
-                                                               ctypes.byref(need)))
-        ws = c.q.new_empty((need.value,), dtype=torch.uint8)
-        ws_bytes = need.value
+        ws_bytes = _scratch_bytes("vbt_b200_rmsnorm_backward8_workspace_bytes", rows, cols, dtype_code(c.dtype),
+                                  c.q.get_device())
+        ws = c.q.new_empty((ws_bytes,), dtype=torch.uint8)
     check(lib().vbt_b200_rmsnorm_backward8(_ptr(dx), _ptr(dgamma), _ptr(gv), _ptr(c.q), _ptr(c.scale), _ptr(inv_rms),
                                            _ptr(gamma), dtype_code(c.dtype), code, rows, cols, rs, _ptr(ws), ws_bytes,
                                            stream_ptr(grad_output)))
@@ -568,13 +575,14 @@ def silu_mul_backward(grad_output: torch.Tensor, gate, up):
     return dgate, dup
 
 
-_I64x3 = ctypes.c_int64 * 3
+_I64x15 = ctypes.c_int64 * 15
+_SECTIONS = [ctypes.c_int64 * n for n in range(5)]
 
 
 def _head_strides(t: torch.Tensor):
     """{batch, token, head} strides of [batch, tokens, heads, dim] or [tokens, heads, dim]."""
     st = t.stride()
-    return _I64x3(0, st[0], st[1]) if len(st) == 3 else _I64x3(st[0], st[1], st[2])
+    return (0, st[0], st[1]) if len(st) == 3 else st[:3]
 
 
 def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what):
@@ -630,22 +638,22 @@ def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what
             _like(what, name, o, x)
             if o.stride(-1) != 1 and dim > 1:
                 raise ValueError(f"{what}: {name} must have a last stride of 1")
-    res, args, keep = [], [], []
-    for i, x in enumerate((q, k)):
-        if x is None:
-            res.append(None)
-            args += (None, None, None, None, 0)
-            continue
-        if x.stride(-1) != 1 and dim > 1:
-            x = _ops.contiguous(x)
-        o = out[i] if out is not None else _dense_like(x)
-        res.append(o)
-        keep.append(x)
-        args += (_ptr(o), _head_strides(o), _ptr(x), _head_strides(x), x.shape[-2])
-    check(lib().vbt_b200_rotary(*args, dtype_code(q.dtype), batch, tokens, dim, _ptr(pos), dtype_code(pos.dtype),
-                                _I64x3(*ps), _ptr(inv_freq), half, (ctypes.c_int64 * axes)(*sections), axes,
-                                int(interleaved), int(inverse), stream_ptr(q)))
-    return tuple(res)
+    qv = q if q.stride(-1) == 1 or dim <= 1 else _ops.contiguous(q)
+    qo = out[0] if out is not None else _dense_like(qv)
+    strides = (*_head_strides(qo), *_head_strides(qv))
+    if k is None:
+        ko, kargs = None, (None, None, 0)
+        strides += (0,) * 6
+    else:
+        kv = k if k.stride(-1) == 1 or dim <= 1 else _ops.contiguous(k)
+        ko = out[1] if out is not None else _dense_like(kv)
+        kargs = (ko.data_ptr(), kv.data_ptr(), kv.shape[-2])
+        strides += (*_head_strides(ko), *_head_strides(kv))
+    check(lib().vbt_b200_rotary(qo.data_ptr(), qv.data_ptr(), shape[-2], *kargs, _I64x15(*strides, *ps),
+                                dtype_code(q.dtype), batch, tokens, dim, pos.data_ptr(), dtype_code(pos.dtype),
+                                inv_freq.data_ptr(), half, _SECTIONS[axes](*sections), axes, int(interleaved),
+                                int(inverse), stream_ptr(q)))
+    return qo, ko
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
