@@ -16,6 +16,8 @@ namespace vb {
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotTokens = 32;  // most tokens of a block
+constexpr int kRotRows = 1;     // heads in flight per thread
 
 struct RotSide {
   const void* in;
@@ -36,18 +38,19 @@ struct RotParams {
   int rot_items, items; // per head: vector pairs that turn, all pieces of work
   int tb, hb;           // tokens and heads of a block
   int end[VBT_B200_ROTARY_MAX_AXES];  // end[a]: first pair behind axis a's section
-  FastDiv div_items, div_half;
+  FastDiv div_heads, div_half;  // by a block's heads, by half
   float sign;
 };
 
-// cos and sin of 2 pi * turns
-__device__ __forceinline__ void turn(double turns, float& c, float& s) {
-  const double quarter = rint(turns * 4.0);
-  const float left = static_cast<float>((turns - quarter * 0.25) * 2.0);  // half turns, |left| <= 1/4
+// cos and sin of pi / 2 * quarters.  Adding 1.5 * 2^52 rounds to the nearest whole quarter and leaves it
+// in the sum's low bits (|quarters| < 2^51); what is left of the turn goes to 32 bits.
+__device__ __forceinline__ void turn(double quarters, float& c, float& s) {
+  constexpr double kRound = 6755399441055744.0;
+  const double whole = quarters + kRound;
+  const float left = 0.5f * static_cast<float>(quarters - (whole - kRound));  // half turns, |left| <= 1/4
+  const int qd = __double2loint(whole) & 3;
   float sl, cl;
   sincospif(left, &sl, &cl);
-  // quarter mod 4 without a trip through a 64-bit integer
-  const int qd = static_cast<int>(quarter - 4.0 * floor(quarter * 0.25));
   c = (qd & 1) ? sl : cl;
   s = (qd & 1) ? cl : sl;
   if (qd == 1 || qd == 2) c = -c;
@@ -57,12 +60,21 @@ __device__ __forceinline__ void turn(double turns, float& c, float& s) {
 // P pairs per piece of work.  PAIRED: neighbours (2i, 2i + 1) in one vector of 2P values; else P
 // values at i and P at half + i.  VEC: the vectors may be read whole.
 template <class T, int P, bool PAIRED, bool VEC>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, 8) rotary_kernel(const __grid_constant__ RotParams p) {
   extern __shared__ float table[];  // cosines [tb][half], then sines
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tb;
   const int tb = static_cast<int>(min(static_cast<int64_t>(p.tb), p.count - first));
   float* cosines = table;
   float* sines = table + p.tb * p.half;
+  constexpr int U = kRotRows;
+  __shared__ int64_t place[kRotTokens][4];  // where a token's q and k begin: in, out, in, out
+  if (threadIdx.x < tb) {
+    const int64_t at = first + threadIdx.x, b = at / p.tokens, t = at - b * p.tokens;
+    place[threadIdx.x][0] = b * p.q.in_b + t * p.q.in_t;
+    place[threadIdx.x][1] = b * p.q.out_b + t * p.q.out_t;
+    place[threadIdx.x][2] = b * p.k.in_b + t * p.k.in_t;
+    place[threadIdx.x][3] = b * p.k.out_b + t * p.k.out_t;
+  }
   for (int i = threadIdx.x; i < tb * p.half; i += kRotThreads) {
     uint32_t tok, f;
     p.div_half.divmod(static_cast<uint32_t>(i), tok, f);
@@ -75,63 +87,76 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
                        : p.pos_dtype == VBT_B200_I32 ? static_cast<double>(static_cast<const int32_t*>(p.pos)[src])
                                                      : static_cast<double>(static_cast<const float*>(p.pos)[src]);
     float c, s;
-    turn(pos * static_cast<double>(p.freq[f]) * 0.15915494309189533577, c, s);
+    turn(pos * (static_cast<double>(p.freq[f]) * 0.63661977236758134308), c, s);  // 2 / pi
     cosines[i] = c;
     sines[i] = p.sign * s;
   }
   __syncthreads();
   const int h0 = blockIdx.y * p.hb;
-  const int hn = min(p.hb, p.heads - h0);
-  const int per_token = hn * p.items;
   constexpr int W = PAIRED ? 2 * P : P;
-  for (int tok = 0; tok < tb; ++tok) {
-    const int64_t at = first + tok, b = at / p.tokens, t = at - b * p.tokens;
-    const float* ct = cosines + tok * p.half;
-    const float* st = sines + tok * p.half;
-    for (int i = threadIdx.x; i < per_token; i += kRotThreads) {
-      uint32_t hl, item;
-      p.div_items.divmod(static_cast<uint32_t>(i), hl, item);
-      const int h = h0 + static_cast<int>(hl);
-      const bool isq = h < p.q_heads;
-      const RotSide& side = isq ? p.q : p.k;
-      const int hh = isq ? h : h - p.q_heads;
-      const T* in = static_cast<const T*>(side.in) + b * side.in_b + t * side.in_t + hh * side.in_h;
-      T* out = static_cast<T*>(side.out) + b * side.out_b + t * side.out_t + hh * side.out_h;
-      if (static_cast<int>(item) >= p.rot_items) {  // values behind the turned ones
-        const int e0 = 2 * p.half + (static_cast<int>(item) - p.rot_items) * W;
+  // A thread keeps its place in a head and walks the (token, head) pairs of the block, `slots` apart
+  // and U at a time.
+  const int span = min(p.items, kRotThreads);
+  const int slots = kRotThreads / span;
+  const int mine = threadIdx.x / span;
+  if (mine >= slots) return;
+  const int pairs = tb * p.hb;
+  for (int item = threadIdx.x - mine * span; item < p.items; item += span) {
+    const bool turns = item < p.rot_items;
+    const int i0 = turns ? item * P : 0;                                       // first pair
+    const int e0 = turns ? (PAIRED ? 2 * i0 : i0) : 2 * p.half + (item - p.rot_items) * W;  // first value
+    for (int k0 = mine; k0 < pairs; k0 += slots * U) {
+      T* out[U];
+      const T* in[U];
+      int at_table[U];
+      Vec<T, W> x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * slots;
+        out[u] = nullptr;
+        if (k >= pairs) continue;
+        uint32_t tok, hl;
+        p.div_heads.divmod(static_cast<uint32_t>(k), tok, hl);
+        const int h = h0 + static_cast<int>(hl);
+        if (h >= p.heads) continue;
+        const bool isq = h < p.q_heads;
+        const int hh = isq ? h : h - p.q_heads;
+        at_table[u] = tok * p.half + i0;
+        in[u] = static_cast<const T*>(isq ? p.q.in : p.k.in) + place[tok][isq ? 0 : 2] + hh * (isq ? p.q.in_h : p.k.in_h) + e0;
+        out[u] = static_cast<T*>(isq ? p.q.out : p.k.out) + place[tok][isq ? 1 : 3] + hh * (isq ? p.q.out_h : p.k.out_h) + e0;
         if constexpr (VEC) {
-          *reinterpret_cast<Vec<T, W>*>(out + e0) = *reinterpret_cast<const Vec<T, W>*>(in + e0);
+          x[u] = *reinterpret_cast<const Vec<T, W>*>(in[u]);
+          if (!PAIRED && turns) y[u] = *reinterpret_cast<const Vec<T, W>*>(in[u] + p.half);
         } else {
 #pragma unroll
           for (int e = 0; e < W; ++e)
-            if (e0 + e < p.dim) out[e0 + e] = in[e0 + e];
+            if (turns || e0 + e < p.dim) x[u].v[e] = in[u][e];
         }
-        continue;
       }
-      const int i0 = static_cast<int>(item) * P;
-      if constexpr (PAIRED) {
-        Vec<T, 2 * P> v;
-        if constexpr (VEC) v = *reinterpret_cast<const Vec<T, 2 * P>*>(in + 2 * i0);
-        else { v.v[0] = in[2 * i0]; v.v[1] = in[2 * i0 + 1]; }
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-          const float c = ct[i0 + e], s = st[i0 + e], x = to_f(v.v[2 * e]), y = to_f(v.v[2 * e + 1]);
-          v.v[2 * e] = from_f<T>(x * c - y * s);
-          v.v[2 * e + 1] = from_f<T>(y * c + x * s);
-        }
-        if constexpr (VEC) *reinterpret_cast<Vec<T, 2 * P>*>(out + 2 * i0) = v;
-        else { out[2 * i0] = v.v[0]; out[2 * i0 + 1] = v.v[1]; }
-      } else {
-        Vec<T, P> x = *reinterpret_cast<const Vec<T, P>*>(in + i0);
-        Vec<T, P> y = *reinterpret_cast<const Vec<T, P>*>(in + p.half + i0);
+      for (int u = 0; u < U; ++u) {
+        if (out[u] == nullptr) continue;
+        if (turns) {
+          const float* ct = cosines + at_table[u];
+          const float* st = sines + at_table[u];
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-          const float c = ct[i0 + e], s = st[i0 + e], xf = to_f(x.v[e]), yf = to_f(y.v[e]);
-          x.v[e] = from_f<T>(xf * c - yf * s);
-          y.v[e] = from_f<T>(yf * c + xf * s);
+          for (int e = 0; e < P; ++e) {
+            const float c = ct[e], s = st[e];
+            T& a = PAIRED ? x[u].v[(2 * e) % W] : x[u].v[e % W];
+            T& b = PAIRED ? x[u].v[(2 * e + 1) % W] : y[u].v[e % W];
+            const float af = to_f(a), bf = to_f(b);
+            a = from_f<T>(af * c - bf * s);
+            b = from_f<T>(bf * c + af * s);
+          }
         }
-        *reinterpret_cast<Vec<T, P>*>(out + i0) = x;
-        *reinterpret_cast<Vec<T, P>*>(out + p.half + i0) = y;
+        if constexpr (VEC) {
+          *reinterpret_cast<Vec<T, W>*>(out[u]) = x[u];
+          if (!PAIRED && turns) *reinterpret_cast<Vec<T, W>*>(out[u] + p.half) = y[u];
+        } else {
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+            if (turns || e0 + e < p.dim) out[u][e] = x[u].v[e];
+        }
       }
     }
   }
@@ -163,17 +188,19 @@ vbt_b200_status launch_rotary(RotParams p, int interleaved, cudaStream_t s) {
   if (!vec) { pairs = 1; values = interleaved ? 2 : 1; }
   p.rot_items = p.half / pairs;
   p.items = p.rot_items + (p.dim - 2 * p.half + values - 1) / values;
-  p.div_items = FastDiv(static_cast<uint32_t>(p.items));
   p.div_half = FastDiv(static_cast<uint32_t>(std::max(p.half, 1)));
-  // a block takes all heads of as many tokens as give each thread four pieces (the table is worked out once
+  // a block takes all heads of as many tokens as give each thread eight vectors (the table is worked out once
   // per token); with too few tokens to fill the card the heads are cut instead
-  const int64_t per_token = int64_t{p.heads} * p.items;
-  p.tb = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4 * kRotThreads / std::max<int64_t>(per_token, 1), 4096 / std::max(p.half, 1))));
+  const int64_t per_token = int64_t{p.heads} * p.items * (interleaved ? 1 : 2);
+  p.tb = static_cast<int>(std::min<int64_t>({int64_t{kRotTokens}, 8 * kRotThreads / std::max<int64_t>(per_token, 1), int64_t{4096 / std::max(p.half, 1)}}));
+  // but no fewer than four blocks per SM
+  p.tb = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tb, p.count / 592)));
   p.hb = p.heads;
   if (p.count <= 296) {
     p.tb = 1;
     p.hb = std::max(1, std::min(p.heads, kRotThreads / std::max(p.items, 1)));
   }
+  p.div_heads = FastDiv(static_cast<uint32_t>(p.hb));
   dim3 grid(static_cast<unsigned>((p.count + p.tb - 1) / p.tb), static_cast<unsigned>((p.heads + p.hb - 1) / p.hb));
   const size_t smem = static_cast<size_t>(p.tb) * p.half * 8;
 #define VB_ROT(P, PAIRED, VEC) rotary_kernel<T, P, PAIRED, VEC><<<grid, kRotThreads, smem, s>>>(p)
