@@ -353,11 +353,13 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
   unsigned char* gbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (A::WARP_FACTORS + A::WARP_ARRAY);
   unsigned char* xbuf = gbuf + A::WARP_FACTORS;
   A::zero_rest(xbuf, true, left);
+  const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
   const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   const int64_t begin = min(worker * p.chunk, p.rows);
   const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
-  const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.stride + j0;
-  if (rl < todo) A::copy(xbuf, x_at, left);
+  const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.stride + seg;
+  const typename A::Shift x_shift(p.x, p.stride);
+  if (rl < todo) A::copy(xbuf, x_at, seg_left, p.x);
   copy_commit();
   A::fill_factors(gbuf, left, [&](int o) { return p.gamma ? p.gamma[j0 + o] : 1.f; });
   T* out = static_cast<T*>(p.out) + (begin + rl) * p.cols + j0;
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
   for (int r0 = 0; r0 < todo; r0 += RW) {
     const bool live = RW == 1 || r0 + rl < todo;
     copy_wait<0>();
+    A::sync();
     float x[kNormElts];
     float s[1] = {0.f};
 #pragma unroll
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
       Vec<T, C> raw[GC];
 #pragma unroll
       for (int k = 0; k < GC; ++k) {
-        A::read_raw(xbuf, c0 + k, raw[k]);
+        A::read_raw(xbuf, x_shift(begin + r0 + rl), c0 + k, live ? left : 0, raw[k]);
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           x[(c0 + k) * C + e] = to_f(raw[k].v[e]);
@@ -395,7 +398,8 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
       }
     }
     x_at += RW * p.stride;
-    if (r0 + RW + rl < todo) A::copy(xbuf, x_at, left);
+    A::sync();
+    if (r0 + RW + rl < todo) A::copy(xbuf, x_at, seg_left, p.x);
     copy_commit();
     if (!live) s[0] = 0.f;
     sum_row<TPR, 1>(s, red, phase);
@@ -469,11 +473,14 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
     A::zero_rest(ring + st * STAGE, true, left);
     Q::zero_rest(ring + st * STAGE + A::WARP_ARRAY, true, left);
   }
+  const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
+  const typename A::Shift dy_shift(p.dy, p.stride);
+  const typename Q::Shift q_shift(p.q, p.cols);
   const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   const int64_t begin = min(worker * p.chunk, p.rows);
   const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
-  const T* dy_at = static_cast<const T*>(p.dy) + (begin + rl) * p.stride + j0;
-  const uint8_t* q_at = p.q + (begin + rl) * p.cols + j0;
+  const T* dy_at = static_cast<const T*>(p.dy) + (begin + rl) * p.stride + seg;
+  const uint8_t* q_at = p.q + (begin + rl) * p.cols + seg;
   const float* scale_at = p.scale + (begin + rl) * p.groups;
   const float* inv_at = p.inv + begin + rl;
   int ahead = rl;
@@ -483,8 +490,8 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
     for (int i = 0; i < NS; ++i) sc[i] = 0.f;
     if (ahead < todo) {
-      A::copy(ring + stage * STAGE, dy_at, left);
-      Q::copy(ring + stage * STAGE + A::WARP_ARRAY, q_at, left);
+      A::copy(ring + stage * STAGE, dy_at, seg_left, p.dy);
+      Q::copy(ring + stage * STAGE + A::WARP_ARRAY, q_at, seg_left, p.q);
       inv = *inv_at;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
@@ -508,6 +515,8 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
   for (int r0 = 0; r0 < todo; r0 += RW) {
     const bool live = RW == 1 || r0 + rl < todo;
     copy_wait<kBwd8Stages - 1>();
+    A::sync();
+    const int64_t row = begin + r0 + rl;
     unsigned char* dbuf = ring + stage * STAGE;
     unsigned char* qbuf = dbuf + A::WARP_ARRAY;
     const float inv = inv_next[0];
@@ -517,10 +526,10 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float d[C], g[C];
-        A::read(dbuf, c, d);
+        A::read(dbuf, dy_shift(row), c, left, d);
         A::read_factors(gbuf, c, g);
         Vec<uint8_t, C> lv;
-        Q::read_raw(qbuf, c, lv);
+        Q::read_raw(qbuf, q_shift(row), c, left, lv);
         const float sc = sc_next[0][c / GC];
         if constexpr (V > 1) {
           q8_widen<F, V>(*reinterpret_cast<const typename Q8Raw<V>::type*>(&lv), sc, *reinterpret_cast<float(*)[V]>(&x[c * C]));
@@ -543,7 +552,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float d[C], g[C];
-        A::read(dbuf, c, d);
+        A::read(dbuf, dy_shift(row), c, left, d);
         A::read_factors(gbuf, c, g);
 #pragma unroll
         for (int e = 0; e < C; ++e) d[e] = fmaf(inv * d[e], g[e], -k * x[c * C + e]);
@@ -557,6 +566,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int i = 0; i < NS; ++i) sc_next[st][i] = sc_next[st + 1][i];
     }
+    A::sync();
     fetch(stage, sc_next[kBwd8Stages - 1], inv_next[kBwd8Stages - 1]);
     stage = stage + 1 == kBwd8Stages ? 0 : stage + 1;
   }
@@ -680,14 +690,15 @@ struct NormShape {
   int64_t chunk, workers;
   unsigned grid;
 };
-inline NormShape norm_shape(int64_t rows, int64_t cols, int elt, int bytes_per_thread, int sms) {
+template <class Bytes>
+inline NormShape norm_shape(int64_t rows, int64_t cols, int elt, bool vec, Bytes bytes, int sms) {
   NormShape h{};
   const int64_t lanes = (cols + kNormElts - 1) / kNormElts;
   if (lanes > 1024) return h;
-  // a group of 128 values lies in 16 lanes of 16-bit values, 32 of 32-bit ones
-  h.tpr = lanes <= 16 && elt == 2 ? 16 : lanes <= 32 ? 32 : 0;
+  // a group of 128 values lies in 16 lanes of 16-bit vectors, else in 32
+  h.tpr = lanes <= 16 && elt == 2 && vec ? 16 : lanes <= 32 ? 32 : 0;
   h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
-  h.smem = h.threads * bytes_per_thread;
+  h.smem = h.threads * bytes(elt, vec, h.tpr);
   if (h.smem > kSmemPerBlock) return NormShape{};
   const int per_block = h.tpr ? h.threads / 32 : 1;
   const int per_sm = std::max(1, std::min(1024 / h.threads, kSmemPerSm / (h.smem + 2048)));
@@ -697,8 +708,11 @@ inline NormShape norm_shape(int64_t rows, int64_t cols, int elt, int bytes_per_t
   h.workers = int64_t{h.grid} * per_block;
   return h;
 }
-constexpr int norm8_bytes(int elt) { return kNormElts * (4 + elt); }
-constexpr int bwd8_bytes(int elt) { return kNormElts * (4 + kBwd8Stages * (elt + 1)); }
+// shared memory per thread: gamma and a row of x, or of dy and the levels
+constexpr int norm8_bytes(int elt, bool vec, int tpr) { return kNormElts * 4 + row_bytes_per_thread(kNormElts, elt, vec, tpr); }
+constexpr int bwd8_bytes(int elt, bool vec, int tpr) {
+  return kNormElts * 4 + kBwd8Stages * (row_bytes_per_thread(kNormElts, elt, vec, tpr) + row_bytes_per_thread(kNormElts, 1, vec, tpr));
+}
 
 #define VB_ROW8(KERNEL, V, TPR)                                                       \
   VB_FORMAT(format, F, do {                                                           \
@@ -725,7 +739,7 @@ vbt_b200_status launch_norm8(Norm8Params p, int format, cudaStream_t s, int devi
   const int sms = sm_count(device);
   const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.x) && a16(p.out) &&
                    reinterpret_cast<uintptr_t>(p.q) % VW == 0;
-  const NormShape h = norm_shape(p.rows, p.cols, vec ? static_cast<int>(sizeof(T)) : 4, norm8_bytes(sizeof(T)), sms);
+  const NormShape h = norm_shape(p.rows, p.cols, sizeof(T), vec, norm8_bytes, sms);
   unsigned g = h.grid;
   p.chunk = h.chunk;
   if (h.threads == 0) {
@@ -748,7 +762,7 @@ vbt_b200_status launch_norm_bwd8(Norm8Params p, float* dgamma, int format, cudaS
   const int sms = sm_count(device);
   const bool vec = p.cols % VW == 0 && p.stride % VW == 0 && a16(p.dy) && a16(p.out) &&
                    reinterpret_cast<uintptr_t>(p.q) % VW == 0;
-  const NormShape h = norm_shape(p.rows, p.cols, vec ? static_cast<int>(sizeof(T)) : 4, bwd8_bytes(sizeof(T)), sms);
+  const NormShape h = norm_shape(p.rows, p.cols, sizeof(T), vec, bwd8_bytes, sms);
   int64_t parts = h.workers;
   unsigned g = h.grid;
   p.chunk = h.chunk;
@@ -846,8 +860,8 @@ vbt_b200_status vbt_b200_rmsnorm_backward8_workspace_bytes(int64_t rows, int64_t
   // whichever form the pointers' alignment takes
   const int sms = sm_count(device), elt = itemsize(dtype);
   int64_t parts = bwd8_stream_blocks(rows, sms);
-  for (int lanes_of : {elt, 4})
-    if (rows > 0 && cols > 0) parts = std::max(parts, norm_shape(rows, cols, lanes_of, bwd8_bytes(elt), sms).workers);
+  for (bool vec : {false, true})
+    if (rows > 0 && cols > 0) parts = std::max(parts, norm_shape(rows, cols, elt, vec, bwd8_bytes, sms).workers);
   *bytes = static_cast<size_t>(parts) * static_cast<size_t>(cols) * 4;
   return VBT_B200_OK;
 }

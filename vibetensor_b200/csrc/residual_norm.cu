@@ -61,21 +61,23 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
   auto buf = [&](int array) { return ring + array * A::WARP_ARRAY; };
 #pragma unroll
   for (int a = 0; a < ARRAYS; ++a) A::zero_rest(buf(a), true, left);
+  const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
   const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
   const float* g2 = p.pre && p.g2 ? p.g2 + j0 : nullptr;
 
   const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   const int64_t begin = min(worker * p.chunk, p.rows);
   const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
-  const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.x_stride + j0;
-  const T* y_at = static_cast<const T*>(p.y) + (begin + rl) * p.y_stride + j0;
-  const T* gate_at = static_cast<const T*>(p.gate) + (begin + rl) * p.gate_stride + j0;  // GATE_ROW
+  const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.x_stride + seg;
+  const T* y_at = static_cast<const T*>(p.y) + (begin + rl) * p.y_stride + seg;
+  const T* gate_at = static_cast<const T*>(p.gate) + (begin + rl) * p.gate_stride + seg;  // GATE_ROW
+  const typename A::Shift x_shift(p.x, p.x_stride), y_shift(p.y, p.y_stride), gate_shift(p.gate, p.gate_stride);
   int ahead = rl;
   auto fetch = [&] {
     if (ahead < todo) {
-      A::copy(buf(0), y_at, left);
-      A::copy(buf(1), x_at, left);
-      if constexpr (GATE_ROW) A::copy(buf(2), gate_at, left);
+      A::copy(buf(0), y_at, seg_left, p.y);
+      A::copy(buf(1), x_at, seg_left, p.x);
+      if constexpr (GATE_ROW) A::copy(buf(2), gate_at, seg_left, p.gate);
     }
     x_at += RW * p.x_stride;
     y_at += RW * p.y_stride;
@@ -101,6 +103,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
       A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
     }
     copy_wait<0>();
+    A::sync();
     float s[1] = {0.f};
     float i1 = 1.f, i2 = 0.f;
     if (p.post) {
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
           float y[C];
-          A::read(buf(0), c, y);
+          A::read(buf(0), y_shift(row), c, left, y);
 #pragma unroll
           for (int e = 0; e < C; ++e) s[0] = fmaf(y[e], y[e], s[0]);
         }
@@ -122,12 +125,12 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float x[C], y[C], w[C];
-        A::read(buf(0), c, y);
-        A::read(buf(1), c, x);
+        A::read(buf(0), y_shift(row), c, left, y);
+        A::read(buf(1), x_shift(row), c, left, x);
         A::read_factors(wbuf, c, w);
         if constexpr (GATE_ROW) {
           float gt[C];
-          A::read(buf(2), c, gt);
+          A::read(buf(2), gate_shift(row), c, left, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }
@@ -139,6 +142,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
         }
       }
     }
+    A::sync();
     fetch();
     if (live) {
 #pragma unroll
@@ -216,11 +220,16 @@ __global__ void __launch_bounds__(512) residual_norm_stream_kernel(const __grid_
   }
 }
 
+// shared memory per thread: two factors, x, y and a gate row
+constexpr int join_bytes(bool gate_row, int elt, bool vec, int tpr) {
+  return kFwdElts * 8 + (gate_row ? 3 : 2) * row_bytes_per_thread(kFwdElts, elt, vec, tpr);
+}
+
 template <class T, int V, int TPR, bool GATE_ROW>
 vbt_b200_status go_join(JoinParams& p, int threads, int sms, unsigned& grid, cudaStream_t s, int device) {
   static std::atomic<uint64_t> done{0};
   VB_CUDA(allow_shared(residual_norm_kernel<T, V, TPR, GATE_ROW>, device, done));
-  const int smem = threads * kFwdElts * (8 + (GATE_ROW ? 3 : 2) * static_cast<int>(sizeof(T)));
+  const int smem = threads * join_bytes(GATE_ROW, sizeof(T), V > 1, TPR);
   const int per_sm = std::max(1, std::min(1024 / threads, kSmemPerSm / (smem + 2048)));
   const int workers = TPR ? threads / 32 : 1;
   // as many workers as fit the card at once, each with a run of rows
@@ -242,7 +251,7 @@ vbt_b200_status launch_join(JoinParams p, cudaStream_t s, int device) {
   const int64_t lanes = (p.cols + kFwdElts - 1) / kFwdElts;
   const int tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
   int threads = tpr ? 256 : static_cast<int>(std::min<int64_t>((lanes + 31) / 32 * 32, 4096));
-  const int smem = threads * kFwdElts * (8 + (gate_row ? 3 : 2) * static_cast<int>(sizeof(T)));
+  const int smem = threads * join_bytes(gate_row, sizeof(T), vec, tpr);
   unsigned g = 0;
   if (threads > kFwdMaxThreads || smem > kSmemPerBlock) {
     threads = 512;

@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       const bool present = a == 0 ? p.dr != nullptr : a == 3 ? p.y != nullptr : a == 4 || p.pre;
       A::zero_rest(buf(st, a), present, left);
     }
+  const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
   const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
   const float* g2p = p.pre && p.g2 ? p.g2 + j0 : nullptr;
   A::fill_factors(gbuf, left, [&](int o) { return g2p ? g2p[o] : 1.f; });
@@ -106,17 +107,21 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     return group * p.per + (u - group * p.cuts) * p.chunk;
   };
   const int64_t row0 = first_row(u0) + rl;
+  const typename A::Shift dr_shift(p.dr, p.dr_stride), dn_shift(p.dn, p.dn_stride), r_shift(p.r, p.r_stride),
+      y_shift(p.y, p.y_stride), gate_shift(p.gate, p.gate_stride);
+  // an absent array reads as zeros
+  const int dr_left = p.dr ? left : 0, pre_left = p.pre ? left : 0, y_left = p.y ? left : 0;
   Walk at;
   at.u = u0;
   at.left = 0;
   at.todo = u0 < u1 ? static_cast<int>(first_row(u1) - first_row(u0)) : 0;
   if (at.todo) at.enter(p);
   Walk ahead = at;
-  const T* dr_at = static_cast<const T*>(p.dr) + row0 * p.dr_stride + j0;
-  const T* dn_at = static_cast<const T*>(p.dn) + row0 * p.dn_stride + j0;
-  const T* r_at = static_cast<const T*>(p.r) + row0 * p.r_stride + j0;
-  const T* y_at = static_cast<const T*>(p.y) + row0 * p.y_stride + j0;
-  const T* gate_at = static_cast<const T*>(p.gate) + row0 * p.gate_stride + j0;  // GATE_ROW
+  const T* dr_at = static_cast<const T*>(p.dr) + row0 * p.dr_stride + seg;
+  const T* dn_at = static_cast<const T*>(p.dn) + row0 * p.dn_stride + seg;
+  const T* r_at = static_cast<const T*>(p.r) + row0 * p.r_stride + seg;
+  const T* y_at = static_cast<const T*>(p.y) + row0 * p.y_stride + seg;
+  const T* gate_at = static_cast<const T*>(p.gate) + row0 * p.gate_stride + seg;  // GATE_ROW
   const float* inv1_at = p.inv1 + row0;
   const float* inv2_at = p.inv2 + row0;
   float i1_next[STAGES], i2_next[STAGES];
@@ -125,14 +130,14 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     i2 = 0.f;
     if (ahead.todo > 0) {
       if (RW == 1 || rl < ahead.left) {
-        if (p.dr) A::copy(buf(stage, 0), dr_at, left);
+        if (p.dr) A::copy(buf(stage, 0), dr_at, seg_left, p.dr);
         if (p.pre) {
-          A::copy(buf(stage, 1), dn_at, left);
-          A::copy(buf(stage, 2), r_at, left);
+          A::copy(buf(stage, 1), dn_at, seg_left, p.dn);
+          A::copy(buf(stage, 2), r_at, seg_left, p.r);
           i2 = *inv2_at;
         }
-        if (p.y) A::copy(buf(stage, 3), y_at, left);
-        if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), gate_at, left);
+        if (p.y) A::copy(buf(stage, 3), y_at, seg_left, p.y);
+        if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), gate_at, seg_left, p.gate);
         if (p.post) i1 = *inv1_at;
       }
       const int n = ahead.next(p);
@@ -163,6 +168,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
   T* dgate = static_cast<T*>(p.dgate) + row0 * p.cols + j0;  // GATE_ROW
   bool first_unit = true, enter = true;
   int phase = 0, stage = 0;
+  int64_t row = row0;
   while (at.todo > 0) {
     if constexpr (MODE == GATE_SHARED) {
       if (enter) {
@@ -171,6 +177,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       }
     }
     copy_wait<STAGES - 1>();
+    A::sync();
     const bool live = RW == 1 || rl < at.left;
     const float i1 = i1_next[0], i2 = i2_next[0];
     float s[3] = {0.f, 0.f, 0.f};
@@ -179,15 +186,15 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float dr[C], dn[C], r[C], y[C], w[C], g2[C];
-        A::read(buf(stage, 0), c, dr);
-        A::read(buf(stage, 1), c, dn);
-        A::read(buf(stage, 2), c, r);
-        A::read(buf(stage, 3), c, y);
+        A::read(buf(stage, 0), dr_shift(row), c, dr_left, dr);
+        A::read(buf(stage, 1), dn_shift(row), c, pre_left, dn);
+        A::read(buf(stage, 2), r_shift(row), c, pre_left, r);
+        A::read(buf(stage, 3), y_shift(row), c, y_left, y);
         A::read_factors(wbuf, c, w);
         A::read_factors(gbuf, c, g2);
         if constexpr (MODE == GATE_ROW) {
           float gt[C];
-          A::read(buf(stage, 4), c, gt);
+          A::read(buf(stage, 4), gate_shift(row), c, left, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }
@@ -210,10 +217,10 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float r[C], y[C], w[C], gt[C], ox[C], oy[C], og[C];
-        A::read(buf(stage, 2), c, r);
-        A::read(buf(stage, 3), c, y);
+        A::read(buf(stage, 2), r_shift(row), c, pre_left, r);
+        A::read(buf(stage, 3), y_shift(row), c, y_left, y);
         A::read_factors(wbuf, c, w);
-        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), c, gt);
+        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), gate_shift(row), c, left, gt);
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           const int i = c * C + e;
@@ -242,10 +249,12 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       i1_next[q] = i1_next[q + 1];
       i2_next[q] = i2_next[q + 1];
     }
+    A::sync();
     fetch(stage, i1_next[STAGES - 1], i2_next[STAGES - 1]);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
     const int64_t unit = at.u;
     const int n = at.next(p);
+    row += n;
     dx += n * p.cols; dy += n * p.cols; dgate += n * p.cols;
     enter = at.todo == 0 || at.u != unit;
     if constexpr (MODE == GATE_SHARED) {
@@ -402,13 +411,13 @@ struct JoinShape {
   int tpr, threads, stages, smem, per_sm;
   int workers() const { return tpr ? threads / 32 : 1; }
 };
-inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row) {
+inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) {
   JoinShape h{0, 0, 0, 0, 4};
   const int64_t lanes = (cols + kBwdElts - 1) / kBwdElts;
   if (lanes > kBwdMaxThreads) return h;
   h.tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
   h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
-  const int factors = 2 * kBwdElts * 4, row = (gate_row ? 5 : 4) * kBwdElts * elt;
+  const int factors = 2 * kBwdElts * 4, row = (gate_row ? 5 : 4) * row_bytes_per_thread(kBwdElts, elt, vec, h.tpr);
   h.stages = h.threads * (factors + 2 * row) <= kSmemPerBlock ? 2 : 1;
   h.smem = h.threads * (factors + h.stages * row);
   if (h.smem > kSmemPerBlock) return JoinShape{0, 0, 0, 0, 4};
@@ -451,7 +460,10 @@ vbt_b200_status go_join_bwd(const JoinBwdParams& p, const JoinShape& h, unsigned
 template <class T>
 vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg2, float* ws, cudaStream_t s, int device) {
   constexpr int VW = 16 / sizeof(T);
-  const JoinShape h = join_bwd_shape(p.cols, sizeof(T), mode == GATE_ROW);
+  const bool vec = p.cols % VW == 0 && p.dr_stride % VW == 0 && p.dn_stride % VW == 0 && p.y_stride % VW == 0 &&
+                   p.r_stride % VW == 0 && p.gate_stride % VW == 0 && a16(p.dr) && a16(p.dn) && a16(p.y) && a16(p.r) &&
+                   a16(p.gate) && a16(p.dx) && a16(p.dy) && a16(p.dgate);
+  const JoinShape h = join_bwd_shape(p.cols, sizeof(T), mode == GATE_ROW, vec);
   const JoinCut cut = join_cut(p.rows, p.per, h, sm_count(device));
   p.chunk = cut.chunk; p.cuts = cut.cuts; p.units = cut.units;
   const unsigned g = static_cast<unsigned>(cut.blocks);
@@ -461,9 +473,6 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
   const bool split_gate = mode == GATE_SHARED && p.dgate != nullptr && cut.cuts > 1;
   // the stream kernel sums a gate row in memory even where it has all its rows
   if (split_gate || (mode == GATE_SHARED && p.dgate != nullptr && h.threads == 0)) p.ws_gate = at;
-  const bool vec = p.cols % VW == 0 && p.dr_stride % VW == 0 && p.dn_stride % VW == 0 && p.y_stride % VW == 0 &&
-                   p.r_stride % VW == 0 && p.gate_stride % VW == 0 && a16(p.dr) && a16(p.dn) && a16(p.y) && a16(p.r) &&
-                   a16(p.gate) && a16(p.dx) && a16(p.dy) && a16(p.dgate);
 #define VB_JB(V, MODE)                                                             \
   (h.tpr == 8      ? go_join_bwd<T, V, 8, MODE, 2>(p, h, g, s, device)             \
    : h.tpr == 16   ? go_join_bwd<T, V, 16, MODE, 2>(p, h, g, s, device)            \
@@ -520,8 +529,8 @@ vbt_b200_status vbt_b200_residual_norm_backward_workspace_bytes(int64_t rows, in
   if (rows == 0) return VBT_B200_OK;
   // a gate row of its own per row is no sum over rows: the rows are cut as if one gate row served all
   const int elt = itemsize(dtype);
-  for (int gate_row = 0; gate_row < 2; ++gate_row) {  // whichever form the gate given takes
-    const JoinShape h = join_bwd_shape(cols, elt, gate_row);
+  for (int form = 0; form < 4; ++form) {  // whichever the gate given and the pointers' alignment take
+    const JoinShape h = join_bwd_shape(cols, elt, form & 1, form & 2);
     const JoinCut c = join_cut(rows, rows_per_gate == 1 ? rows : rows_per_gate, h, sm_count(device));
     *bytes = std::max(*bytes, join_bwd_floats(c, h) * static_cast<size_t>(cols) * 4);
   }

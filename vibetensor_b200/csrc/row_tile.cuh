@@ -118,76 +118,106 @@ __device__ __forceinline__ void narrow2(__half* p, float2 v) { *reinterpret_cast
 
 // A thread's E values of a row, worked on in chunks of C: V neighbours for V-value vectors, two
 // single values for V = 1.  TPR lanes of a warp share a row, or (TPR = 0) every warp of the block owns
-// 32 E neighbouring values of it; either way the columns of a thread's chunks and their places in
-// shared memory are compile-time offsets from one base.  A thread has slots of its own in every
-// buffer: what it copied it may read after its own wait, without a barrier.
+// a segment of 32 E neighbouring values of it; either way the columns of a thread's chunks and their
+// places in shared memory are compile-time offsets from one base.
+//
+// V > 1 (16-byte aligned rows): a thread has slots of its own in every buffer; what it copied it may
+// read after its own wait, without a barrier.
+// V = 1 (any alignment): the lanes of a segment copy the 16-byte granules that cover it, whole, and
+// read single values behind the segment's shift against a 16-byte boundary; sync() stands between the
+// wait and the reads, and between the reads and the next copy.  Nothing in front of the tensor's
+// first value or behind the row's last is read.  (Copies of single 4-byte values ran [6151,1365] fp32
+// at half the rate, and 2-byte ones cannot be asynchronous.)
 template <class T, int V, int TPR, int E> struct RowChunks {
   static constexpr int C = V > 1 ? V : 2;
   static constexpr int N = E / C;
   static constexpr int STEP = TPR ? TPR : 32;
-  static constexpr int WARP_ARRAY = 32 * E * static_cast<int>(sizeof(T));  // bytes of one array in a warp's part
+  static constexpr int ELT = static_cast<int>(sizeof(T));
+  static constexpr int REGION = STEP * E * ELT + (V > 1 ? 0 : 16);  // bytes of one row's segment
+  static constexpr int WARP_ARRAY = 32 / STEP * REGION;             // of one array in a warp's part
   static constexpr int WARP_FACTORS = 32 * E * 4;
   static constexpr int FW = C >= 4 ? 4 : 2;  // fp32 factors per access
-  // first column of this thread
-  static __device__ __forceinline__ int base() {
-    return TPR ? static_cast<int>(threadIdx.x % STEP) * V : static_cast<int>(threadIdx.x >> 5) * (32 * E) + static_cast<int>(threadIdx.x & 31) * V;
-  }
+  static_assert(V == 1 || V * ELT <= 16, "one vector per slot");
+
+  static __device__ __forceinline__ int lane() { return static_cast<int>(threadIdx.x & 31) % STEP; }
+  // first column of this thread's segment, and of this thread
+  static __device__ __forceinline__ int segment() { return TPR ? 0 : static_cast<int>(threadIdx.x >> 5) * (32 * E); }
+  static __device__ __forceinline__ int base() { return segment() + lane() * V; }
   // offset of element e of chunk c from it
   static __device__ __forceinline__ constexpr int off(int c, int e) { return V > 1 ? c * STEP * V + e : (2 * c + e) * STEP; }
-  // a warp's array in shared memory -> the thread's slot for chunk c (element e for V = 1)
-  static __device__ __forceinline__ T* slot(unsigned char* array, int c, int e) {
-    return reinterpret_cast<T*>(array) + (V > 1 ? c : 2 * c + e) * (32 * V) + static_cast<int>(threadIdx.x & 31) * V;
+  static __device__ __forceinline__ unsigned char* region(unsigned char* array) {
+    return array + (V > 1 ? 0 : static_cast<int>(threadIdx.x & 31) / STEP * REGION);
   }
-  // starts the copies of the thread's part of a row; `row` points at the thread's first column, `left`
-  // values of the row lie from there on (single values of less than four bytes are copied at once: they
-  // are smaller than the smallest asynchronous copy)
-  static __device__ __forceinline__ void copy(unsigned char* array, const T* row, int left) {
+  // V > 1: the thread's slot for chunk c
+  static __device__ __forceinline__ T* slot(unsigned char* array, int c) {
+    return reinterpret_cast<T*>(array) + c * (32 * V) + static_cast<int>(threadIdx.x & 31) * V;
+  }
+  static __device__ __forceinline__ void sync() {
+    if constexpr (V == 1) __syncwarp();
+  }
+  // the shift of a row's segment: rows of `stride` values from `first` on
+  struct Shift {
+    int at0, step;
+    __device__ __forceinline__ Shift(const void* first, int64_t stride)
+        : at0(static_cast<int>(reinterpret_cast<uintptr_t>(first) & 15)), step(static_cast<int>(stride * ELT) & 15) {}
+    __device__ __forceinline__ int operator()(int64_t row) const {
+      return V > 1 ? 0 : (at0 + (static_cast<int>(row) & 15) * step) & 15;
+    }
+  };
+  // starts the copies of a segment: `seg` points at its first column, `len` values of the row lie from
+  // there on, `floor` is the tensor's first value
+  static __device__ __forceinline__ void copy(unsigned char* array, const T* seg, int len, const void* floor) {
+    if constexpr (V > 1) {
+      const int left = len - lane() * V;
+      const T* row = seg + lane() * V;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      if constexpr (V > 1) {
-        if (off(c, 0) < left) copy_async<V * static_cast<int>(sizeof(T))>(slot(array, c, 0), row + off(c, 0));
-      } else if constexpr (sizeof(T) == 4) {
+      for (int c = 0; c < N; ++c)
+        if (off(c, 0) < left) copy_async<V * ELT>(slot(array, c), row + off(c, 0));
+    } else {
+      if (len <= 0) return;
+      const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(seg) & 15);
+      const unsigned char* from = reinterpret_cast<const unsigned char*>(seg) - shift;
+      const int bytes = shift + min(len, STEP * E) * ELT;
+      unsigned char* to = region(array);
+      constexpr int GRANULES = STEP * E * ELT / 16 + 1;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (off(c, e) < left) copy_async<4>(slot(array, c, e), row + off(c, e));
+      for (int i = 0; i < (GRANULES + STEP - 1) / STEP; ++i) {
+        const int at = (lane() + i * STEP) * 16;
+        if (at >= bytes) break;
+        if (i == 0 && at == 0 && from < floor) {
+          for (int e = shift; e < min(16, bytes); e += ELT)
+            *reinterpret_cast<T*>(to + e) = *reinterpret_cast<const T*>(from + e);
+        } else {
+          const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(to + at));
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from + at), "r"(min(16, bytes - at)) : "memory");
+        }
       }
     }
-    if constexpr (V == 1 && sizeof(T) < 4) {
-      T v[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (i * STEP < left) v[i] = row[i * STEP];
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (i * STEP < left) *slot(array, i / 2, i & 1) = v[i];
-    }
   }
-  // zeros where no copy ever lands: behind the row's end, or everywhere if the array is absent
+  // V > 1: zeros where no copy ever lands: behind the row's end, or everywhere if the array is absent.
+  // V = 1 reads nothing there.
   static __device__ __forceinline__ void zero_rest(unsigned char* array, bool present, int left) {
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-#pragma unroll
-      for (int e = 0; e < C; ++e)
-        if (!present || off(c, e) >= left) (V > 1 ? slot(array, c, 0)[e] : *slot(array, c, e)) = T{};
-  }
-  static __device__ __forceinline__ void read(unsigned char* array, int c, float (&v)[C]) {
     if constexpr (V > 1) {
-      const Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(slot(array, c, 0));
 #pragma unroll
-      for (int e = 0; e < C; ++e) v[e] = to_f(raw.v[e]);
-    } else {
-      v[0] = to_f(*slot(array, c, 0));
-      v[1] = to_f(*slot(array, c, 1));
+      for (int c = 0; c < N; ++c)
+        if (!present || off(c, 0) >= left) *reinterpret_cast<Vec<T, V>*>(slot(array, c)) = Vec<T, V>{};
     }
   }
-  // the same without the conversion
-  static __device__ __forceinline__ void read_raw(unsigned char* array, int c, Vec<T, C>& v) {
+  static __device__ __forceinline__ void read_raw(unsigned char* array, int shift, int c, int left, Vec<T, C>& v) {
     if constexpr (V > 1) {
-      v = *reinterpret_cast<const Vec<T, V>*>(slot(array, c, 0));
+      v = *reinterpret_cast<const Vec<T, V>*>(slot(array, c));
     } else {
-      v.v[0] = *slot(array, c, 0);
-      v.v[1] = *slot(array, c, 1);
+      const T* row = reinterpret_cast<const T*>(region(array) + shift) + lane();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v.v[e] = off(c, e) < left ? row[off(c, e)] : T{};
     }
+  }
+  // `left`: values of the row from the thread's first column on, 0 if the array is absent
+  static __device__ __forceinline__ void read(unsigned char* array, int shift, int c, int left, float (&v)[C]) {
+    Vec<T, C> raw;
+    read_raw(array, shift, c, left, raw);
+#pragma unroll
+    for (int e = 0; e < C; ++e) v[e] = to_f(raw.v[e]);
   }
   static __device__ __forceinline__ void write(T* row, int c, int left, const float (&v)[C]) {
     if constexpr (V > 1) {
@@ -226,6 +256,15 @@ template <class T, int V, int TPR, int E> struct RowChunks {
       }
   }
 };
+// A thread's share of RowChunks::WARP_ARRAY, rounded up.
+constexpr int row_bytes_per_thread(int elts, int elt, bool vec, int tpr) {
+  const int step = tpr ? tpr : 32;
+  return elts * elt + (vec ? 0 : (16 + step - 1) / step);
+}
+static_assert(32 * row_bytes_per_thread(16, 2, false, 0) >= RowChunks<__half, 1, 0, 16>::WARP_ARRAY &&
+              32 * row_bytes_per_thread(16, 4, false, 8) >= RowChunks<float, 1, 8, 16>::WARP_ARRAY &&
+              32 * row_bytes_per_thread(16, 1, false, 16) >= RowChunks<uint8_t, 1, 16, 16>::WARP_ARRAY &&
+              32 * row_bytes_per_thread(16, 2, true, 32) >= RowChunks<__half, 8, 32, 16>::WARP_ARRAY);
 
 // Sums over the threads that share a row: TPR lanes of a warp, or the whole block (TPR = 0; `red`
 // holds two phases, so one barrier per call is enough).  N <= 4.
