@@ -418,11 +418,15 @@ inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) 
   h.tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
   h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
   const int factors = 2 * kBwdElts * 4, row = (gate_row ? 5 : 4) * row_bytes_per_thread(kBwdElts, elt, vec, h.tpr);
-  h.stages = h.threads * (factors + 2 * row) <= kSmemPerBlock ? 2 : 1;
-  h.smem = h.threads * (factors + h.stages * row);
-  if (h.smem > kSmemPerBlock) return JoinShape{0, 0, 0, 0, 4};
+  auto smem = [&](int stages) { return h.threads * (factors + stages * row); };
   // registers allow 512 threads per SM (128 each)
-  h.per_sm = std::max(1, std::min(512 / h.threads, kSmemPerSm / (h.smem + 2048)));
+  auto per_sm = [&](int stages) { return std::max(1, std::min(512 / h.threads, kSmemPerSm / (smem(stages) + 2048))); };
+  // two rows ahead where they fit; the warp forms are built for that alone
+  h.stages = 2;
+  if (!h.tpr && smem(2) > kSmemPerBlock) h.stages = 1;
+  h.smem = smem(h.stages);
+  if (h.smem > kSmemPerBlock) return JoinShape{0, 0, 0, 0, 4};
+  h.per_sm = per_sm(h.stages);
   return h;
 }
 // How the rows are cut: units of `chunk` rows, `cuts` of them per gate row.  As many units as there
