@@ -617,8 +617,8 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd8_stream_kernel(const __grid_c
   }
 }
 
-__global__ void __launch_bounds__(256) rmsnorm_bwd8_fold_kernel(float* dgamma, const float* ws, int64_t parts, int64_t cols) {
-  __shared__ float sm[8][8];
+__global__ void __launch_bounds__(kStripThreads) rmsnorm_bwd8_fold_kernel(float* dgamma, const float* ws, int64_t parts, int64_t cols) {
+  __shared__ float sm[kStripThreads / 32][8];
   const float s = strip_sum(ws, parts, cols, sm);
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x;
   if (threadIdx.x < 8 && c < cols) dgamma[c] = s;
@@ -774,7 +774,7 @@ vbt_b200_status launch_norm_bwd8(Norm8Params p, float* dgamma, int format, cudaS
     VB_ROW8_ALL(rmsnorm_bwd8_kernel);
   }
   VB_LAUNCH_CHECK();
-  if (p.ws) rmsnorm_bwd8_fold_kernel<<<static_cast<unsigned>((p.cols + 7) / 8), 256, 0, s>>>(dgamma, p.ws, parts, p.cols);
+  if (p.ws) rmsnorm_bwd8_fold_kernel<<<static_cast<unsigned>((p.cols + 7) / 8), kStripThreads, 0, s>>>(dgamma, p.ws, parts, p.cols);
   VB_LAUNCH_CHECK();
   note_launch(VBT_B200_FAMILY_ROWOP, VBT_B200_WK_RMSNORM_BACKWARD8, dim3(g), dim3(h.threads ? h.threads : 256), vec ? VW : 1,
               1, 0, p.ws ? 2 : 1, p.rows * p.cols, p.cols, p.ws ? static_cast<size_t>(parts) * p.cols * 4 : 0, s);

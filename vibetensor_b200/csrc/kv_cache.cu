@@ -50,13 +50,11 @@ __global__ void __launch_bounds__(kKvThreads) kv_claim_kernel(const __grid_const
 }
 
 constexpr int kKvMaxTokens = 32;  // tokens of a block
-constexpr int kKvWriteRows = 2;   // rows in flight per thread
 
 // L lanes own a row; VEC: 16-byte vectors, VPL of them per lane; else single values, the row read twice
 template <class T, bool VEC, int L, int VPL, int F>
 __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
   constexpr int V = 16 / sizeof(T);
-  constexpr int U = VPL == 1 && VEC ? kKvWriteRows : 1;
   __shared__ int64_t slot_of[kKvMaxTokens];
   __shared__ int later[kKvMaxTokens];
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tb;
@@ -85,52 +83,40 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const __grid_const
   }
   const int lane = threadIdx.x % L;
   const int rows = tb * 2 * p.heads;
-  // every lane of a warp makes the same number of rounds (shuffles inside); U rows of a thread are in
-  // flight at once
-  constexpr int S = kKvThreads / L;
-  for (int r0 = 0; r0 < rows; r0 += S * U) {
-    const T* src[U];
-    int64_t row[U];
-    int side[U];
-    Vec<T, V> raw[U][VPL];
+  // every lane of a warp makes the same number of rounds (shuffles inside)
+  for (int r0 = 0; r0 < rows; r0 += kKvThreads / L) {
+    const int r = r0 + threadIdx.x / L;
+    uint32_t tk = 0, h = 0;
+    if (r < rows) p.div_heads.divmod(static_cast<uint32_t>(r), tk, h);
+    const int kv = tk & 1, tok = tk >> 1;
+    const int64_t slot = r < rows && !later[tok] ? slot_of[tok] : -1;
+    const bool live = slot >= 0;
+    const int64_t row = live ? slot * p.heads + h : 0;
+    const T* src = static_cast<const T*>(p.src[kv]) + (first + tok) * p.src_t[kv] + static_cast<int64_t>(h) * p.src_h[kv];
+    uint8_t* dst = p.cache[kv] + row * p.dim;
+    Q8Scale s;
+    if constexpr (VEC) {
+      const int nv = live ? p.dim / V : 0;
+      Vec<T, V> raw[VPL];
+      load_vecs<T, V, VPL>(src, lane, L, nv, raw);
+      s = q8_scale<F>(group_mag<T, V, VPL, L>(raw));
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * S + threadIdx.x / L;
-      uint32_t tk = 0, h = 0;
-      if (r < rows) p.div_heads.divmod(static_cast<uint32_t>(r), tk, h);
-      const int kv = tk & 1, tok = tk >> 1;
-      const int64_t slot = r < rows && !later[tok] ? slot_of[tok] : -1;
-      side[u] = kv;
-      row[u] = slot < 0 ? -1 : slot * p.heads + h;
-      src[u] = static_cast<const T*>(p.src[kv]) + (first + tok) * p.src_t[kv] + static_cast<int64_t>(h) * p.src_h[kv];
-      if constexpr (VEC) load_vecs<T, V, VPL>(src[u], lane, L, slot < 0 ? 0 : p.dim / V, raw[u]);
-    }
+      for (int k = 0; k < VPL; ++k) {
+        const int j = lane + k * L;
+        if (j >= nv) continue;
+        float v[V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool live = row[u] >= 0;
-      uint8_t* dst = p.cache[side[u]] + (live ? row[u] : 0) * p.dim;
-      Q8Scale s;
-      if constexpr (VEC) {
-        s = q8_scale<F>(group_mag<T, V, VPL, L>(raw[u]));
-        const int nv = live ? p.dim / V : 0;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-          const int j = lane + k * L;
-          if (j >= nv) continue;
-          float v[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) v[e] = to_f(raw[u][k].v[e]);
-          q8_store<F, V>(dst + j * V, v, s.up);
-        }
-      } else {
-        const int n = live ? p.dim : 0;
-        uint32_t m = 0;
-        for (int j = lane; j < n; j += L) m = max(m, mag_bits(to_f(src[u][j])));
-        s = q8_scale<F>(lanes_max<L>(m));
-        for (int j = lane; j < n; j += L) dst[j] = q8_pack1<F>(to_f(src[u][j]), s.up);
+        for (int e = 0; e < V; ++e) v[e] = to_f(raw[k].v[e]);
+        q8_store<F, V>(dst + j * V, v, s.up);
       }
-      if (live && lane == 0) p.scale[side[u]][row[u]] = s.down;
+    } else {
+      const int n = live ? p.dim : 0;
+      uint32_t m = 0;
+      for (int j = lane; j < n; j += L) m = max(m, mag_bits(to_f(src[j])));
+      s = q8_scale<F>(lanes_max<L>(m));
+      for (int j = lane; j < n; j += L) dst[j] = q8_pack1<F>(to_f(src[j]), s.up);
     }
+    if (live && lane == 0) p.scale[kv][row] = s.down;
   }
 }
 
@@ -258,7 +244,9 @@ int launch_write(KvWriteParams p, int format, cudaStream_t s) {
   for (int i = 0; i < 2; ++i)
     vec = vec && aligned(p.src[i], 16) && aligned(p.cache[i], 8) && p.src_t[i] % V == 0 && p.src_h[i] % V == 0;
   const int nv = vec ? p.dim / V : 0;
-  const int lanes = !vec || nv > 16 ? 32 : nv > 8 ? 16 : nv > 4 ? 8 : 4;
+  // four vectors per lane: what a lane works out per row (slot, addresses, the scale) is shared by 32 or
+  // 64 bytes of it.  135,000 tokens of 8 heads x 128 bf16: one vector per lane 200 us, two 155, four 133
+  const int lanes = !vec || nv > 64 ? 32 : nv > 32 ? 16 : nv > 16 ? 8 : nv > 8 ? 4 : 2;
   // about eight rounds of rows per thread, as long as the card is full of blocks
   const int64_t rows = 2 * int64_t{p.heads};
   int64_t tb = std::max<int64_t>(1, 8 * (kKvThreads / lanes) / rows);
@@ -273,11 +261,10 @@ int launch_write(KvWriteParams p, int format, cudaStream_t s) {
   const unsigned g = static_cast<unsigned>((p.tokens + p.tb - 1) / p.tb);
 #define VB_KW(VEC, L, VPL) VB_KV_FORMAT(format, F, (kv_write_kernel<T, VEC, L, VPL, F><<<g, kKvThreads, 0, s>>>(p)))
   if (!vec) VB_KW(false, 32, 1);
-  else if (nv <= 4) VB_KW(true, 4, 1);
-  else if (nv <= 8) VB_KW(true, 8, 1);
-  else if (nv <= 16) VB_KW(true, 16, 1);
-  else if (nv <= 32) VB_KW(true, 32, 1);
-  else if (nv <= 64) VB_KW(true, 32, 2);
+  else if (nv <= 8) VB_KW(true, 2, 4);
+  else if (nv <= 16) VB_KW(true, 4, 4);
+  else if (nv <= 32) VB_KW(true, 8, 4);
+  else if (nv <= 64) VB_KW(true, 16, 4);
   else VB_KW(true, 32, 8);
 #undef VB_KW
   note_launch(VBT_B200_FAMILY_INDEX, VBT_B200_IK_KV_CACHE_WRITE, dim3(g), dim3(kKvThreads), vec ? V : 1, 1, 0, launches,

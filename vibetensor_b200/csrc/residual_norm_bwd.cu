@@ -374,32 +374,53 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_stream_kernel(const __g
   }
 }
 
-// Column sums of partial rows in a fixed order: blockIdx.y 0 and 1 fold dgamma_post and
-// dgamma_pre over the blocks' rows, the others a gate row each over its units.  A block owns a strip of 8
-// columns (one 32-byte sector per partial row); its 256 threads take 32 rows per step.
+// Column sums of partial rows in a fixed order.  blockIdx.y says which: dgamma_post and dgamma_pre over the
+// workers' rows, the gradient of one gate row that serves all over its units.
 struct JoinFoldParams {
-  float* out1;
-  float* out2;
+  float* out[2];
+  const float* ws[2];
   void* dgate;
-  const float* ws1;
-  const float* ws2;
   const float* ws_gate;
-  int64_t cols, parts, cuts, gates;
-  int first;  // what blockIdx.y == 0 stands for
+  int64_t cols, parts, cuts;
+  int what[3];
 };
 template <class T>
-__global__ void __launch_bounds__(256) residual_norm_fold_kernel(const __grid_constant__ JoinFoldParams p) {
-  __shared__ float sm[8][8];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x & 7);
-  for (int64_t what = blockIdx.y + p.first; what < p.gates + 2; what += gridDim.y) {
-    if ((what == 0 && !p.out1) || (what == 1 && !p.out2)) continue;
-    const float* src = what == 0 ? p.ws1 : what == 1 ? p.ws2 : p.ws_gate + (what - 2) * p.cuts * p.cols;
-    const int64_t n = what < 2 ? p.parts : p.cuts;
-    const float s = strip_sum(src, n, p.cols, sm);
-    if (threadIdx.x < 8 && c < p.cols) {
-      if (what == 0) p.out1[c] = s;
-      else if (what == 1) p.out2[c] = s;
-      else static_cast<T*>(p.dgate)[(what - 2) * p.cols + c] = from_f<T>(s);
+__global__ void __launch_bounds__(kStripThreads) residual_norm_fold_kernel(const __grid_constant__ JoinFoldParams p) {
+  __shared__ float sm[kStripThreads / 32][8];
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x;
+  const int what = p.what[blockIdx.y];
+  const float s = what < 2 ? strip_sum(p.ws[what], p.parts, p.cols, sm) : strip_sum(p.ws_gate, p.cuts, p.cols, sm);
+  if (threadIdx.x < 8 && c < p.cols) {
+    if (what < 2) p.out[what][c] = s;
+    else static_cast<T*>(p.dgate)[c] = from_f<T>(s);
+  }
+}
+// Several gate rows, few units each: 32 columns per block, eight warps take every eighth unit.
+template <class T>
+__global__ void __launch_bounds__(256) residual_norm_gate_fold_kernel(T* dgate, const float* ws, int64_t cuts, int64_t cols,
+                                                                      int64_t gates) {
+  __shared__ float sm[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  for (int64_t g = blockIdx.y; g < gates; g += gridDim.y) {
+    const float* src = ws + g * cuts * cols + c;
+    float acc = 0.f;
+    if (c < cols) {
+      for (int64_t r = w; r < cuts; r += 8 * 8) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = r + 8 * q < cuts ? __ldcg(src + (r + 8 * q) * cols) : 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc += v[q];
+      }
+    }
+    sm[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && c < cols) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += sm[k][lane];
+      dgate[g * cols + c] = from_f<T>(s);
     }
     __syncthreads();
   }
@@ -429,8 +450,10 @@ inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) 
   h.per_sm = per_sm(h.stages);
   return h;
 }
-// How the rows are cut: units of `chunk` rows, `cuts` of them per gate row.  As many units as there
-// are workers on the card, unless that leaves a worker's unit less than its rows at a time.
+// How the rows are cut: units of `chunk` rows, `cuts` of them per gate row, dealt out evenly to the
+// workers that fit the card.  At least as many units as workers, and up to eight times that where it
+// evens out what a worker gets (30 gate rows of 1000 rows of 4096 on 296 workers: 463 us with as many units
+// as workers, 335 with more); the end of a unit is counted as eight steps.
 struct JoinCut {
   int64_t chunk, cuts, units, blocks, workers;
 };
@@ -438,11 +461,21 @@ inline JoinCut join_cut(int64_t rows, int64_t per, const JoinShape& h, int sms) 
   const int per_block = h.threads ? h.workers() : 1;
   const int64_t groups = rows / per, most = int64_t{sms} * h.per_sm * per_block;
   const int64_t at_once = h.tpr ? 32 / h.tpr : 1;
-  JoinCut c;
-  c.cuts = std::max<int64_t>(1, std::min<int64_t>((per + at_once - 1) / at_once, (most + groups - 1) / groups));
-  c.chunk = (per + c.cuts - 1) / c.cuts;
-  c.cuts = (per + c.chunk - 1) / c.chunk;
-  c.units = groups * c.cuts;
+  const int64_t least = (most + groups - 1) / groups, finest = (per + at_once - 1) / at_once;
+  JoinCut c{};
+  int64_t best = INT64_MAX;
+  for (int k = 1; k <= 8; ++k) {
+    const int64_t want = std::min(finest, least * k);
+    const int64_t steps = (finest + want - 1) / want;  // of a unit
+    const int64_t cuts = (finest + steps - 1) / steps, units = groups * cuts;
+    const int64_t cost = (units + most - 1) / most * (steps + 8);
+    if (cost < best) {
+      best = cost;
+      c.chunk = steps * at_once;
+      c.cuts = cuts;
+      c.units = units;
+    }
+  }
   c.blocks = (std::min<int64_t>(c.units, most) + per_block - 1) / per_block;
   c.workers = c.blocks * per_block;
   return c;
@@ -497,15 +530,23 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
   VB_LAUNCH_CHECK();
   const int threads = h.threads ? h.threads : 512;
   int launches = 1;
-  if (dg1 || dg2 || split_gate) {
-    JoinFoldParams f{};
-    f.out1 = dg1; f.out2 = dg2; f.dgate = p.dgate;
-    f.ws1 = p.ws_g1; f.ws2 = p.ws_g2; f.ws_gate = p.ws_gate;
-    f.cols = p.cols; f.parts = cut.workers; f.cuts = cut.cuts; f.gates = split_gate ? p.rows / p.per : 0;
-    f.first = dg1 ? 0 : dg2 ? 1 : 2;
-    const int64_t ny = f.gates + 2 - f.first;
-    dim3 fg(static_cast<unsigned>((p.cols + 7) / 8), static_cast<unsigned>(std::min<int64_t>(ny, 65535)));
-    residual_norm_fold_kernel<T><<<fg, 256, 0, s>>>(f);
+  const int64_t gates = p.rows / p.per;
+  JoinFoldParams f{};
+  f.out[0] = dg1; f.out[1] = dg2; f.ws[0] = p.ws_g1; f.ws[1] = p.ws_g2;
+  f.dgate = p.dgate; f.ws_gate = p.ws_gate;
+  f.cols = p.cols; f.parts = cut.workers; f.cuts = cut.cuts;
+  unsigned sums = 0;
+  if (dg1) f.what[sums++] = 0;
+  if (dg2) f.what[sums++] = 1;
+  if (split_gate && gates == 1) f.what[sums++] = 2;
+  if (sums) {
+    residual_norm_fold_kernel<T><<<dim3(static_cast<unsigned>((p.cols + 7) / 8), sums), kStripThreads, 0, s>>>(f);
+    VB_LAUNCH_CHECK();
+    ++launches;
+  }
+  if (split_gate && gates > 1) {
+    const dim3 grid(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(std::min<int64_t>(gates, 65535)));
+    residual_norm_gate_fold_kernel<T><<<grid, 256, 0, s>>>(static_cast<T*>(p.dgate), p.ws_gate, cut.cuts, p.cols, gates);
     VB_LAUNCH_CHECK();
     ++launches;
   }

@@ -71,18 +71,20 @@ __device__ __forceinline__ void load_floats(const float* src, int j, int nvec, f
 }
 inline bool a16(const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; }
 
-// Sums the n rows of src[n][cols] for the 8 columns of a strip (one
-// 32-byte sector per row) with 256 threads, in a fixed order; the sum of column `lane` is returned
-// to the first 8 lanes of warp 0.  `sm` is free again at the next barrier behind the call.
+// Sums the n rows of src[n][cols] for the 8 columns of a strip (one 32-byte sector per row) with
+// kStripThreads threads, in a fixed order; the sum of column `lane` is returned to the first 8 lanes of
+// warp 0.  `sm` is free again at the next barrier behind the call.  128 rows per step keep the ~600
+// partial rows of a launch to one step: with 256 threads the fold of [586,4096] took 10 us.
+constexpr int kStripThreads = 1024;
 __device__ __forceinline__ float strip_sum(const float* src, int64_t n, int64_t cols, float (*sm)[8]) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + (lane & 7);
   float acc = 0.f;
   if (c < cols) {
-    for (int64_t r = w * 4 + (lane >> 3); r < n; r += 8 * 32) {
+    for (int64_t r = w * 4 + (lane >> 3); r < n; r += 8 * 128) {
       float v[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = r + 32 * q < n ? __ldcg(src + (r + 32 * q) * cols + c) : 0.f;
+      for (int q = 0; q < 8; ++q) v[q] = r + 128 * q < n ? __ldcg(src + (r + 128 * q) * cols + c) : 0.f;
 #pragma unroll
       for (int q = 0; q < 8; ++q) acc += v[q];
     }
@@ -94,7 +96,7 @@ __device__ __forceinline__ float strip_sum(const float* src, int64_t n, int64_t 
   float s = 0.f;
   if (w == 0 && lane < 8)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += sm[k][lane];
+    for (int k = 0; k < kStripThreads / 32; ++k) s += sm[k][lane];
   return s;
 }
 
