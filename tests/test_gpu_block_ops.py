@@ -3,10 +3,10 @@ plain 64-bit forms of their formulas.
 
 Tolerances are derived, not fitted.  u = 2^-24 is half a step of fp32.  A value computed in fp32 from
 terms of total magnitude M is off by at most K * u * M, where K counts the roundings on the longest
-path: a row sum is sequential over at most cols / 256 values per thread plus a tree of at most 15
-levels, a sum over rows over at most rows / 296 rows per block plus the fold (at most 8 rows per
+path: a row sum is sequential over at most 137 values per thread (70001 / 512 and 20001 / 256 in the
+kernels for rows of any length, 16 in the others) plus a tree of at most 15 levels, a sum over rows over at most rows / 296 rows per block plus the fold (at most 8 rows per
 thread and step, 15 levels), square roots, exponentials and sines add at most 4 each, the products
-around them at most 10.  K = 128 covers every size below (20001 / 256 + 15 + 14 < 128).  Storing to t
+around them at most 10.  K = 192 covers every size below (137 + 15 + 14 < 192).  Storing to t
 adds half a step, eps(t) / 2 relative, and half the smallest subnormal.  8-bit levels and scales are a
 fixed sequence of correctly rounded fp32 operations: they are compared bit for bit."""
 import ctypes
@@ -19,7 +19,7 @@ from tests.util import note_worst
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
-U, K = 2.0 ** -24, 128
+U, K = 2.0 ** -24, 192
 TINY = {F32: 2.0 ** -149, F16: 2.0 ** -24, BF16: 2.0 ** -133}
 
 
@@ -127,7 +127,8 @@ def gate_for(g, kind, shape, dtype):
 
 
 # one width per kernel variant, with the odd ones that take single values
-COLS = [1, 7, 64, 128, 200, 333, 512, 1000, 1365, 2048, 4096, 5000, 8192, 12345, 16384, 16400, 20001]
+COLS = [1, 7, 64, 128, 200, 333, 512, 1000, 1365, 2048, 4096, 5000, 8192, 12345, 16384, 16400, 20001,
+        33000, 70001]
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])

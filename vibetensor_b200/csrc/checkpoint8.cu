@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
   constexpr int GC = V > 1 ? 1 : 2, GL = V > 1 ? kQ8Group / V : 32;
   static_assert(A::STEP % GL == 0, "a group's lanes are neighbours");
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float4 red[2][32];
+  __shared__ float4 red[2][TPR ? 1 : 32];
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
   const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
     if (r0 + RW + rl < todo) A::copy(xbuf, x_at, seg_left, p.x);
     copy_commit();
     if (!live) s[0] = 0.f;
-    sum_row<TPR, 1>(s, red, phase);
+    sum_row<TPR, 1>(s, &red[0][0], phase);
     const float inv = rsqrtf(s[0] * inv_cols + p.eps);
     if (live) {
 #pragma unroll
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
   constexpr int GC = V > 1 ? 1 : 2;    // chunks of this thread in one group
   constexpr int NS = A::N / GC;        // scales of this thread
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float4 red[2][32];
+  __shared__ float4 red[2][TPR ? 1 : 32];
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
   const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
         }
       }
     }
-    sum_row<TPR, 1>(s, red, phase);
+    sum_row<TPR, 1>(s, &red[0][0], phase);
     const float k = inv * inv * inv * s[0] * inv_cols;
     if (live) {
 #pragma unroll
@@ -699,9 +699,9 @@ inline NormShape norm_shape(int64_t rows, int64_t cols, int elt, bool vec, Bytes
   h.tpr = lanes <= 16 && elt == 2 && vec ? 16 : lanes <= 32 ? 32 : 0;
   h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
   h.smem = h.threads * bytes(elt, vec, h.tpr);
-  if (h.smem > kSmemPerBlock) return NormShape{};
+  if (h.smem > kSmemPerBlock - 1024) return NormShape{};
   const int per_block = h.tpr ? h.threads / 32 : 1;
-  const int per_sm = std::max(1, std::min(1024 / h.threads, kSmemPerSm / (h.smem + 2048)));
+  const int per_sm = std::max(1, std::min(1024 / h.threads, kSmemPerSm / (h.smem + (h.tpr ? 1024 : 2048))));
   const int64_t most = int64_t{sms} * per_sm * per_block;
   h.chunk = (rows + most - 1) / most;
   h.grid = static_cast<unsigned>(((rows + h.chunk - 1) / h.chunk + per_block - 1) / per_block);
@@ -717,7 +717,7 @@ constexpr int bwd8_bytes(int elt, bool vec, int tpr) {
 #define VB_ROW8(KERNEL, V, TPR)                                                       \
   VB_FORMAT(format, F, do {                                                           \
     static std::atomic<uint64_t> done{0};                                             \
-    VB_CUDA(allow_shared(KERNEL<T, V, TPR, F>, device, done));                        \
+    VB_CUDA(allow_shared(KERNEL<T, V, TPR, F>, device, done, kSmemPerBlock - 1024));                       \
     KERNEL<T, V, TPR, F><<<h.grid, h.threads, h.smem, s>>>(p);                        \
   } while (0))
 // single values of 16 bits may share a row between 32 lanes only (a group lies in 32 of them)

@@ -27,6 +27,7 @@ struct JoinParams {
   int64_t x_stride, y_stride, gate_stride;  // elements
   int64_t per;                              // rows that share a gate row
   int64_t chunk;                            // rows of a worker
+  int ranks;                                // blocks that share a row
   float a, b, eps;
   int post, pre;
 };
@@ -51,21 +52,24 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
   constexpr int RW = TPR ? 32 / TPR : 1;
   constexpr int ARRAYS = GATE_ROW ? 3 : 2;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float4 red[2][32];
+    const int ranks = TPR ? 1 : p.ranks;
+  const int warp0 = ranks > 1 ? cluster_rank() * static_cast<int>(blockDim.x >> 5) : 0;
+  if (ranks > 1) cluster_sync();  // the other blocks' shared memory is there
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
-  const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
+  const int j0 = A::base(warp0), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
   unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + ARRAYS * A::WARP_ARRAY);
+  float4* red = reinterpret_cast<float4*>(smem + static_cast<size_t>(blockDim.x >> 5) * (2 * A::WARP_FACTORS + ARRAYS * A::WARP_ARRAY));
   unsigned char* gbuf = wbuf + A::WARP_FACTORS;
   unsigned char* ring = gbuf + A::WARP_FACTORS;
   auto buf = [&](int array) { return ring + array * A::WARP_ARRAY; };
 #pragma unroll
   for (int a = 0; a < ARRAYS; ++a) A::zero_rest(buf(a), true, left);
-  const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
+  const int seg = A::segment(warp0), seg_left = static_cast<int>(p.cols) - seg;
   const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
   const float* g2 = p.pre && p.g2 ? p.g2 + j0 : nullptr;
 
-  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x / ranks;
   const int64_t begin = min(worker * p.chunk, p.rows);
   const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
   const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.x_stride + seg;
@@ -116,7 +120,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
           for (int e = 0; e < C; ++e) s[0] = fmaf(y[e], y[e], s[0]);
         }
       }
-      sum_row<TPR, 1>(s, red, phase);
+      sum_row<TPR, 1>(s, red, phase, p.ranks);
       i1 = rsqrtf(s[0] * inv_cols + p.eps);
     }
     float r[E];
@@ -149,7 +153,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
       for (int c = 0; c < A::N; ++c) A::write(r_out, c, left, *reinterpret_cast<const float(*)[C]>(&r[c * C]));
     }
     if (p.pre) {
-      sum_row<TPR, 1>(s, red, phase);
+      sum_row<TPR, 1>(s, red, phase, p.ranks);
       i2 = rsqrtf(s[0] * inv_cols + p.eps);
       if (live) {
 #pragma unroll
@@ -170,6 +174,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
     }
   }
   copy_wait<0>();
+  if (ranks > 1) cluster_sync();  // no block leaves while another may still write to its shared memory
 }
 
 // rows of any length and alignment: a block per row, scalar accesses, the row read once per sum
@@ -229,15 +234,15 @@ template <class T, int V, int TPR, bool GATE_ROW>
 vbt_b200_status go_join(JoinParams& p, int threads, int sms, unsigned& grid, cudaStream_t s, int device) {
   static std::atomic<uint64_t> done{0};
   VB_CUDA(allow_shared(residual_norm_kernel<T, V, TPR, GATE_ROW>, device, done));
-  const int smem = threads * join_bytes(GATE_ROW, sizeof(T), V > 1, TPR);
-  const int per_sm = std::max(1, std::min(1024 / threads, kSmemPerSm / (smem + 2048)));
+  const int smem = threads * join_bytes(GATE_ROW, sizeof(T), V > 1, TPR) + (TPR ? 0 : sum_bytes(p.ranks));
+  const int per_sm = std::max(1, std::min(1024 / threads, kSmemPerSm / (smem + 1024)));
   const int workers = TPR ? threads / 32 : 1;
   // as many workers as fit the card at once, each with a run of rows
-  const int64_t most = int64_t{sms} * per_sm * workers;
+  const int64_t most = p.ranks > 1 ? clusters_at_once(sms, p.ranks) : int64_t{sms} * per_sm * workers;
   p.chunk = (p.rows + most - 1) / most;
   const int64_t used = (p.rows + p.chunk - 1) / p.chunk;
-  grid = static_cast<unsigned>((used + workers - 1) / workers);
-  residual_norm_kernel<T, V, TPR, GATE_ROW><<<grid, threads, smem, s>>>(p);
+  grid = static_cast<unsigned>((used + workers - 1) / workers * p.ranks);
+  VB_CUDA(launch_ranks(residual_norm_kernel<T, V, TPR, GATE_ROW>, p, grid, threads, smem, p.ranks, s));
   return VBT_B200_OK;
 }
 
@@ -250,10 +255,17 @@ vbt_b200_status launch_join(JoinParams p, cudaStream_t s, int device) {
   const bool gate_row = p.gate != nullptr && p.per == 1 && p.rows > 1;
   const int64_t lanes = (p.cols + kFwdElts - 1) / kFwdElts;
   const int tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
-  int threads = tpr ? 256 : static_cast<int>(std::min<int64_t>((lanes + 31) / 32 * 32, 4096));
-  const int smem = threads * join_bytes(gate_row, sizeof(T), vec, tpr);
+  int threads = 0;
+  for (p.ranks = 1; p.ranks <= kMaxRanks; p.ranks *= 2) {
+    const int64_t part = (lanes + p.ranks - 1) / p.ranks;
+    const int64_t n = tpr ? 256 : (part + 31) / 32 * 32;
+    if (n <= (p.ranks > 1 ? 512 : kFwdMaxThreads) && n * join_bytes(gate_row, sizeof(T), vec, tpr) + sum_bytes(p.ranks) <= kSmemPerBlock) {
+      threads = static_cast<int>(n);
+      break;
+    }
+  }
   unsigned g = 0;
-  if (threads > kFwdMaxThreads || smem > kSmemPerBlock) {
+  if (threads == 0) {
     threads = 512;
     g = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{sms} * 4));
     residual_norm_stream_kernel<T><<<g, threads, 0, s>>>(p);

@@ -42,6 +42,7 @@ struct JoinBwdParams {
   int64_t units;
   float a, b;
   int post, pre;
+  int ranks;         // blocks that share a row
 };
 
 // A worker (a warp when TPR lanes of it share a row, else the block) walks a range of neighbouring
@@ -61,12 +62,16 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
   constexpr int RW = TPR ? 32 / TPR : 1;                 // rows a worker takes at once
   constexpr int ARRAYS = MODE == GATE_ROW ? 5 : 4;       // dr, dn, r, y, gate
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float4 red[2][32];
+    const int ranks = TPR ? 1 : p.ranks;
+  const int warp0 = ranks > 1 ? cluster_rank() * static_cast<int>(blockDim.x >> 5) : 0;
+  if (ranks > 1) cluster_sync();  // the other blocks' shared memory is there
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
-  const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
+  const int j0 = A::base(warp0), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
   // a warp's part of the shared memory: w, g2, then `stages` times the arrays
   unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY);
+  float4* red = reinterpret_cast<float4*>(smem + static_cast<size_t>(blockDim.x >> 5) *
+                                                     (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY));
   unsigned char* gbuf = wbuf + A::WARP_FACTORS;
   unsigned char* ring = gbuf + A::WARP_FACTORS;
   auto buf = [&](int stage, int array) { return ring + stage * (ARRAYS * A::WARP_ARRAY) + array * A::WARP_ARRAY; };
@@ -76,14 +81,14 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       const bool present = a == 0 ? p.dr != nullptr : a == 3 ? p.y != nullptr : a == 4 || p.pre;
       A::zero_rest(buf(st, a), present, left);
     }
-  const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
+  const int seg = A::segment(warp0), seg_left = static_cast<int>(p.cols) - seg;
   const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
   const float* g2p = p.pre && p.g2 ? p.g2 + j0 : nullptr;
   A::fill_factors(gbuf, left, [&](int o) { return g2p ? g2p[o] : 1.f; });
   if constexpr (MODE != GATE_SHARED) A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f); });
 
-  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
-  const int64_t workers = TPR ? static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x / ranks;
+  const int64_t workers = TPR ? static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) : gridDim.x / ranks;
   // the worker's units [u, last) are one run of rows; a unit's rows are taken RW at a time
   struct Walk {
     int64_t u;
@@ -210,7 +215,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
         }
       }
     }
-    sum_row<TPR, 3>(s, red, phase);
+    sum_row<TPR, 3>(s, red, phase, p.ranks);
     const float c2 = i2 * i2 * i2 * s[0] * inv_cols;
     const float c1 = p.post ? i1 * i1 * i1 * (s[1] - c2 * s[2]) * inv_cols : 0.f;
     if (live) {
@@ -288,6 +293,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     }
   }
   copy_wait<0>();
+  if (ranks > 1) cluster_sync();  // no block leaves while another may still write to its shared memory
   if constexpr (MODE != GATE_SHARED) over_rows(sum1);
   over_rows(sum2);
   if (rl == 0) {
@@ -426,29 +432,37 @@ __global__ void __launch_bounds__(256) residual_norm_gate_fold_kernel(T* dgate, 
   }
 }
 
-// How the backward runs: `tpr` lanes of a warp share a row, or (0) a block of `threads` does; what does
-// not fit a block's shared memory takes the stream kernel (threads == 0).
+// How the backward runs: `tpr` lanes of a warp share a row, or (0) `ranks` blocks of `threads` do; what
+// eight blocks cannot hold takes the stream kernel (threads == 0).
 struct JoinShape {
-  int tpr, threads, stages, smem, per_sm;
+  int tpr, threads, stages, smem, per_sm, ranks;
   int workers() const { return tpr ? threads / 32 : 1; }
+  // workers on the card at once
+  int64_t most(int sms) const {
+    return ranks > 1 ? clusters_at_once(sms, ranks) : int64_t{sms} * per_sm * (threads ? workers() : 1);
+  }
 };
 inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) {
-  JoinShape h{0, 0, 0, 0, 4};
+  JoinShape h{0, 0, 0, 0, 4, 1};
   const int64_t lanes = (cols + kBwdElts - 1) / kBwdElts;
-  if (lanes > kBwdMaxThreads) return h;
+  if (lanes > int64_t{kBwdMaxThreads} * kMaxRanks) return h;
   h.tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
-  h.threads = h.tpr ? 256 : static_cast<int>((lanes + 31) / 32 * 32);
   const int factors = 2 * kBwdElts * 4, row = (gate_row ? 5 : 4) * row_bytes_per_thread(kBwdElts, elt, vec, h.tpr);
-  auto smem = [&](int stages) { return h.threads * (factors + stages * row); };
-  // registers allow 512 threads per SM (128 each)
-  auto per_sm = [&](int stages) { return std::max(1, std::min(512 / h.threads, kSmemPerSm / (smem(stages) + 2048))); };
-  // two rows ahead where they fit; the warp forms are built for that alone
-  h.stages = 2;
-  if (!h.tpr && smem(2) > kSmemPerBlock) h.stages = 1;
-  h.smem = smem(h.stages);
-  if (h.smem > kSmemPerBlock) return JoinShape{0, 0, 0, 0, 4};
-  h.per_sm = per_sm(h.stages);
-  return h;
+  auto smem = [&](int stages) { return h.threads * (factors + stages * row) + (h.tpr ? 0 : sum_bytes(h.ranks)); };
+  for (h.ranks = 1; h.ranks <= kMaxRanks; h.ranks *= 2) {
+    const int64_t part = (lanes + h.ranks - 1) / h.ranks;
+    h.threads = h.tpr ? 256 : static_cast<int>((part + 31) / 32 * 32);
+    if (h.threads > kBwdMaxThreads) continue;
+    // two rows ahead where they fit; the warp forms are built for that alone
+    h.stages = 2;
+    if (!h.tpr && smem(2) > kSmemPerBlock) h.stages = 1;
+    h.smem = smem(h.stages);
+    if (h.smem > kSmemPerBlock) continue;
+    // registers allow 512 threads per SM (128 each)
+    h.per_sm = std::max(1, std::min(512 / h.threads, kSmemPerSm / (h.smem + 1024)));
+    return h;
+  }
+  return JoinShape{0, 0, 0, 0, 4, 1};
 }
 // How the rows are cut: units of `chunk` rows, `cuts` of them per gate row, dealt out evenly to the
 // workers that fit the card.  At least as many units as workers, and up to eight times that where it
@@ -459,7 +473,7 @@ struct JoinCut {
 };
 inline JoinCut join_cut(int64_t rows, int64_t per, const JoinShape& h, int sms) {
   const int per_block = h.threads ? h.workers() : 1;
-  const int64_t groups = rows / per, most = int64_t{sms} * h.per_sm * per_block;
+  const int64_t groups = rows / per, most = h.most(sms);
   const int64_t at_once = h.tpr ? 32 / h.tpr : 1;
   const int64_t least = (most + groups - 1) / groups, finest = (per + at_once - 1) / at_once;
   JoinCut c{};
@@ -490,7 +504,7 @@ template <class T, int V, int TPR, int MODE, int STAGES>
 vbt_b200_status go_join_bwd(const JoinBwdParams& p, const JoinShape& h, unsigned grid, cudaStream_t s, int device) {
   static std::atomic<uint64_t> done{0};
   VB_CUDA(allow_shared(residual_norm_bwd_kernel<T, V, TPR, MODE, STAGES>, device, done));
-  residual_norm_bwd_kernel<T, V, TPR, MODE, STAGES><<<grid, h.threads, h.smem, s>>>(p);
+  VB_CUDA(launch_ranks(residual_norm_bwd_kernel<T, V, TPR, MODE, STAGES>, p, grid, h.threads, h.smem, h.ranks, s));
   return VBT_B200_OK;
 }
 
@@ -502,8 +516,8 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
                    a16(p.gate) && a16(p.dx) && a16(p.dy) && a16(p.dgate);
   const JoinShape h = join_bwd_shape(p.cols, sizeof(T), mode == GATE_ROW, vec);
   const JoinCut cut = join_cut(p.rows, p.per, h, sm_count(device));
-  p.chunk = cut.chunk; p.cuts = cut.cuts; p.units = cut.units;
-  const unsigned g = static_cast<unsigned>(cut.blocks);
+  p.chunk = cut.chunk; p.cuts = cut.cuts; p.units = cut.units; p.ranks = h.ranks;
+  const unsigned g = static_cast<unsigned>(cut.blocks * h.ranks);
   float* at = ws;
   if (dg1) { p.ws_g1 = at; at += cut.workers * p.cols; }
   if (dg2) { p.ws_g2 = at; at += cut.workers * p.cols; }

@@ -2,6 +2,7 @@
 // row, thread t holds the V-element vectors t, t + TPR, t + 2 TPR, ...
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -119,8 +120,8 @@ __device__ __forceinline__ void narrow2(__nv_bfloat16* p, float2 v) {
 __device__ __forceinline__ void narrow2(__half* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
 
 // A thread's E values of a row, worked on in chunks of C: V neighbours for V-value vectors, two
-// single values for V = 1.  TPR lanes of a warp share a row, or (TPR = 0) every warp of the block owns
-// a segment of 32 E neighbouring values of it; either way the columns of a thread's chunks and their
+// single values for V = 1.  TPR lanes of a warp share a row, or (TPR = 0) every warp of the block (of
+// the cluster, counted from `warp0`) owns a segment of 32 E neighbouring values of it; either way the columns of a thread's chunks and their
 // places in shared memory are compile-time offsets from one base.
 //
 // V > 1 (16-byte aligned rows): a thread has slots of its own in every buffer; what it copied it may
@@ -143,8 +144,10 @@ template <class T, int V, int TPR, int E> struct RowChunks {
 
   static __device__ __forceinline__ int lane() { return static_cast<int>(threadIdx.x & 31) % STEP; }
   // first column of this thread's segment, and of this thread
-  static __device__ __forceinline__ int segment() { return TPR ? 0 : static_cast<int>(threadIdx.x >> 5) * (32 * E); }
-  static __device__ __forceinline__ int base() { return segment() + lane() * V; }
+  static __device__ __forceinline__ int segment(int warp0 = 0) {
+    return TPR ? 0 : (warp0 + static_cast<int>(threadIdx.x >> 5)) * (32 * E);
+  }
+  static __device__ __forceinline__ int base(int warp0 = 0) { return segment(warp0) + lane() * V; }
   // offset of element e of chunk c from it
   static __device__ __forceinline__ constexpr int off(int c, int e) { return V > 1 ? c * STEP * V + e : (2 * c + e) * STEP; }
   static __device__ __forceinline__ unsigned char* region(unsigned char* array) {
@@ -268,24 +271,66 @@ static_assert(32 * row_bytes_per_thread(16, 2, false, 0) >= RowChunks<__half, 1,
               32 * row_bytes_per_thread(16, 1, false, 16) >= RowChunks<uint8_t, 1, 16, 16>::WARP_ARRAY &&
               32 * row_bytes_per_thread(16, 2, true, 32) >= RowChunks<__half, 8, 32, 16>::WARP_ARRAY);
 
-// Sums over the threads that share a row: TPR lanes of a warp, or the whole block (TPR = 0; `red`
-// holds two phases, so one barrier per call is enough).  N <= 4.
+// ---- thread-block clusters: rows wider than a block holds are shared by up to kMaxRanks blocks ----
+constexpr int kMaxRanks = 8;
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// writes v to the same place of block `rank`'s shared memory
+__device__ __forceinline__ void store_at_rank(float4* mine, int rank, float4 v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+// Sums over the threads that share a row: TPR lanes of a warp, or (TPR = 0) the block or the `ranks`
+// blocks of its cluster.  `red` (sum_bytes of shared memory) holds two phases of a float4 per warp
+// of the row, so one barrier per call is enough: a block that runs ahead writes the other phase, and
+// waits there for the ones behind it.  N <= 4.
+constexpr int kBlockWarps = 32, kRowWarps = 128;  // at most, of a block and of kMaxRanks blocks of 16
+constexpr int sum_bytes(int ranks) { return 2 * 16 * (ranks == 1 ? kBlockWarps : kRowWarps); }
 template <int TPR, int N>
-__device__ __forceinline__ void sum_row(float (&s)[N], float4 (*red)[32], int& phase) {
+__device__ __forceinline__ void sum_row(float (&s)[N], float4* red, int& phase, int ranks = 1) {
   constexpr int G = TPR ? TPR : 32;
 #pragma unroll
   for (int d = G / 2; d > 0; d >>= 1)
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
   if constexpr (TPR == 0) {
-    const int w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0)
-      red[phase][w] = make_float4(s[0], N > 1 ? s[N > 1 ? 1 : 0] : 0.f, N > 2 ? s[N > 2 ? 2 : 0] : 0.f, N > 3 ? s[N > 3 ? 3 : 0] : 0.f);
-    __syncthreads();
-    float4 t = red[phase][0];
-    for (int k = 1; k < warps; ++k) {
-      const float4 f = red[phase][k];
-      t.x += f.x; t.y += f.y; t.z += f.z; t.w += f.w;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const float4 mine = make_float4(s[0], N > 1 ? s[N > 1 ? 1 : 0] : 0.f, N > 2 ? s[N > 2 ? 2 : 0] : 0.f, N > 3 ? s[N > 3 ? 3 : 0] : 0.f);
+    float4 t;
+    if (ranks == 1 && N == 1) {
+      float* row = reinterpret_cast<float*>(red) + phase * kBlockWarps;
+      if (lane == 0) row[w] = s[0];
+      __syncthreads();
+      t.x = row[0];
+      for (int k = 1; k < warps; ++k) t.x += row[k];
+    } else if (ranks == 1) {
+      if (lane == 0) red[phase * kBlockWarps + w] = mine;
+      __syncthreads();
+      t = red[phase * kBlockWarps];
+      for (int k = 1; k < warps; ++k) {
+        const float4 f = red[phase * kBlockWarps + k];
+        t.x += f.x; t.y += f.y; t.z += f.z; t.w += f.w;
+      }
+    } else {
+      float4* row = red + phase * kRowWarps;
+      if (lane < ranks) store_at_rank(row + cluster_rank() * warps + w, lane, mine);
+      __syncwarp();
+      cluster_sync();
+      t = row[0];
+#pragma unroll 1
+      for (int k = 1; k < warps * ranks; ++k) {
+        const float4 f = row[k];
+        t.x += f.x; t.y += f.y; t.z += f.z; t.w += f.w;
+      }
     }
     s[0] = t.x;
     if constexpr (N > 1) s[1] = t.y;
@@ -295,14 +340,35 @@ __device__ __forceinline__ void sum_row(float (&s)[N], float4 (*red)[32], int& p
   }
 }
 
+// Launches `kernel` with clusters of `ranks` blocks (1: none).
+template <class Kernel, class Params>
+inline cudaError_t launch_ranks(Kernel kernel, const Params& p, unsigned grid, int threads, int smem, int ranks, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+// Clusters of this size that fit the card at once: pairs always do, larger ones leave out what a
+// group of SMs has left over.
+inline int64_t clusters_at_once(int sms, int ranks) { return std::max(1, ranks <= 2 ? sms / ranks : sms / ranks * 7 / 8); }
+
 constexpr int kSmemPerSm = 228 * 1024;     // of which every block takes 1 KB for the system
-constexpr int kSmemPerBlock = 226 * 1024;  // beside sum_row's 1 KB
+constexpr int kSmemPerBlock = 227 * 1024;
 
 // Shared memory beyond the default limit has to be asked for once per kernel and device.
-template <class Kernel> inline cudaError_t allow_shared(Kernel kernel, int device, std::atomic<uint64_t>& done) {
+template <class Kernel>
+inline cudaError_t allow_shared(Kernel kernel, int device, std::atomic<uint64_t>& done, int most = kSmemPerBlock) {
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
