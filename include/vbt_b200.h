@@ -526,7 +526,7 @@ VBT_B200_API vbt_b200_status vbt_b200_residual_norm_backward(
  * values (the last one may be shorter); a group is held as 8-bit levels and one F32 scale:
  *   amax = max |x|;  scale = amax * fl(1/top);  q = rn(fl(x * fl(top / amax)));  x' = q * scale
  * with top = 127 (INT8) or 448 (E4M3); amax < 2^-119 gives zeros.  A group with a NaN or an infinity
- * reads back as NaN throughout.  q: one byte per value, dense [rows, cols]; scale: F32, dense
+ * is held as zeros with a NaN scale and reads back as NaN throughout.  q: one byte per value, dense [rows, cols]; scale: F32, dense
  * [rows, ceil(cols / VBT_B200_Q8_GROUP)]. */
 #define VBT_B200_Q8_INT8 0
 #define VBT_B200_Q8_E4M3 1

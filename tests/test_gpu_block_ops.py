@@ -4,8 +4,8 @@ plain 64-bit forms of their formulas.
 Tolerances are derived, not fitted.  u = 2^-24 is half a step of fp32.  A value computed in fp32 from
 terms of total magnitude M is off by at most K * u * M, where K counts the roundings on the longest
 path: a row sum is sequential over at most 137 values per thread (70001 / 512 and 20001 / 256 in the
-kernels for rows of any length, 16 in the others) plus a tree of at most 15 levels, a sum over rows over at most rows / 296 rows per block plus the fold (at most 8 rows per
-thread and step, 15 levels), square roots, exponentials and sines add at most 4 each, the products
+kernels for rows of any length, 16 in the others) plus a tree of at most 15 levels, a sum over rows
+over at most rows / 296 rows per block plus the fold (at most 8 rows per thread and step, 15 levels), square roots, exponentials and sines add at most 4 each, the products
 around them at most 10.  K = 192 covers every size below (137 + 15 + 14 < 192).  Storing to t
 adds half a step, eps(t) / 2 relative, and half the smallest subnormal.  8-bit levels and scales are a
 fixed sequence of correctly rounded fp32 operations: they are compared bit for bit."""
@@ -603,6 +603,32 @@ def test_cache_equal_slots_keep_the_last_token_whole(cache, tokens):
         assert c._owner.abs().sum() == 0
 
 
+@pytest.mark.parametrize("seqs", [1, 31, 32, 33, 1025, 3000])
+def test_cache_read_finds_its_sequence(cache, seqs):
+    """Many short and empty sequences, their number around the search's 32-way steps."""
+    g = gen(seqs)
+    heads, dim, page = 1, 8, 2
+    lens = torch.randint(0, 4, (seqs,), generator=g, device="cuda")
+    lens[0] = 0
+    starts = torch.zeros(seqs + 1, dtype=torch.int64, device="cuda")
+    starts[1:] = lens.cumsum(0)
+    total = int(starts[-1])
+    table = torch.arange(2 * seqs, device="cuda").reshape(seqs, 2)[torch.randperm(seqs, generator=g, device="cuda")]
+    c = cache.QuantCache(2 * seqs, page, heads, dim)
+    k = acts(g, (c.num_slots, heads, dim), F32)
+    c.write(k, -k, torch.arange(c.num_slots, device="cuda"))
+    rk, rv = c.read(table, starts, total + 3, dtype=F32)
+    row = torch.arange(total, device="cuda")
+    s = torch.searchsorted(starts, row, right=True) - 1
+    at = row - starts[s]
+    slot = table[s, at // page] * page + at % page
+    full = (c.k.float() * c.k_scale[..., None]).reshape(c.num_slots, heads, dim)
+    assert torch.equal(rk[:total], full[slot]) and torch.equal(rv[:total], -full[slot]) and (rk[total:] == 0).all()
+    # sequences that begin behind row 0: the rows in front belong to nobody
+    rk2, _ = c.read(table, starts + 2, total + 2, dtype=F32)
+    assert (rk2[:2] == 0).all() and torch.equal(rk2[2:], rk[:total])
+
+
 def test_cache_bad_slots_and_pages(cache):
     from vibetensor_b200 import ops
     g = gen(2)
@@ -904,6 +930,9 @@ def test_refusals(kernels, cache):
                       (lambda: kernels.rotary(q, None, pos[None], f, (31,)), ValueError),
                       (lambda: kernels.rotary(q, None, pos[:, :4], f), ValueError),
                       (lambda: kernels.rotary(q, None, pos, f, out=(q[:1], None)), ValueError),
+                      (lambda: kernels.rotary(q[:, 1:], None, pos[:, 1:], f, out=(q[:, :-1], None)), ValueError),
+                      (lambda: kernels.rotary(q, q, pos, f, out=(q, q)), ValueError),
+                      (lambda: kernels.rotary(q, None, pos, f, out=(q[:, :1].expand(2, 5, 3, 64), None)), ValueError),
                       (lambda: kernels.rotary(q, None, pos.cpu(), f), RuntimeError)):
         with pytest.raises(exc):
             call()

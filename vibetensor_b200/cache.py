@@ -115,8 +115,8 @@ class QuantCache:
                 raise ValueError(f"{what}: total, the number of rows, is needed without out")
             if dtype not in _FLOATS:
                 raise TypeError(f"{what} gives float32, float16 or bfloat16")
-            shape = (int(total), self.num_heads, self.head_dim)
-            ko, vo = self.k.new_empty(shape, dtype=dtype), self.k.new_empty(shape, dtype=dtype)
+            ko = self.k.new_empty(int(total), self.num_heads, self.head_dim, dtype=dtype)
+            vo = torch.empty_like(ko)
         else:
             ko, vo = out
             self._on_device(what, ko, vo)

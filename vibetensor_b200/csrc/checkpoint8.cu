@@ -629,7 +629,7 @@ inline unsigned flat_grid(int64_t groups, int lanes, int u) {
   const int64_t per = int64_t{kCkThreads} / lanes * u;
   return static_cast<unsigned>((groups + per - 1) / per);
 }
-inline bool rows_fit(int64_t groups) { return groups < (int64_t{1} << 34); }  // a grid of 2^31 blocks
+inline bool rows_fit(int64_t groups) { return groups < (int64_t{1} << 32); }  // at least four groups per block
 
 // calls fn(format constant)
 #define VB_FORMAT(format, F, ...)                                                     \

@@ -222,8 +222,11 @@ def scatter_add(out: torch.Tensor, dim: int, index: torch.Tensor, src: torch.Ten
 # --------------------------------------------------------------------------------------
 # around a transformer block's matrix products
 # --------------------------------------------------------------------------------------
+_F32 = torch.float32
+
+
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    return t if t is None else t.data_ptr()
 
 
 def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
@@ -235,15 +238,21 @@ def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]
             raise ValueError(f"{what}: operands on {first.device} and {t.device}")
 
 
+# Allocations on the host path: sizes as plain integers and no device argument parse in 1.4 us where a
+# tuple takes 2.3 and a device 3.3.
 def _dense_like(x: torch.Tensor) -> torch.Tensor:
+    if x.is_contiguous():
+        return torch.empty_like(x)
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _floats(x: torch.Tensor, n: int) -> torch.Tensor:
-    return x.new_empty((n,), dtype=torch.float32)
+    return x.new_empty(n, dtype=_F32)
 
 
 def _like(what: str, name: str, t: torch.Tensor, x: torch.Tensor) -> None:
+    if t is x:
+        return
     if t.shape != x.shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(x.shape)}")
     if t.dtype != x.dtype:
@@ -261,9 +270,9 @@ def _scratch_bytes(entry: str, *sizes: int) -> int:
 def _gamma(name: str, g: Optional[torch.Tensor], cols: int) -> Optional[torch.Tensor]:
     if g is None:
         return None
-    if g.dtype != torch.float32 or g.numel() != cols:
+    if g.dtype != _F32 or g.numel() != cols:
         raise TypeError(f"{name} must be float32 of shape [hidden_size]")
-    return g.contiguous()
+    return g if g.is_contiguous() else g.contiguous()
 
 
 def _row_scalars(name: str, t: Optional[torch.Tensor], rows: int) -> Optional[torch.Tensor]:
@@ -320,10 +329,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gamma_post: Optional[torch.T
     gv, rs_g, per = _gate_rows(what, gate, x, rows)
     r = _dense_like(x)
     n = _dense_like(x) if pre_norm else None
-    if post_norm and pre_norm:
-        inv_post, inv_pre = x.new_empty((2, rows), dtype=torch.float32).unbind()
-    else:
-        inv_post, inv_pre = (_floats(x, rows) if on else None for on in (post_norm, pre_norm))
+    inv_post = _floats(x, rows) if post_norm else None
+    inv_pre = _floats(x, rows) if pre_norm else None
     if rows and cols:
         check(lib().vbt_b200_residual_norm(
             _ptr(r), _ptr(n), _ptr(inv_post), _ptr(inv_pre), _ptr(xv), _ptr(yv), _ptr(gamma_post), _ptr(gv),
@@ -381,7 +388,7 @@ def residual_norm_backward(grad_r: Optional[torch.Tensor], grad_n: Optional[torc
     if rows and (dg1 is not None or dg2 is not None or dgate is not None):
         ws_bytes = _scratch_bytes("vbt_b200_residual_norm_backward_workspace_bytes", rows, cols, dtype_code(first.dtype),
                                   per, first.get_device())
-        ws = first.new_empty((ws_bytes,), dtype=torch.uint8)
+        ws = first.new_empty(ws_bytes, dtype=torch.uint8)
     (drv, rs_dr), (dnv, rs_dn), (yv, rs_y), (rv, rs_r) = views
     check(lib().vbt_b200_residual_norm_backward(
         _ptr(dx), _ptr(dy), _ptr(dg1), _ptr(dgate), _ptr(dg2), _ptr(drv), _ptr(dnv), _ptr(yv), _ptr(rv),
@@ -422,7 +429,7 @@ def _q8_format(what: str, fmt: str):
 
 def _new_checkpoint(x: torch.Tensor, rows: int, cols: int, fmt: str, store: torch.dtype) -> Checkpoint8:
     return Checkpoint8(torch.empty_like(x, dtype=store, memory_format=torch.contiguous_format),
-                       x.new_empty((rows, -(-cols // Q8_GROUP)), dtype=torch.float32), fmt, x.dtype)
+                       x.new_empty(rows, -(-cols // Q8_GROUP), dtype=_F32), fmt, x.dtype)
 
 
 def _held_rows(what: str, c: Checkpoint8):
@@ -506,7 +513,7 @@ def _rmsnorm_backward8(grad_output: torch.Tensor, c: Checkpoint8, inv_rms: torch
     if rows and dgamma is not None:
         ws_bytes = _scratch_bytes("vbt_b200_rmsnorm_backward8_workspace_bytes", rows, cols, dtype_code(c.dtype),
                                   c.q.get_device())
-        ws = c.q.new_empty((ws_bytes,), dtype=torch.uint8)
+        ws = c.q.new_empty(ws_bytes, dtype=torch.uint8)
     check(lib().vbt_b200_rmsnorm_backward8(_ptr(dx), _ptr(dgamma), _ptr(gv), _ptr(c.q), _ptr(c.scale), _ptr(inv_rms),
                                            _ptr(gamma), dtype_code(c.dtype), code, rows, cols, rs, _ptr(ws), ws_bytes,
                                            stream_ptr(grad_output)))
@@ -579,6 +586,31 @@ _I64x15 = ctypes.c_int64 * 15
 _SECTIONS = [ctypes.c_int64 * n for n in range(5)]
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the views may share a value: their heads lie between one another in one memory, as
+    the parts of a fused projection do without sharing any."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or not a.numel() or not b.numel():
+        return False
+
+    def span(t):
+        end = builtins.sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (end + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    # parts of one projection: equal steps from token to token, and within a token apart from each other
+    if a.dim() == b.dim() and a.dtype == b.dtype and a.stride()[:-2] == b.stride()[:-2] and a.shape[:-2] == b.shape[:-2]:
+        step = min((st for n, st in zip(a.shape[:-2], a.stride()[:-2]) if n > 1), default=0) * a.element_size()
+
+        def inner(t):
+            return ((t.shape[-2] - 1) * t.stride(-2) + t.shape[-1]) * t.element_size()
+        first, second = (a, b) if a0 <= b0 else (b, a)
+        gap = second.data_ptr() - first.data_ptr()
+        if inner(first) <= gap and (step == 0 or gap + inner(second) <= step):
+            return False
+    return True
+
+
 def _head_strides(t: torch.Tensor):
     """{batch, token, head} strides of [batch, tokens, heads, dim] or [tokens, heads, dim]."""
     st = t.stride()
@@ -638,6 +670,14 @@ def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what
             _like(what, name, o, x)
             if o.stride(-1) != 1 and dim > 1:
                 raise ValueError(f"{what}: {name} must have a last stride of 1")
+            if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+                raise ValueError(f"{what}: {name} has values that share memory")
+            for t in (q, k, positions, inv_freq):
+                same = t is x and o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+                if t is not None and not same and _overlap(o, t):
+                    raise ValueError(f"{what}: {name} overlaps an input that it does not replace")
+        if out[1] is not None and _overlap(*out):
+            raise ValueError(f"{what}: the two outputs overlap")
     qv = q if q.stride(-1) == 1 or dim <= 1 else _ops.contiguous(q)
     qo = out[0] if out is not None else _dense_like(qv)
     strides = (*_head_strides(qo), *_head_strides(qv))
