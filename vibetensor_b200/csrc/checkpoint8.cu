@@ -333,7 +333,6 @@ struct Norm8Params {
 // Rows staged in shared memory as in residual_norm: a worker (a warp when TPR lanes of it share a row,
 // else the block) walks neighbouring rows, a thread reads back only what it copied itself.
 constexpr int kNormElts = 16;
-constexpr int kBwd8Stages = 1;  // rows in flight of the backward
 // group of 128 values that chunk c of this thread belongs to, counted from the row's start
 template <class A> __device__ __forceinline__ int chunk_group(int j0, int c) { return (j0 + A::off(c, 0)) / kQ8Group; }
 
@@ -465,14 +464,11 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
   const int j0 = A::base(), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
-  constexpr int STAGE = A::WARP_ARRAY + Q::WARP_ARRAY;
-  unsigned char* gbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (A::WARP_FACTORS + kBwd8Stages * STAGE);
-  unsigned char* ring = gbuf + A::WARP_FACTORS;
-#pragma unroll
-  for (int st = 0; st < kBwd8Stages; ++st) {
-    A::zero_rest(ring + st * STAGE, true, left);
-    Q::zero_rest(ring + st * STAGE + A::WARP_ARRAY, true, left);
-  }
+  unsigned char* gbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (A::WARP_FACTORS + A::WARP_ARRAY + Q::WARP_ARRAY);
+  unsigned char* dbuf = gbuf + A::WARP_FACTORS;
+  unsigned char* qbuf = dbuf + A::WARP_ARRAY;
+  A::zero_rest(dbuf, true, left);
+  Q::zero_rest(qbuf, true, left);
   const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
   const typename A::Shift dy_shift(p.dy, p.stride);
   const typename Q::Shift q_shift(p.q, p.cols);
@@ -484,18 +480,18 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
   const float* scale_at = p.scale + (begin + rl) * p.groups;
   const float* inv_at = p.inv + begin + rl;
   int ahead = rl;
-  float sc_next[kBwd8Stages][NS], inv_next[kBwd8Stages];
-  auto fetch = [&](int stage, float (&sc)[NS], float& inv) {
-    inv = 0.f;
+  float sc_next[NS], inv_next;
+  auto fetch = [&] {
+    inv_next = 0.f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) sc[i] = 0.f;
+    for (int i = 0; i < NS; ++i) sc_next[i] = 0.f;
     if (ahead < todo) {
-      A::copy(ring + stage * STAGE, dy_at, seg_left, p.dy);
-      Q::copy(ring + stage * STAGE + A::WARP_ARRAY, q_at, seg_left, p.q);
-      inv = *inv_at;
+      A::copy(dbuf, dy_at, seg_left, p.dy);
+      Q::copy(qbuf, q_at, seg_left, p.q);
+      inv_next = *inv_at;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
-        if (A::off(i * GC, 0) < left) sc[i] = __ldg(scale_at + chunk_group<A>(j0, i * GC));
+        if (A::off(i * GC, 0) < left) sc_next[i] = __ldg(scale_at + chunk_group<A>(j0, i * GC));
     }
     ahead += RW;
     dy_at += RW * p.stride;
@@ -504,33 +500,31 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
     inv_at += RW;
     copy_commit();
   };
-#pragma unroll
-  for (int st = 0; st < kBwd8Stages; ++st) fetch(st, sc_next[st], inv_next[st]);
+  fetch();
   A::fill_factors(gbuf, left, [&](int o) { return p.gamma ? p.gamma[j0 + o] : 1.f; });
   T* dx = static_cast<T*>(p.out) + (begin + rl) * p.cols + j0;
   float sum[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) sum[i] = 0.f;
-  int phase = 0, stage = 0;
+  int phase = 0;
   for (int r0 = 0; r0 < todo; r0 += RW) {
     const bool live = RW == 1 || r0 + rl < todo;
-    copy_wait<kBwd8Stages - 1>();
+    copy_wait<0>();
     A::sync();
     const int64_t row = begin + r0 + rl;
-    unsigned char* dbuf = ring + stage * STAGE;
-    unsigned char* qbuf = dbuf + A::WARP_ARRAY;
-    const float inv = inv_next[0];
+    const float inv = inv_next;
     float x[E];
+    Vec<T, C> dy[A::N];
     float s[1] = {0.f};
     if (live) {
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
-        float d[C], g[C];
-        A::read(dbuf, dy_shift(row), c, left, d);
+        float g[C];
+        A::read_raw(dbuf, dy_shift(row), c, left, dy[c]);
         A::read_factors(gbuf, c, g);
         Vec<uint8_t, C> lv;
         Q::read_raw(qbuf, q_shift(row), c, left, lv);
-        const float sc = sc_next[0][c / GC];
+        const float sc = sc_next[c / GC];
         if constexpr (V > 1) {
           q8_widen<F, V>(*reinterpret_cast<const typename Q8Raw<V>::type*>(&lv), sc, *reinterpret_cast<float(*)[V]>(&x[c * C]));
         } else {
@@ -540,11 +534,18 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           const int i = c * C + e;
-          const float t = d[e] * x[i];
+          const float t = to_f(dy[c].v[e]) * x[i];
           sum[i] = fmaf(t, inv, sum[i]);
           s[0] = fmaf(t, g[e], s[0]);
         }
       }
+    }
+    // 16-bit rows stay in registers, and the next row's copies run through the reduction and the stores
+    // ([32768,4096] bf16, both passes: 302 -> 278 us; 32-bit rows are too many registers, 222 -> 230 us)
+    constexpr bool kEarly = sizeof(T) == 2;
+    if constexpr (kEarly) {
+      A::sync();
+      fetch();
     }
     sum_row<TPR, 1>(s, &red[0][0], phase);
     const float k = inv * inv * inv * s[0] * inv_cols;
@@ -552,23 +553,18 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float d[C], g[C];
-        A::read(dbuf, dy_shift(row), c, left, d);
+        if constexpr (!kEarly) A::read_raw(dbuf, dy_shift(row), c, left, dy[c]);
         A::read_factors(gbuf, c, g);
 #pragma unroll
-        for (int e = 0; e < C; ++e) d[e] = fmaf(inv * d[e], g[e], -k * x[c * C + e]);
+        for (int e = 0; e < C; ++e) d[e] = fmaf(inv * to_f(dy[c].v[e]), g[e], -k * x[c * C + e]);
         A::write(dx, c, left, d);
       }
     }
     dx += RW * p.cols;
-#pragma unroll
-    for (int st = 0; st + 1 < kBwd8Stages; ++st) {
-      inv_next[st] = inv_next[st + 1];
-#pragma unroll
-      for (int i = 0; i < NS; ++i) sc_next[st][i] = sc_next[st + 1][i];
+    if constexpr (!kEarly) {
+      A::sync();
+      fetch();
     }
-    A::sync();
-    fetch(stage, sc_next[kBwd8Stages - 1], inv_next[kBwd8Stages - 1]);
-    stage = stage + 1 == kBwd8Stages ? 0 : stage + 1;
   }
   copy_wait<0>();
   if (p.ws == nullptr) return;
@@ -711,7 +707,7 @@ inline NormShape norm_shape(int64_t rows, int64_t cols, int elt, bool vec, Bytes
 // shared memory per thread: gamma and a row of x, or of dy and the levels
 constexpr int norm8_bytes(int elt, bool vec, int tpr) { return kNormElts * 4 + row_bytes_per_thread(kNormElts, elt, vec, tpr); }
 constexpr int bwd8_bytes(int elt, bool vec, int tpr) {
-  return kNormElts * 4 + kBwd8Stages * (row_bytes_per_thread(kNormElts, elt, vec, tpr) + row_bytes_per_thread(kNormElts, 1, vec, tpr));
+  return kNormElts * 4 + row_bytes_per_thread(kNormElts, elt, vec, tpr) + row_bytes_per_thread(kNormElts, 1, vec, tpr);
 }
 
 #define VB_ROW8(KERNEL, V, TPR)                                                       \

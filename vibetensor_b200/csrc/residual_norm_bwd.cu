@@ -439,7 +439,7 @@ struct JoinShape {
   int workers() const { return tpr ? threads / 32 : 1; }
   // workers on the card at once
   int64_t most(int sms) const {
-    return ranks > 1 ? clusters_at_once(sms, ranks) : int64_t{sms} * per_sm * (threads ? workers() : 1);
+    return ranks > 1 ? clusters_at_once(sms * per_sm, ranks) : int64_t{sms} * per_sm * (threads ? workers() : 1);
   }
 };
 inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) {
