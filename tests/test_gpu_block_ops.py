@@ -944,6 +944,7 @@ def test_refusals(kernels, cache):
                       (lambda: kv.read(s[None], s[:2].int(), 4), TypeError), (lambda: kv.read(s[None], s[:2]), ValueError),
                       (lambda: kv.read(s[None], s[:2], 4, dtype=torch.float64), TypeError),
                       (lambda: kv.read(s[None], s[:2], out=(k, k[:4])), ValueError),
+                      (lambda: kv.read(s[None], s[:2], out=(k, k)), ValueError),
                       (lambda: cache.QuantCache(2, 4, 3, 16, fmt="int4"), ValueError), (lambda: cache.QuantCache(0, 4, 3, 16), ValueError),
                       (lambda: cache.QuantCache(2, 4, 3, 16, device="cpu"), RuntimeError)):
         with pytest.raises(exc):

@@ -125,6 +125,8 @@ class QuantCache:
             if ko.dim() != 3 or tuple(ko.shape[1:]) != (self.num_heads, self.head_dim) or ko.shape != vo.shape or \
                     not ko.is_contiguous() or not vo.is_contiguous():
                 raise ValueError(f"{what}: out must be two dense [rows, {self.num_heads}, {self.head_dim}] tensors")
+            if ko.numel() and abs(ko.data_ptr() - vo.data_ptr()) < ko.numel() * ko.element_size():
+                raise ValueError(f"{what}: the two outputs overlap")
         if ko.shape[0] == 0:
             return ko, vo
         if page_table.stride(-1) != 1 and page_table.shape[1] > 1:

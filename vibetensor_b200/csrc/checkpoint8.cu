@@ -19,64 +19,61 @@
 namespace vb {
 namespace {
 
-// How a group of up to 128 neighbouring values lies in the lanes of a warp.  VEC: 16-byte vectors
-// (needs rows of whole vectors, 16-byte aligned); else 32 lanes with the values lane, lane + 32, ...
-template <class T, bool VEC> struct Lanes {
+// How a group of up to 128 neighbouring values lies in the lanes of a warp: L lanes with W vectors of
+// V values each.  VEC: 16-byte vectors (needs rows of whole vectors, 16-byte aligned); else single
+// values.  What a lane works out per group (its place, the scale) is shared by its W vectors.
+template <class T, bool VEC, int WV> struct Lanes {
   static constexpr int V = VEC ? 16 / sizeof(T) : 1;
-  static constexpr int L = VEC ? kQ8Group / V : 32;
-  static constexpr int N = kQ8Group / L;  // values per lane
-  using Raw = Vec<T, N>;
-  using Q = typename Q8Raw<N>::type;
+  static constexpr int W = VEC ? WV : 4;
+  static constexpr int L = kQ8Group / (V * W);
+  static constexpr int N = V * W;  // values per lane
+  struct Raw { Vec<T, V> v[W]; };
+  struct Q { typename Q8Raw<V>::type v[W]; };
+  static __device__ __forceinline__ int off(int lane, int w) { return (w * L + lane) * V; }
 
   static __device__ __forceinline__ Raw load(const T* group, int lane, int len) {
     Raw r;
-    if constexpr (VEC) {
-      if (lane * V < len) return *reinterpret_cast<const Raw*>(group + lane * V);
 #pragma unroll
-      for (int e = 0; e < N; ++e) r.v[e] = from_f<T>(0.f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) r.v[e] = lane + 32 * e < len ? group[lane + 32 * e] : from_f<T>(0.f);
+    for (int w = 0; w < W; ++w) {
+      if (off(lane, w) < len) r.v[w] = *reinterpret_cast<const Vec<T, V>*>(group + off(lane, w));
+      else r.v[w] = Vec<T, V>{};
     }
     return r;
   }
+  static __device__ __forceinline__ void widen(const Raw& r, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f(r.v[i / V].v[i % V]);
+  }
   static __device__ __forceinline__ void store(T* group, int lane, int len, const float (&v)[N]) {
-    if constexpr (VEC) {
-      if (lane * V >= len) return;
-      Raw r;
 #pragma unroll
-      for (int e = 0; e < N; ++e) r.v[e] = from_f<T>(v[e]);
-      *reinterpret_cast<Raw*>(group + lane * V) = r;
-    } else {
+    for (int w = 0; w < W; ++w) {
+      if (off(lane, w) >= len) continue;
+      Vec<T, V> r;
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (lane + 32 * e < len) group[lane + 32 * e] = from_f<T>(v[e]);
+      for (int e = 0; e < V; ++e) r.v[e] = from_f<T>(v[w * V + e]);
+      *reinterpret_cast<Vec<T, V>*>(group + off(lane, w)) = r;
     }
   }
   static __device__ __forceinline__ Q load_q(const uint8_t* group, int lane, int len) {
-    if constexpr (VEC) {
-      Q q{};
-      if (lane * V < len) q = *reinterpret_cast<const Q*>(group + lane * V);
-      return q;
-    } else {
-      uint32_t q = 0;
+    Q q{};
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (lane + 32 * e < len) q |= static_cast<uint32_t>(group[lane + 32 * e]) << (8 * e);
-      return q;
-    }
+    for (int w = 0; w < W; ++w)
+      if (off(lane, w) < len) q.v[w] = *reinterpret_cast<const typename Q8Raw<V>::type*>(group + off(lane, w));
+    return q;
+  }
+  template <int F> static __device__ __forceinline__ void widen_q(const Q& q, float scale, float (&v)[N]) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) q8_widen<F, V>(q.v[w], scale, *reinterpret_cast<float(*)[V]>(&v[w * V]));
   }
   // quantises the group: returns its stored scale
   template <int F>
   static __device__ __forceinline__ float store_q(uint8_t* group, int lane, int len, const Raw& raw, const float (&v)[N]) {
-    const Raw one[1] = {raw};
-    const Q8Scale s = q8_scale<F>(group_mag<T, N, 1, L>(one));
-    if constexpr (VEC) {
-      if (lane * V < len) q8_store<F, N>(group + lane * V, v, s.up);
-    } else {
+    const Q8Scale s = q8_scale<F>(group_mag<T, V, W, L>(raw.v));
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (lane + 32 * e < len) group[lane + 32 * e] = q8_pack1<F>(v[e], s.up);
+    for (int w = 0; w < W; ++w) {
+      if (off(lane, w) >= len) continue;
+      if constexpr (VEC) q8_store<F, V>(group + off(lane, w), *reinterpret_cast<const float(*)[V]>(&v[w * V]), s.up);
+      else group[off(lane, w)] = q8_pack1<F>(v[w], s.up);
     }
     return s.down;
   }
@@ -130,10 +127,12 @@ struct CkParams {
 // threads per SM) and 256 threads the 8-bit copy and its way back took 222 us for [16384,8192] bf16
 // against 152, the gated activation's two passes 409 against 376.
 constexpr int kCkThreads = 128;
+constexpr int kCopyVecs = 4;
+constexpr int kGluVecs = 2;
 
-template <class T, bool VEC, int F, int U>
+template <class T, bool VEC, int F, int WV, int U>
 __global__ void __launch_bounds__(kCkThreads) checkpoint8_kernel(const __grid_constant__ CkParams p) {
-  using A = Lanes<T, VEC>;
+  using A = Lanes<T, VEC, WV>;
   constexpr int S = kCkThreads / A::L;
   const int lane = threadIdx.x % A::L;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
@@ -150,16 +149,15 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint8_kernel(const __grid_co
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float v[A::N];
-#pragma unroll
-    for (int e = 0; e < A::N; ++e) v[e] = to_f(x[u].v[e]);
+    A::widen(x[u], v);
     const float s = A::template store_q<F>(p.q + row[u] * p.g.cols + col[u], lane, len[u], x[u], v);
     if (lane == 0 && len[u]) p.scale[first + u * S] = s;
   }
 }
 
-template <class T, bool VEC, int F, int U>
+template <class T, bool VEC, int F, int WV, int U>
 __global__ void __launch_bounds__(kCkThreads) restore8_kernel(const __grid_constant__ CkParams p) {
-  using A = Lanes<T, VEC>;
+  using A = Lanes<T, VEC, WV>;
   constexpr int S = kCkThreads / A::L;
   const int lane = threadIdx.x % A::L;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
@@ -180,7 +178,7 @@ __global__ void __launch_bounds__(kCkThreads) restore8_kernel(const __grid_const
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float v[A::N];
-    q8_widen<F, A::N>(q[u], s[u], v);
+    A::template widen_q<F>(q[u], s[u], v);
     A::store(static_cast<T*>(p.out) + row[u] * p.g.cols + col[u], lane, len[u], v);
   }
 }
@@ -217,9 +215,9 @@ struct GluParams {
 };
 
 // KEEP: also writes the 8-bit copies
-template <class T, bool VEC, int F, bool KEEP, int U>
+template <class T, bool VEC, int F, bool KEEP, int WV, int U>
 __global__ void __launch_bounds__(kCkThreads) silu_mul_kernel(const __grid_constant__ GluParams p) {
-  using A = Lanes<T, VEC>;
+  using A = Lanes<T, VEC, WV>;
   constexpr int S = kCkThreads / A::L;
   const int lane = threadIdx.x % A::L;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
@@ -237,12 +235,10 @@ __global__ void __launch_bounds__(kCkThreads) silu_mul_kernel(const __grid_const
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float a[A::N], b[A::N], h[A::N];
+    A::widen(ga[u], a);
+    A::widen(up[u], b);
 #pragma unroll
-    for (int e = 0; e < A::N; ++e) {
-      a[e] = to_f(ga[u].v[e]);
-      b[e] = to_f(up[u].v[e]);
-      h[e] = a[e] * sigmoid<T>(a[e]) * b[e];
-    }
+    for (int e = 0; e < A::N; ++e) h[e] = a[e] * sigmoid<T>(a[e]) * b[e];
     const int64_t at = row[u] * p.g.cols + col[u];
     A::store(static_cast<T*>(p.out) + at, lane, len[u], h);
     if constexpr (KEEP) {
@@ -257,9 +253,9 @@ __global__ void __launch_bounds__(kCkThreads) silu_mul_kernel(const __grid_const
 }
 
 // KEPT: gate and up come from their 8-bit copies
-template <class T, bool VEC, int F, bool KEPT, int U>
+template <class T, bool VEC, int F, bool KEPT, int WV, int U>
 __global__ void __launch_bounds__(kCkThreads) silu_mul_bwd_kernel(const __grid_constant__ GluParams p) {
-  using A = Lanes<T, VEC>;
+  using A = Lanes<T, VEC, WV>;
   constexpr int S = kCkThreads / A::L;
   const int lane = threadIdx.x % A::L;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (S * U) + threadIdx.x / A::L;
@@ -289,22 +285,20 @@ __global__ void __launch_bounds__(kCkThreads) silu_mul_bwd_kernel(const __grid_c
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float a[A::N], b[A::N], da[A::N], db[A::N];
+    float a[A::N], b[A::N], da[A::N], db[A::N], dv[A::N];
     if constexpr (KEPT) {
-      q8_widen<F, A::N>(qa[u], sa[u], a);
-      q8_widen<F, A::N>(qb[u], sb[u], b);
+      A::template widen_q<F>(qa[u], sa[u], a);
+      A::template widen_q<F>(qb[u], sb[u], b);
     } else {
-#pragma unroll
-      for (int e = 0; e < A::N; ++e) {
-        a[e] = to_f(ga[u].v[e]);
-        b[e] = to_f(up[u].v[e]);
-      }
+      A::widen(ga[u], a);
+      A::widen(up[u], b);
     }
+    A::widen(d[u], dv);
 #pragma unroll
     for (int e = 0; e < A::N; ++e) {
-      const float s = sigmoid<T>(a[e]), dv = to_f(d[u].v[e]);
-      da[e] = dv * b[e] * s * (1.f + a[e] * (1.f - s));
-      db[e] = dv * a[e] * s;
+      const float s = sigmoid<T>(a[e]);
+      da[e] = dv[e] * b[e] * s * (1.f + a[e] * (1.f - s));
+      db[e] = dv[e] * a[e] * s;
     }
     const int64_t at = row[u] * p.g.cols + col[u];
     A::store(static_cast<T*>(p.dgate) + at, lane, len[u], da);
@@ -357,7 +351,6 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
   const int64_t begin = min(worker * p.chunk, p.rows);
   const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
   const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.stride + seg;
-  const typename A::Shift x_shift(p.x, p.stride);
   if (rl < todo) A::copy(xbuf, x_at, seg_left, p.x);
   copy_commit();
   A::fill_factors(gbuf, left, [&](int o) { return p.gamma ? p.gamma[j0 + o] : 1.f; });
@@ -376,7 +369,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
       Vec<T, C> raw[GC];
 #pragma unroll
       for (int k = 0; k < GC; ++k) {
-        A::read_raw(xbuf, x_shift(begin + r0 + rl), c0 + k, live ? left : 0, raw[k]);
+        A::read_raw(xbuf, A::shift(p.x, p.stride, begin + r0 + rl), c0 + k, live ? left : 0, raw[k]);
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           x[(c0 + k) * C + e] = to_f(raw[k].v[e]);
@@ -424,7 +417,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
 // any length and alignment: a block per row, a warp per group
 template <class T, int F>
 __global__ void __launch_bounds__(256) rmsnorm8_stream_kernel(const __grid_constant__ Norm8Params p) {
-  using A = Lanes<T, false>;
+  using A = Lanes<T, false, 4>;
   __shared__ float red[2][1][8];
   RowFold<256, 1, 256> fold{red};
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -435,11 +428,9 @@ __global__ void __launch_bounds__(256) rmsnorm8_stream_kernel(const __grid_const
       const int len = static_cast<int>(min(int64_t{kQ8Group}, p.cols - g * kQ8Group));
       const typename A::Raw raw = A::load(x + g * kQ8Group, lane, len);
       float v[A::N];
+      A::widen(raw, v);
 #pragma unroll
-      for (int e = 0; e < A::N; ++e) {
-        v[e] = to_f(raw.v[e]);
-        s[0] = fmaf(v[e], v[e], s[0]);
-      }
+      for (int e = 0; e < A::N; ++e) s[0] = fmaf(v[e], v[e], s[0]);
       const float sc = A::template store_q<F>(p.q + row * p.cols + g * kQ8Group, lane, len, raw, v);
       if (lane == 0) p.scale[row * p.groups + g] = sc;
     }
@@ -470,8 +461,6 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
   A::zero_rest(dbuf, true, left);
   Q::zero_rest(qbuf, true, left);
   const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
-  const typename A::Shift dy_shift(p.dy, p.stride);
-  const typename Q::Shift q_shift(p.q, p.cols);
   const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   const int64_t begin = min(worker * p.chunk, p.rows);
   const int todo = static_cast<int>(min(p.chunk, p.rows - begin));
@@ -520,10 +509,10 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float g[C];
-        A::read_raw(dbuf, dy_shift(row), c, left, dy[c]);
+        A::read_raw(dbuf, A::shift(p.dy, p.stride, row), c, left, dy[c]);
         A::read_factors(gbuf, c, g);
         Vec<uint8_t, C> lv;
-        Q::read_raw(qbuf, q_shift(row), c, left, lv);
+        Q::read_raw(qbuf, Q::shift(p.q, p.cols, row), c, left, lv);
         const float sc = sc_next[c / GC];
         if constexpr (V > 1) {
           q8_widen<F, V>(*reinterpret_cast<const typename Q8Raw<V>::type*>(&lv), sc, *reinterpret_cast<float(*)[V]>(&x[c * C]));
@@ -553,7 +542,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float d[C], g[C];
-        if constexpr (!kEarly) A::read_raw(dbuf, dy_shift(row), c, left, dy[c]);
+        if constexpr (!kEarly) A::read_raw(dbuf, A::shift(p.dy, p.stride, row), c, left, dy[c]);
         A::read_factors(gbuf, c, g);
 #pragma unroll
         for (int e = 0; e < C; ++e) d[e] = fmaf(inv * to_f(dy[c].v[e]), g[e], -k * x[c * C + e]);
@@ -639,13 +628,13 @@ void launch_checkpoint(const CkParams& p, int format, bool restore, cudaStream_t
   constexpr int VW = 16 / sizeof(T);
   const bool vec = p.g.cols % VW == 0 && p.x_stride % VW == 0 && a16(p.x) && a16(p.out) &&
                    reinterpret_cast<uintptr_t>(p.q) % VW == 0;
-  constexpr int U = 2;
+  constexpr int WV = kCopyVecs, U = 1;
   unsigned grid = 0;
 #define VB_CK(VEC)                                                                   \
   do {                                                                               \
-    grid = flat_grid(p.g.total, Lanes<T, VEC>::L, U);                                \
-    if (restore) VB_FORMAT(format, F, (restore8_kernel<T, VEC, F, U><<<grid, kCkThreads, 0, s>>>(p)));    \
-    else VB_FORMAT(format, F, (checkpoint8_kernel<T, VEC, F, U><<<grid, kCkThreads, 0, s>>>(p)));         \
+    grid = flat_grid(p.g.total, Lanes<T, VEC, WV>::L, U);                            \
+    if (restore) VB_FORMAT(format, F, (restore8_kernel<T, VEC, F, WV, U><<<grid, kCkThreads, 0, s>>>(p)));    \
+    else VB_FORMAT(format, F, (checkpoint8_kernel<T, VEC, F, WV, U><<<grid, kCkThreads, 0, s>>>(p)));         \
   } while (0)
   if (vec) VB_CK(true);
   else VB_CK(false);
@@ -662,15 +651,15 @@ void launch_glu(const GluParams& p, int format, bool backward, bool kept, cudaSt
              p.dout_stride % VW == 0 && q_ok(p.q_gate) && q_ok(p.q_up);
   if (backward && kept) vec = vec && q_ok(p.gate) && q_ok(p.up);
   else vec = vec && a16(p.gate) && a16(p.up) && p.gate_stride % VW == 0 && p.up_stride % VW == 0;
-  constexpr int U = 1;
+  constexpr int WV = kGluVecs, U = 1;
   unsigned grid = 0;
 #define VB_GLU(VEC)                                                                                             \
   do {                                                                                                          \
-    grid = flat_grid(p.g.total, Lanes<T, VEC>::L, U);                                                           \
-    if (!backward && !kept) silu_mul_kernel<T, VEC, 0, false, U><<<grid, kCkThreads, 0, s>>>(p);                \
-    else if (!backward) VB_FORMAT(format, F, (silu_mul_kernel<T, VEC, F, true, U><<<grid, kCkThreads, 0, s>>>(p)));   \
-    else if (!kept) silu_mul_bwd_kernel<T, VEC, 0, false, U><<<grid, kCkThreads, 0, s>>>(p);                    \
-    else VB_FORMAT(format, F, (silu_mul_bwd_kernel<T, VEC, F, true, U><<<grid, kCkThreads, 0, s>>>(p)));              \
+    grid = flat_grid(p.g.total, Lanes<T, VEC, WV>::L, U);                                                       \
+    if (!backward && !kept) silu_mul_kernel<T, VEC, 0, false, WV, U><<<grid, kCkThreads, 0, s>>>(p);                \
+    else if (!backward) VB_FORMAT(format, F, (silu_mul_kernel<T, VEC, F, true, WV, U><<<grid, kCkThreads, 0, s>>>(p)));   \
+    else if (!kept) silu_mul_bwd_kernel<T, VEC, 0, false, WV, U><<<grid, kCkThreads, 0, s>>>(p);                    \
+    else VB_FORMAT(format, F, (silu_mul_bwd_kernel<T, VEC, F, true, WV, U><<<grid, kCkThreads, 0, s>>>(p)));              \
   } while (0)
   if (vec) VB_GLU(true);
   else VB_GLU(false);

@@ -292,9 +292,9 @@ int launch_read(KvReadParams p, int format, cudaStream_t s) {
   p.tb = static_cast<int>(std::min<int64_t>(tb, kKvMaxTokens));
   const unsigned g = static_cast<unsigned>((p.rows + p.tb - 1) / p.tb);
 #define VB_KR(V) VB_KV_FORMAT(format, F, (kv_read_kernel<T, V, F, U><<<g, kKvThreads, 0, s>>>(p)))
-  if (v == 8) VB_KR(8);
-  else if (v == 4) VB_KR(4);
-  else VB_KR(1);
+  if (v == 4) VB_KR(4);
+  else if (v == 1) VB_KR(1);
+  else if constexpr (sizeof(T) == 2) VB_KR(8);
 #undef VB_KR
   note_launch(VBT_B200_FAMILY_INDEX, VBT_B200_IK_KV_CACHE_READ, dim3(g), dim3(kKvThreads), v, 1, 0, 1,
               2 * p.rows * p.heads * p.dim, p.rows, 0, s);

@@ -75,7 +75,6 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
   const T* x_at = static_cast<const T*>(p.x) + (begin + rl) * p.x_stride + seg;
   const T* y_at = static_cast<const T*>(p.y) + (begin + rl) * p.y_stride + seg;
   const T* gate_at = static_cast<const T*>(p.gate) + (begin + rl) * p.gate_stride + seg;  // GATE_ROW
-  const typename A::Shift x_shift(p.x, p.x_stride), y_shift(p.y, p.y_stride), gate_shift(p.gate, p.gate_stride);
   int ahead = rl;
   auto fetch = [&] {
     if (ahead < todo) {
@@ -115,7 +114,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
           float y[C];
-          A::read(buf(0), y_shift(row), c, left, y);
+          A::read(buf(0), A::shift(p.y, p.y_stride, row), c, left, y);
 #pragma unroll
           for (int e = 0; e < C; ++e) s[0] = fmaf(y[e], y[e], s[0]);
         }
@@ -129,12 +128,12 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float x[C], y[C], w[C];
-        A::read(buf(0), y_shift(row), c, left, y);
-        A::read(buf(1), x_shift(row), c, left, x);
+        A::read(buf(0), A::shift(p.y, p.y_stride, row), c, left, y);
+        A::read(buf(1), A::shift(p.x, p.x_stride, row), c, left, x);
         A::read_factors(wbuf, c, w);
         if constexpr (GATE_ROW) {
           float gt[C];
-          A::read(buf(2), gate_shift(row), c, left, gt);
+          A::read(buf(2), A::shift(p.gate, p.gate_stride, row), c, left, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }

@@ -91,10 +91,10 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
   const int64_t workers = TPR ? static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) : gridDim.x / ranks;
   // the worker's units [u, last) are one run of rows; a unit's rows are taken RW at a time
   struct Walk {
-    int64_t u;
+    int u;
     int todo, left;  // rows of the worker, rows of the unit still to take
     __device__ __forceinline__ void enter(const JoinBwdParams& q) {
-      const int64_t cut = u % q.cuts;
+      const int cut = u % static_cast<int>(q.cuts);
       left = static_cast<int>(min(q.chunk, q.per - cut * q.chunk));
     }
     // takes the next rows; returns how many
@@ -111,44 +111,35 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     const int64_t group = u / p.cuts;
     return group * p.per + (u - group * p.cuts) * p.chunk;
   };
-  const int64_t row0 = first_row(u0) + rl;
-  const typename A::Shift dr_shift(p.dr, p.dr_stride), dn_shift(p.dn, p.dn_stride), r_shift(p.r, p.r_stride),
-      y_shift(p.y, p.y_stride), gate_shift(p.gate, p.gate_stride);
+  const int row0 = static_cast<int>(first_row(u0)) + rl;  // rows are fewer than 2^31
   // an absent array reads as zeros
   const int dr_left = p.dr ? left : 0, pre_left = p.pre ? left : 0, y_left = p.y ? left : 0;
   Walk at;
-  at.u = u0;
+  at.u = static_cast<int>(u0);
   at.left = 0;
   at.todo = u0 < u1 ? static_cast<int>(first_row(u1) - first_row(u0)) : 0;
   if (at.todo) at.enter(p);
   Walk ahead = at;
-  const T* dr_at = static_cast<const T*>(p.dr) + row0 * p.dr_stride + seg;
-  const T* dn_at = static_cast<const T*>(p.dn) + row0 * p.dn_stride + seg;
-  const T* r_at = static_cast<const T*>(p.r) + row0 * p.r_stride + seg;
-  const T* y_at = static_cast<const T*>(p.y) + row0 * p.y_stride + seg;
-  const T* gate_at = static_cast<const T*>(p.gate) + row0 * p.gate_stride + seg;  // GATE_ROW
-  const float* inv1_at = p.inv1 + row0;
-  const float* inv2_at = p.inv2 + row0;
+  // rows are addressed from their number: a running pointer per array is 20 registers of the 128
+  int row = row0, row_ahead = row0;
+  auto at_row = [&](const void* base, int64_t stride, int r) { return static_cast<const T*>(base) + r * stride + seg; };
   float i1_next[STAGES], i2_next[STAGES];
   auto fetch = [&](int stage, float& i1, float& i2) {
     i1 = 1.f;
     i2 = 0.f;
     if (ahead.todo > 0) {
       if (RW == 1 || rl < ahead.left) {
-        if (p.dr) A::copy(buf(stage, 0), dr_at, seg_left, p.dr);
+        if (p.dr) A::copy(buf(stage, 0), at_row(p.dr, p.dr_stride, row_ahead), seg_left, p.dr);
         if (p.pre) {
-          A::copy(buf(stage, 1), dn_at, seg_left, p.dn);
-          A::copy(buf(stage, 2), r_at, seg_left, p.r);
-          i2 = *inv2_at;
+          A::copy(buf(stage, 1), at_row(p.dn, p.dn_stride, row_ahead), seg_left, p.dn);
+          A::copy(buf(stage, 2), at_row(p.r, p.r_stride, row_ahead), seg_left, p.r);
+          i2 = p.inv2[row_ahead];
         }
-        if (p.y) A::copy(buf(stage, 3), y_at, seg_left, p.y);
-        if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), gate_at, seg_left, p.gate);
-        if (p.post) i1 = *inv1_at;
+        if (p.y) A::copy(buf(stage, 3), at_row(p.y, p.y_stride, row_ahead), seg_left, p.y);
+        if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), at_row(p.gate, p.gate_stride, row_ahead), seg_left, p.gate);
+        if (p.post) i1 = p.inv1[row_ahead];
       }
-      const int n = ahead.next(p);
-      dr_at += n * p.dr_stride; dn_at += n * p.dn_stride; r_at += n * p.r_stride; y_at += n * p.y_stride;
-      if constexpr (MODE == GATE_ROW) gate_at += n * p.gate_stride;
-      inv1_at += n; inv2_at += n;
+      row_ahead += ahead.next(p);
     }
     copy_commit();
   };
@@ -168,16 +159,12 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     }
   };
   const T* gate = nullptr;
-  T* dx = static_cast<T*>(p.dx) + row0 * p.cols + j0;
-  T* dy = static_cast<T*>(p.dy) + row0 * p.cols + j0;
-  T* dgate = static_cast<T*>(p.dgate) + row0 * p.cols + j0;  // GATE_ROW
   bool first_unit = true, enter = true;
   int phase = 0, stage = 0;
-  int64_t row = row0;
   while (at.todo > 0) {
     if constexpr (MODE == GATE_SHARED) {
       if (enter) {
-        gate = static_cast<const T*>(p.gate) + at.u / p.cuts * p.gate_stride + j0;
+        gate = static_cast<const T*>(p.gate) + at.u / static_cast<int>(p.cuts) * p.gate_stride + j0;
         A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
       }
     }
@@ -191,15 +178,15 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float dr[C], dn[C], r[C], y[C], w[C], g2[C];
-        A::read(buf(stage, 0), dr_shift(row), c, dr_left, dr);
-        A::read(buf(stage, 1), dn_shift(row), c, pre_left, dn);
-        A::read(buf(stage, 2), r_shift(row), c, pre_left, r);
-        A::read(buf(stage, 3), y_shift(row), c, y_left, y);
+        A::read(buf(stage, 0), A::shift(p.dr, p.dr_stride, row), c, dr_left, dr);
+        A::read(buf(stage, 1), A::shift(p.dn, p.dn_stride, row), c, pre_left, dn);
+        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, pre_left, r);
+        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y_left, y);
         A::read_factors(wbuf, c, w);
         A::read_factors(gbuf, c, g2);
         if constexpr (MODE == GATE_ROW) {
           float gt[C];
-          A::read(buf(stage, 4), gate_shift(row), c, left, gt);
+          A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, left, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }
@@ -219,13 +206,14 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     const float c2 = i2 * i2 * i2 * s[0] * inv_cols;
     const float c1 = p.post ? i1 * i1 * i1 * (s[1] - c2 * s[2]) * inv_cols : 0.f;
     if (live) {
+      const int64_t o = static_cast<int64_t>(row) * p.cols + j0;
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float r[C], y[C], w[C], gt[C], ox[C], oy[C], og[C];
-        A::read(buf(stage, 2), r_shift(row), c, pre_left, r);
-        A::read(buf(stage, 3), y_shift(row), c, y_left, y);
+        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, pre_left, r);
+        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y_left, y);
         A::read_factors(wbuf, c, w);
-        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), gate_shift(row), c, left, gt);
+        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, left, gt);
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           const int i = c * C + e;
@@ -242,10 +230,10 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
           // without the norm (c1 = 0, i1 = 1) dy does not depend on y, not even on a NaN in it
           oy[e] = p.post ? fmaf(Gi, w[e], -c1 * y[e]) : Gi * w[e];
         }
-        A::write(dx, c, left, ox);
-        A::write(dy, c, left, oy);
+        A::write(static_cast<T*>(p.dx) + o, c, left, ox);
+        A::write(static_cast<T*>(p.dy) + o, c, left, oy);
         if constexpr (MODE == GATE_ROW) {
-          if (p.dgate) A::write(dgate, c, left, og);
+          if (p.dgate) A::write(static_cast<T*>(p.dgate) + o, c, left, og);
         }
       }
     }
@@ -257,15 +245,13 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     A::sync();
     fetch(stage, i1_next[STAGES - 1], i2_next[STAGES - 1]);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
-    const int64_t unit = at.u;
-    const int n = at.next(p);
-    row += n;
-    dx += n * p.cols; dy += n * p.cols; dgate += n * p.cols;
+    const int unit = at.u;
+    row += at.next(p);
     enter = at.todo == 0 || at.u != unit;
     if constexpr (MODE == GATE_SHARED) {
       if (!enter) continue;
       over_rows(sum1);
-      const int64_t group = unit / p.cuts;
+      const int64_t group = unit / static_cast<int>(p.cuts);
       if (rl == 0) {
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
@@ -606,7 +592,7 @@ vbt_b200_status vbt_b200_residual_norm_backward(
   using namespace vb;
   const char* name = "residual_norm_backward";
   VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
-  VB_ARG(rows < (int64_t{1} << 36), std::string(name) + ": too many rows");
+  VB_ARG(rows < (int64_t{1} << 31), std::string(name) + ": too many rows");
   VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
   const bool pre = flags & VBT_B200_RESNORM_PRE, post = flags & VBT_B200_RESNORM_POST;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

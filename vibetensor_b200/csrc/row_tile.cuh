@@ -161,14 +161,11 @@ template <class T, int V, int TPR, int E> struct RowChunks {
     if constexpr (V == 1) __syncwarp();
   }
   // the shift of a row's segment: rows of `stride` values from `first` on
-  struct Shift {
-    int at0, step;
-    __device__ __forceinline__ Shift(const void* first, int64_t stride)
-        : at0(static_cast<int>(reinterpret_cast<uintptr_t>(first) & 15)), step(static_cast<int>(stride * ELT) & 15) {}
-    __device__ __forceinline__ int operator()(int64_t row) const {
-      return V > 1 ? 0 : (at0 + (static_cast<int>(row) & 15) * step) & 15;
-    }
-  };
+  static __device__ __forceinline__ int shift(const void* first, int64_t stride, int64_t row) {
+    if constexpr (V > 1) return 0;
+    return static_cast<int>((static_cast<uint32_t>(reinterpret_cast<uintptr_t>(first)) +
+                             static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) * ELT) & 15u);
+  }
   // starts the copies of a segment: `seg` points at its first column, `len` values of the row lie from
   // there on, `floor` is the tensor's first value
   static __device__ __forceinline__ void copy(unsigned char* array, const T* seg, int len, const void* floor) {
