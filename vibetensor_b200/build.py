@@ -29,11 +29,6 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--default-stream", "legacy",
 ]
 
-# Flags of single files.  The backward of residual_norm keeps two sums per column in registers; compiled
-# function by function its kernels fit their 128 registers, compiled as one module several spill
-# ([16384,4095] bf16: 253 against 341 us).
-FILE_FLAGS = {"residual_norm_bwd.cu": ["--split-compile=8"]}
-
 
 def _nvcc() -> str:
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
@@ -64,7 +59,7 @@ def build(force: bool = False, verbose: bool = False, release: bool = False) -> 
         o = os.path.join(OBJ, os.path.basename(s)[:-3] + suffix)
         objs.append(o)
         if force or _stale(o, [s] + hdrs):
-            cmd = [nvcc] + flags + FILE_FLAGS.get(os.path.basename(s), []) + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o]
+            cmd = [nvcc] + flags + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o]
             jobs.append(cmd)
 
     def run(cmd):

@@ -52,13 +52,16 @@ struct JoinBwdParams {
 // registers between the two passes.  w = b * gate * g1 and g2 lie beside them.
 // The sum over a unit of G * y * i1 gives the gate's gradient (times b * g1) and the unit's part of
 // dgamma_post (times b * gate).  A gate row of its own per row (GATE_ROW) is a factor of the sum.
-constexpr int kBwdElts = 16;        // values of a row per thread
+// Values of a row per thread: two sums per column and the gradient at r stay in registers for each.
+// Single values need more registers around them.
+constexpr int kVecElts = 16, kSingleElts = 8;
 constexpr int kBwdMaxThreads = 512;   // of a block that shares a row
 
 template <class T, int V, int TPR, int MODE, int STAGES>
 __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
-  using A = RowChunks<T, V, TPR, kBwdElts>;
-  constexpr int C = A::C, E = kBwdElts;
+  constexpr int E = V > 1 ? kVecElts : kSingleElts;
+  using A = RowChunks<T, V, TPR, E>;
+  constexpr int C = A::C;
   constexpr int RW = TPR ? 32 / TPR : 1;                 // rows a worker takes at once
   constexpr int ARRAYS = MODE == GATE_ROW ? 5 : 4;       // dr, dn, r, y, gate
   extern __shared__ __align__(16) unsigned char smem[];
@@ -124,10 +127,11 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
   int row = row0, row_ahead = row0;
   auto at_row = [&](const void* base, int64_t stride, int r) { return static_cast<const T*>(base) + r * stride + seg; };
   float i1_next[STAGES], i2_next[STAGES];
+  const int row_end = row0 + at.todo;
   auto fetch = [&](int stage, float& i1, float& i2) {
     i1 = 1.f;
     i2 = 0.f;
-    if (ahead.todo > 0) {
+    if (RW == 1 ? row_ahead < row_end : ahead.todo > 0) {
       if (RW == 1 || rl < ahead.left) {
         if (p.dr) A::copy(buf(stage, 0), at_row(p.dr, p.dr_stride, row_ahead), seg_left, p.dr);
         if (p.pre) {
@@ -139,7 +143,9 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
         if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), at_row(p.gate, p.gate_stride, row_ahead), seg_left, p.gate);
         if (p.post) i1 = p.inv1[row_ahead];
       }
-      row_ahead += ahead.next(p);
+      // the rows of a worker follow one another; several at once stop at a unit's end
+      if constexpr (RW == 1) ++row_ahead;
+      else row_ahead += ahead.next(p);
     }
     copy_commit();
   };
@@ -158,13 +164,14 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
         for (int d = TPR; d < 32; d <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
     }
   };
-  const T* gate = nullptr;
+  // the gate row of unit u, from this thread's first column on
+  auto gate_of = [&](int u) { return static_cast<const T*>(p.gate) + u / static_cast<int>(p.cuts) * p.gate_stride + j0; };
   bool first_unit = true, enter = true;
   int phase = 0, stage = 0;
   while (at.todo > 0) {
     if constexpr (MODE == GATE_SHARED) {
       if (enter) {
-        gate = static_cast<const T*>(p.gate) + at.u / static_cast<int>(p.cuts) * p.gate_stride + j0;
+        const T* gate = gate_of(at.u);
         A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
       }
     }
@@ -252,6 +259,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       if (!enter) continue;
       over_rows(sum1);
       const int64_t group = unit / static_cast<int>(p.cuts);
+      const T* gate = gate_of(unit);
       if (rl == 0) {
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
@@ -430,10 +438,11 @@ struct JoinShape {
 };
 inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) {
   JoinShape h{0, 0, 0, 0, 4, 1};
-  const int64_t lanes = (cols + kBwdElts - 1) / kBwdElts;
+  const int elts = vec ? kVecElts : kSingleElts;
+  const int64_t lanes = (cols + elts - 1) / elts;
   if (lanes > int64_t{kBwdMaxThreads} * kMaxRanks) return h;
   h.tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;
-  const int factors = 2 * kBwdElts * 4, row = (gate_row ? 5 : 4) * row_bytes_per_thread(kBwdElts, elt, vec, h.tpr);
+  const int factors = 2 * elts * 4, row = (gate_row ? 5 : 4) * row_bytes_per_thread(elts, elt, vec, h.tpr);
   auto smem = [&](int stages) { return h.threads * (factors + stages * row) + (h.tpr ? 0 : sum_bytes(h.ranks)); };
   for (h.ranks = 1; h.ranks <= kMaxRanks; h.ranks *= 2) {
     const int64_t part = (lanes + h.ranks - 1) / h.ranks;
