@@ -655,6 +655,33 @@ def test_cache_bad_slots_and_pages(cache):
     c.write(k[:0], v[:0], torch.empty(0, dtype=torch.int64, device="cuda"))
 
 
+def test_cache_starts_that_do_not_ascend(cache):
+    # the search for row 0's sequence ends at sequence 0, which starts at 100: no position of it
+    from vibetensor_b200 import ops
+    c = cache.QuantCache(4, 16, 2, 32)
+    k = torch.ones(64, 2, 32, device="cuda")
+    c.write(k, k, torch.arange(64, device="cuda"))
+    table = torch.zeros((32, 4), dtype=torch.int64, device="cuda")
+    starts = torch.full((33,), 100, device="cuda")
+    starts[20] = 0
+    st = ops.IndexStatus("cuda")
+    rk, rv = c.read(table, starts, 64, dtype=F32, status=st)
+    assert (rk == 0).all() and (rv == 0).all()
+    with pytest.raises(IndexError, match="64 bad indices"):
+        st.check("QuantCache.read", c.num_pages)
+
+
+def test_cache_status_on_the_cache_device(cache):
+    from vibetensor_b200 import ops
+    c = cache.QuantCache(1, 4, 2, 32)
+    k, st = torch.ones(1, 2, 32, device="cuda"), ops.IndexStatus("cpu")
+    slots = torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(RuntimeError, match="requires CUDA tensors"):
+        c.write(k, k, slots, status=st)
+    with pytest.raises(RuntimeError, match="requires CUDA tensors"):
+        c.read(slots[None], torch.arange(2, device="cuda"), 1, status=st)
+
+
 def test_cache_special_rows(cache):
     c = cache.QuantCache(2, 4, 2, 16)
     k = torch.ones((3, 2, 16), device="cuda")

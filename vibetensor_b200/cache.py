@@ -51,6 +51,12 @@ class QuantCache:
     def device(self):
         return self.k.device
 
+    def _status(self, what: str, status):
+        if status is None:
+            return None
+        self._on_device(what, status.buf)
+        return status.ptr
+
     def _on_device(self, what: str, *ts: torch.Tensor) -> None:
         device = self.k.get_device()
         for t in ts:
@@ -88,7 +94,7 @@ class QuantCache:
             self.k.data_ptr(), self.k_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(), self.num_slots,
             self.num_heads, self.head_dim, self._code, k.data_ptr(), _I64x2(*k.stride()[:2]), v.data_ptr(),
             _I64x2(*v.stride()[:2]), dtype_code(k.dtype), slots.data_ptr(), dtype_code(slots.dtype), slots.shape[0],
-            self._owner.data_ptr(), status.ptr if status is not None else None, stream_ptr(self.k)))
+            self._owner.data_ptr(), self._status(what, status), stream_ptr(self.k)))
 
     def read(self, page_table: torch.Tensor, starts: torch.Tensor, total: Optional[int] = None,
              dtype: torch.dtype = torch.bfloat16, out=None, status=None):
@@ -99,9 +105,9 @@ class QuantCache:
         device.  Returns (k, v), each [total, num_heads, head_dim] of ``dtype``; rows that no
         sequence owns are zero.  With ``out`` (a pair of dense tensors) their row count and dtype
         count instead of ``total`` and ``dtype``, and rows that no sequence owns are left as they
-        are.  A page outside the cache, or a position behind the table's last page, reads as zeros and is
-        counted in ``status`` (an ops.IndexStatus, checked against ``num_pages``) when one is
-        given."""
+        are.  A page outside the cache, a position behind the table's last page, or one in front of
+        its sequence (starts that do not ascend) reads as zeros and is counted in ``status`` (an
+        ops.IndexStatus, checked against ``num_pages``) when one is given."""
         what = "QuantCache.read"
         self._on_device(what, page_table, starts)
         if page_table.dtype not in (torch.int64, torch.int32):
@@ -137,5 +143,5 @@ class QuantCache:
             self.v.data_ptr(), self.v_scale.data_ptr(), self.num_slots, self.page_size, self.num_heads, self.head_dim,
             self._code, page_table.data_ptr() if page_table.numel() else None, dtype_code(page_table.dtype), page_table.stride(0),
             page_table.shape[1], starts.data_ptr(), page_table.shape[0], int(out is None),
-            status.ptr if status is not None else None, stream_ptr(self.k)))
+            self._status(what, status), stream_ptr(self.k)))
         return ko, vo
