@@ -8,6 +8,15 @@
 // The second mean needs G, which needs the first.  It splits into sums that do not:
 //   sum(dv g1 y) = sum(w y (dr + i2 dn g2)) - c sum(w y r),  w = b gate g1, c = i2^3 mean(dn g2 r),
 // so a row costs one reduction of three sums.
+//
+// Bound by memory and, close behind, by instructions: four rows read, two written, 14 fp32 operations
+// and six conversions per value.  [32768,4096] bf16 with a gate row per 4096 rows takes 295 us = 5.5
+// TB/s, 0.83 of the measured copy bandwidth (16 warps per SM at 128 registers, half of the issue slots
+// busy).  What it came through: rows in registers 678 us; staged by asynchronous copies 370; one base per
+// warp and compile-time offsets instead of an address per access (744 instructions per warp and row
+// against 964) 314; units of neighbouring rows rather than every n-th one 306 (379).  Arithmetic on
+// float pairs was slower here (335: moves to pair the registers), and so were one block per SM with
+// four rows in flight (759), eight values per thread (424), and one row in flight (333).
 #include <algorithm>
 
 #include "row_tile.cuh"
@@ -65,13 +74,13 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
   constexpr int RW = TPR ? 32 / TPR : 1;                 // rows a worker takes at once
   constexpr int ARRAYS = MODE == GATE_ROW ? 5 : 4;       // dr, dn, r, y, gate
   extern __shared__ __align__(16) unsigned char smem[];
-    const int ranks = TPR ? 1 : p.ranks;
+  const int ranks = TPR ? 1 : p.ranks;
   const int warp0 = ranks > 1 ? cluster_rank() * static_cast<int>(blockDim.x >> 5) : 0;
   if (ranks > 1) cluster_sync();  // the other blocks' shared memory is there
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
   const int j0 = A::base(warp0), left = static_cast<int>(p.cols) - j0;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
-  // a warp's part of the shared memory: w, g2, then `stages` times the arrays
+  // a warp's part of the shared memory: w, g2, then STAGES times the arrays
   unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY);
   float4* red = reinterpret_cast<float4*>(smem + static_cast<size_t>(blockDim.x >> 5) *
                                                      (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY));
@@ -447,7 +456,11 @@ inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) 
   for (h.ranks = 1; h.ranks <= kMaxRanks; h.ranks *= 2) {
     const int64_t part = (lanes + h.ranks - 1) / h.ranks;
     h.threads = h.tpr ? 256 : static_cast<int>((part + 31) / 32 * 32);
-    if (h.threads > kBwdMaxThreads) continue;
+    // Of a shared row, two blocks of 256 threads per SM overlap one's reduction with the other's copies:
+    // [8192,16384] bf16 641 -> 548 us with four blocks per row, fp32 [4096,16384] 567 -> 500.  Not with a
+    // gate row per row (652 -> 765: two rows in flight of five arrays leave room for one block), nor
+    // where one block holds the row (8192 columns: 434 -> 532).
+    if (h.threads > (h.ranks > 1 && h.ranks < kMaxRanks && !gate_row ? 384 : kBwdMaxThreads)) continue;
     // two rows ahead where they fit; the warp forms are built for that alone
     h.stages = 2;
     if (!h.tpr && smem(2) > kSmemPerBlock) h.stages = 1;

@@ -54,22 +54,6 @@ __device__ __forceinline__ void load_vecs(const T* row, int first, int step, int
     }
   }
 }
-template <int V>
-__device__ __forceinline__ void load_floats(const float* src, int j, int nvec, float (&v)[V], float other) {
-  if (src == nullptr || j >= nvec) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = other;
-  } else if constexpr (V % 4 == 0) {
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(src + static_cast<int64_t>(j) * V) + q);
-      v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = __ldg(src + static_cast<int64_t>(j) * V + e);
-  }
-}
 inline bool a16(const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; }
 
 // Sums the n rows of src[n][cols] for the 8 columns of a strip (one 32-byte sector per row) with
