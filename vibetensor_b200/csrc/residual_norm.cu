@@ -6,6 +6,10 @@
 //
 // The two sums stay apart: sum(r^2) expanded in x and v would save a reduction and cancel where the
 // branch nearly undoes the stream.
+//
+// Bound by memory: two rows read, two written.  [32768,4096] bf16 with a gate row per 4096 rows takes
+// 178 us = 6.0 TB/s, 0.92 of the measured copy bandwidth; rows in registers, read when they are
+// needed, took 254 us (93 registers, two blocks per SM, nothing in flight during the reductions).
 #include <algorithm>
 
 #include "row_tile.cuh"
@@ -52,7 +56,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
   constexpr int RW = TPR ? 32 / TPR : 1;
   constexpr int ARRAYS = GATE_ROW ? 3 : 2;
   extern __shared__ __align__(16) unsigned char smem[];
-    const int ranks = TPR ? 1 : p.ranks;
+  const int ranks = TPR ? 1 : p.ranks;
   const int warp0 = ranks > 1 ? cluster_rank() * static_cast<int>(blockDim.x >> 5) : 0;
   if (ranks > 1) cluster_sync();  // the other blocks' shared memory is there
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
