@@ -187,3 +187,37 @@ def test_overlap_of_views():
     assert _overlap(q, q) and not _overlap(q, q.clone())
     assert not _overlap(q[:1], q[1:]) and _overlap(q[:, :3], q[:, 2:])
     assert not _overlap(q[:, :0], q)
+
+
+class OnCard(torch.Tensor):
+    """A CPU tensor that passes for a CUDA one where only its shape and strides are looked at."""
+    is_cuda = property(lambda self: True)
+
+
+@pytest.mark.parametrize("x", [
+    pytest.param(torch.arange(4 * 48).reshape(4, 1, 48).chunk(6, -1)[1], id="one part of a projection, one row per sample"),
+    pytest.param(torch.arange(4 * 48).reshape(4, 1, 1, 48)[..., 8:16], id="the same, two axes of one"),
+    pytest.param(torch.arange(6 * 48).reshape(2, 3, 1, 48)[..., 8:16], id="one row per sample and step"),
+    pytest.param(torch.arange(6 * 48).reshape(1, 6, 48)[..., 8:16], id="a leading axis of one"),
+    pytest.param(torch.arange(6 * 48).reshape(2, 1, 3, 48)[..., 8:16], id="an axis of one in the middle"),
+    pytest.param(torch.arange(4 * 5 * 8).reshape(4, 5, 8)[:, -1:], id="the last token of each sample"),
+    pytest.param(torch.arange(4 * 6 * 8).reshape(4, 6, 8)[:, ::2], id="every other token"),
+    pytest.param(torch.arange(4 * 6 * 8).reshape(4, 6, 8)[:, 1:4], id="some tokens of each sample"),
+    pytest.param(torch.arange(4 * 6 * 8).reshape(4, 6, 8).transpose(0, 1), id="samples behind tokens"),
+    pytest.param(torch.arange(8).expand(5, 8), id="one row for all"),
+    pytest.param(torch.arange(4 * 8).reshape(4, 1, 8).expand(4, 3, 8), id="one row per sample for all tokens"),
+    pytest.param(torch.arange(999).as_strided((4, 1, 8), (48, 7, 1)), id="an axis of one with a stride of its own"),
+    pytest.param(torch.arange(96).reshape(1, 1, 96)[..., 8:16], id="one row"),
+    pytest.param(torch.arange(4 * 6).reshape(4, 6)[:, 2:3], id="single values"),
+    pytest.param(torch.arange(48)[::3], id="a strided row"),
+    pytest.param(torch.arange(48).reshape(6, 8).t(), id="columns"),
+])
+def test_rows_of_a_view(monkeypatch, x):
+    """What the row ops hand to a kernel -- a first value, a number of rows and one stride -- reaches the
+    view's own values, whatever axes of one lie between."""
+    from vibetensor_b200 import kernels
+    monkeypatch.setattr(kernels._ops, "contiguous", lambda t: t.contiguous())
+    monkeypatch.setattr(kernels, "_FLOATS", (torch.int64,))
+    view, rows, cols, stride = kernels._rows_view(x.as_subclass(OnCard), "rows")
+    got = view.as_subclass(torch.Tensor).as_strided((rows, cols), (stride, 1))
+    assert torch.equal(got, x.reshape(-1, x.shape[-1]))

@@ -976,3 +976,47 @@ def test_refusals(kernels, cache):
                       (lambda: cache.QuantCache(2, 4, 3, 16, device="cpu"), RuntimeError)):
         with pytest.raises(exc):
             call()
+
+
+# ------------------------------------------------------------------------ views with an axis of one
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [64, 129, 1024])
+def test_parts_of_a_projection_with_one_token_or_row_per_sample(kernels, dtype, cols):
+    """[batch, 1, k * cols] cut along its last axis: a modulation row per sample, or the one new token of
+    each request.  Every sample's own row counts, as in the dense copy of the part."""
+    g = gen(cols + 1)
+    batch, tokens = 5, 7
+    gam = 1 + 0.1 * randn(g, (cols,))
+    mod = randn(g, (batch, 1, 6 * cols), dtype)
+    x, y, dr, dn = (randn(g, (batch, tokens, cols), dtype) for _ in range(4))
+
+    def same(call, *views):
+        # the reads of an unaligned part go another way, the arithmetic per value does not
+        got, want = call(*views), call(*(v.contiguous() for v in views))
+        for a, b in zip(got, want):
+            if a is not None:
+                close("a part of a projection", a, b.double(), b.double().abs() + 1.0)
+    for i in (1, 5):
+        gate = mod.chunk(6, -1)[i]
+        assert not gate.is_contiguous()
+        r, n, i1, i2 = kernels.residual_norm(x, y, gam, gate, gam)
+        w = join_ref(x, y, gam, gate, gam, 1e-6, True, True, 1.0, 1.0)
+        close("residual_norm r, a part as the gate", r, w["r"], w["mass"])
+        got = dict(zip(("dx", "dy", "dgp", "dgate", "dgn"),
+                       kernels.residual_norm_backward(dr, dn, y, r, i1, i2, gam, gate, gam)))
+        for name, (t, mass) in join_bwd_ref(dr, dn, y, r, i1, i2, gam, gate, gam, 1.0, 1.0).items():
+            close(f"residual_norm_backward {name}, a part as the gate", got[name], t, mass)
+    new = mod[..., cols:2 * cols], mod[..., 3 * cols:4 * cols]     # [batch, 1, cols]
+    inv = torch.rand(batch, generator=g, device="cuda") + 0.5
+    same(lambda a, b: kernels.residual_norm(a, b, gam, None, gam), *new)
+    same(lambda a, b: kernels.residual_norm_backward(a, b, b, a, inv, inv, gam, a, gam), *new)
+    same(lambda a, b: (kernels.silu_mul(a, b),), *new)
+    same(lambda a, b: kernels.silu_mul_backward(b, a, b), *new)
+    same(lambda a: (kernels.checkpoint8_restore(kernels.checkpoint8(a)),), new[0])
+    same(lambda a, b: kernels.silu_mul_backward(b, kernels.checkpoint8(a), kernels.checkpoint8(b)), *new)
+    same(lambda a: kernels.rmsnorm_checkpoint8(a, gam)[:2], new[0])
+    same(lambda a, b: kernels.rmsnorm_backward(b, kernels.checkpoint8(a), inv, gam), *new)
+    same(lambda a: kernels.rmsnorm(a, gam), new[0])
+    same(lambda a, b: kernels.rmsnorm_backward(b, a, inv, gam), *new)
+    same(lambda a: (kernels.softmax(a), kernels.log_softmax(a)), new[0])
+    same(lambda a, b: (kernels.softmax_backward(a, b), kernels.log_softmax_backward(a, b)), *new)

@@ -35,6 +35,22 @@ from ._lib import Q8_FORMATS as _Q8_FORMATS, Q8_GROUP, check, dtype_code, lib, s
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
+def _row_stride(x: torch.Tensor) -> Optional[int]:
+    """The one stride onto which x's leading dims collapse, that of the innermost with more than one
+    index (a row's length with none); None if they do not.  A dim of one index has no say: whatever
+    stride it carries is never taken."""
+    step, rows = None, 1
+    for n, st in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+        if n == 1:
+            continue
+        if step is None:
+            step = st
+        elif st != step * rows:
+            return None
+        rows *= n
+    return x.shape[-1] if step is None else step
+
+
 def _rows_view(x: torch.Tensor, what: str):
     """(rows, cols, row_stride) of x seen as a stack of last-dim rows, the reference's 2-D
     view (rows = product of leading dims, row stride = strides[-2])."""
@@ -48,21 +64,9 @@ def _rows_view(x: torch.Tensor, what: str):
     rows = x.numel() // cols if cols else 0
     if cols and x.is_contiguous():
         return x, rows, cols, cols
-    if x.dim() >= 2:
-        lead_ok = x.stride(-1) == 1 or cols <= 1
-        # leading dims must collapse onto one row stride
-        expect = x.stride(-2)
-        for d in range(x.dim() - 3, -1, -1):
-            expect *= x.shape[d + 1]
-            if x.shape[d] != 1 and x.stride(d) != expect:
-                lead_ok = False
-        if not lead_ok:
-            x = _ops.contiguous(x)
-        row_stride = x.stride(-2) if x.shape[-2] != 1 else max(cols, 1)
-    else:
-        if x.stride(-1) != 1 and cols > 1:
-            x = _ops.contiguous(x)
-        row_stride = cols
+    row_stride = _row_stride(x)
+    if row_stride is None or (x.stride(-1) != 1 and cols > 1):
+        x, row_stride = _ops.contiguous(x), cols
     return x, rows, cols, row_stride
 
 
