@@ -221,3 +221,41 @@ def test_rows_of_a_view(monkeypatch, x):
     view, rows, cols, stride = kernels._rows_view(x.as_subclass(OnCard), "rows")
     got = view.as_subclass(torch.Tensor).as_strided((rows, cols), (stride, 1))
     assert torch.equal(got, x.reshape(-1, x.shape[-1]))
+
+
+class FakeLib:
+    """Stands in for the library: takes note of the calls and launches nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append(name) or 0
+
+
+@pytest.fixture
+def host_only(monkeypatch):
+    from vibetensor_b200 import kernels
+    fake = FakeLib()
+    monkeypatch.setattr(kernels, "lib", lambda: fake)
+    monkeypatch.setattr(kernels, "stream_ptr", lambda t=None: 0)
+    return fake
+
+
+def test_rotary_output_replaces_its_own_operand_only(host_only):
+    """An output may be the operand in its place.  Queries that are also the keys are read by the other
+    half of the launch: an output there would be turned while it is still read."""
+    from vibetensor_b200 import kernels
+    q, other = (torch.zeros(2, 5, 3, 64).as_subclass(OnCard) for _ in range(2))
+    pos, f = torch.zeros(2, 5, dtype=torch.int64), torch.ones(32)
+    for call in (kernels.rotary, kernels.rotary_backward):
+        for out in ((q, other), (other, q)):
+            with pytest.raises(ValueError, match="overlaps an input"):
+                call(q, q, pos, f, out=out)
+        with pytest.raises(ValueError, match="overlaps an input"):
+            call(q, other, pos, f, out=(other, q))     # each in the other's place
+    assert not host_only.calls
+    kernels.rotary(q, other, pos, f, out=(q, other))
+    kernels.rotary(q, q, pos, f)
+    kernels.rotary(q, None, pos, f, out=(q, None))
+    assert host_only.calls == ["vbt_b200_rotary"] * 3

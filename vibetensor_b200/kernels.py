@@ -676,9 +676,10 @@ def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what
                 raise ValueError(f"{what}: {name} must have a last stride of 1")
             if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
                 raise ValueError(f"{what}: {name} has values that share memory")
-            for t in (q, k, positions, inv_freq):
-                same = t is x and o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
-                if t is not None and not same and _overlap(o, t):
+            # it may replace the operand of its own place; the other one, the same tensor or not, is read meanwhile
+            replaces = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+            for t in (None if replaces else x, k if name == "out[0]" else q, positions, inv_freq):
+                if t is not None and _overlap(o, t):
                     raise ValueError(f"{what}: {name} overlaps an input that it does not replace")
         if out[1] is not None and _overlap(*out):
             raise ValueError(f"{what}: the two outputs overlap")
