@@ -259,3 +259,21 @@ def test_rotary_output_replaces_its_own_operand_only(host_only):
     kernels.rotary(q, q, pos, f)
     kernels.rotary(q, None, pos, f, out=(q, None))
     assert host_only.calls == ["vbt_b200_rotary"] * 3
+
+
+def test_rotary_output_values_are_apart(host_only):
+    """Outputs whose own values share memory are refused, whichever way they come to."""
+    from vibetensor_b200 import kernels
+    q = torch.zeros(2, 5, 3, 64).as_subclass(OnCard)
+    pos, f = torch.zeros(2, 5, dtype=torch.int64), torch.ones(32)
+    base = torch.zeros(4000)
+    for strides in ((0, 192, 64, 1), (960, 0, 64, 1), (960, 192, 0, 1), (960, 192, 63, 1), (960, 128, 64, 1), (64, 192, 64, 1),
+                    (191, 192, 960, 1)):
+        with pytest.raises(ValueError, match="share memory"):
+            kernels.rotary(q, None, pos, f, out=(base.as_strided(q.shape, strides).as_subclass(OnCard), None))
+    assert not host_only.calls
+    for strides in ((960, 192, 64, 1), (192, 384, 64, 1), (64, 512, 128, 1), (1500, 240, 80, 1)):
+        kernels.rotary(q, None, pos, f, out=(base.as_strided(q.shape, strides).as_subclass(OnCard), None))
+    one = q[:1, :1]
+    kernels.rotary(one, None, pos[:1, :1], f, out=(base.as_strided(one.shape, (0, 0, 64, 1)).as_subclass(OnCard), None))
+    assert len(host_only.calls) == 5

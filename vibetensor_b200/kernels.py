@@ -590,6 +590,17 @@ _I64x15 = ctypes.c_int64 * 15
 _SECTIONS = [ctypes.c_int64 * n for n in range(5)]
 
 
+def _values_apart(t: torch.Tensor) -> bool:
+    """Whether each value of t has memory of its own: every stride steps over all that the smaller
+    strides reach."""
+    reach = 0
+    for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if st <= reach:
+            return False
+        reach += (n - 1) * st
+    return True
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the views may share a value: their heads lie between one another in one memory, as
     the parts of a fused projection do without sharing any."""
@@ -674,7 +685,7 @@ def _rotary(q, k, positions, inv_freq, sections, interleaved, inverse, out, what
             _like(what, name, o, x)
             if o.stride(-1) != 1 and dim > 1:
                 raise ValueError(f"{what}: {name} must have a last stride of 1")
-            if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+            if not _values_apart(o):
                 raise ValueError(f"{what}: {name} has values that share memory")
             # it may replace the operand of its own place; the other one, the same tensor or not, is read meanwhile
             replaces = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
