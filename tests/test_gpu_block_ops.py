@@ -1020,3 +1020,41 @@ def test_parts_of_a_projection_with_one_token_or_row_per_sample(kernels, dtype, 
     same(lambda a, b: kernels.rmsnorm_backward(b, a, inv, gam), *new)
     same(lambda a: (kernels.softmax(a), kernels.log_softmax(a)), new[0])
     same(lambda a, b: (kernels.softmax_backward(a, b), kernels.log_softmax_backward(a, b)), *new)
+
+
+# ---------------------------------------------------------------------------- rows of any magnitude
+def row_steps(cols):
+    """Roundings on the longest path of a gradient of one row, K of ``close``: a thread adds up at most
+    16 values (one of every 512 in the kernels for rows of any length), a warp has 5 levels, a row at
+    most one warp per 256 values and no more than 128; the products around the sums are at most 14."""
+    return max(16, -(-cols // 512)) + 5 + min(128, -(-cols // 256)) + 14
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [64, 333, 512, 1365, 4096, 16400, 70001])
+def test_gradients_of_rows_of_any_magnitude(kernels, dtype, cols):
+    """A norm's gradient is that of its row's direction over the row's size: it keeps its relative
+    accuracy for rows as large as the forward pass takes and, with a small eps, as small."""
+    g = gen(cols + 2)
+    shape, k = (2, 3, cols), row_steps(cols) + 6    # six rows for a column sum
+    gp, gn = 1 + 0.1 * randn(g, (cols,)), 1 + 0.1 * randn(g, (cols,))
+    for rms_y, rms_r, top in ((1e17, 1.0, 1.0), (1.0, 1e17, 1.0), (3e16, 1e17, 1e-3), (1e15, 3e13, 1e-6), (1e-15, 1e-12, 1.0),
+                              (1e-17, 1e-17, 10.0), (1e-16, 1e16, 1.0)):
+        y, r = randn(g, shape, dtype, rms_y), randn(g, shape, dtype, rms_r)
+        # what arrives at r and at n moves the stream by about the same
+        dr, dn = randn(g, shape, dtype, top / rms_r), randn(g, shape, dtype, top)
+        i1 = y.double().pow(2).mean(-1).rsqrt().float().reshape(-1)
+        i2 = r.double().pow(2).mean(-1).rsqrt().float().reshape(-1)
+        for kind in ("none", "sample", "full"):
+            gate = gate_for(g, kind, shape, dtype)
+            got = dict(zip(("dx", "dy", "dgp", "dgate", "dgn"), kernels.residual_norm_backward(dr, dn, y, r, i1, i2, gp, gate, gn)))
+            for name, (t, mass) in join_bwd_ref(dr, dn, y, r, i1, i2, gp, gate, gn, 1.0, 1.0).items():
+                close(f"residual_norm_backward {name}, any magnitude", got[name], t, mass, k)
+    z, d = torch.zeros(shape, dtype=dtype, device="cuda"), randn(g, shape, dtype, 1e-6)
+    i = torch.full((6,), 1e15, device="cuda")      # zero rows and an eps of 1e-30
+    dx, dy, dgp, _, dgn = kernels.residual_norm_backward(None, d, z, z, i, i, gp, None, gn)
+    want = d.double() * gn.double() * 1e15
+    close("residual_norm_backward dx, zero rows", dx, want, want.abs(), k)
+    want = want * gp.double() * 1e15
+    close("residual_norm_backward dy, zero rows", dy, want, want.abs(), k)
+    assert (dgp == 0).all() and (dgn == 0).all()

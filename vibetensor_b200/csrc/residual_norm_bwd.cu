@@ -6,8 +6,11 @@
 //   dy  = i1 * dv * g1 - y * i1^3 * mean(dv * g1 * y)       dg1 = sum_rows dv * y * i1
 //
 // The second mean needs G, which needs the first.  It splits into sums that do not:
-//   sum(dv g1 y) = sum(w y (dr + i2 dn g2)) - c sum(w y r),  w = b gate g1, c = i2^3 mean(dn g2 r),
+//   sum(dv g1 y) = sum(w y (dr + i2 dn g2)) - c i2 sum(w y r),  w = b gate g1, c = i2^2 mean(dn g2 r),
 // so a row costs one reduction of three sums.
+// A product of several i leaves the normal numbers for rows far from one (i^3 does for an rms above 5e12
+// or below 2e-13).  Such rows, told by their i, are brought near one in place by i's power of two, which
+// rounds nothing: r i = (r 2^k) (i 2^-k).  A factor per value instead, i (r i), took 4 to 8 % longer.
 //
 // Bound by memory and, close behind, by instructions: four rows read, two written, 14 fp32 operations
 // and six conversions per value.  [32768,4096] bf16 with a gate row per 4096 rows takes 295 us = 5.5
@@ -65,6 +68,13 @@ struct JoinBwdParams {
 // Single values need more registers around them.
 constexpr int kVecElts = 16, kSingleElts = 8;
 constexpr int kBwdMaxThreads = 512;   // of a block that shares a row
+
+// A row is far from one if its i is.  16-bit floats of five exponent bits never are.
+template <class T> __device__ __forceinline__ bool far_row(float i) {
+  if constexpr (std::is_same_v<T, __half>) return false;
+  return (i > 0x1p25f && i < __int_as_float(0x7f800000)) || (i < 0x1p-25f && i >= 0x1p-126f);
+}
+__device__ __forceinline__ float power_of_two(float i) { return __int_as_float(__float_as_int(i) & 0x7f800000); }
 
 template <class T, int V, int TPR, int MODE, int STAGES>
 __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
@@ -187,7 +197,15 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     copy_wait<STAGES - 1>();
     A::sync();
     const bool live = RW == 1 || rl < at.left;
-    const float i1 = i1_next[0], i2 = i2_next[0];
+    const float i2 = i2_next[0];
+    float i1 = i1_next[0], ir = i2;  // of the rows as they lie in shared memory
+    const bool far_y = far_row<T>(i1);
+    if (far_y || far_row<T>(i2)) {
+      if (live && far_y) A::scale(buf(stage, 3), A::shift(p.y, p.y_stride, row), y_left, power_of_two(i1));
+      if (live && far_row<T>(i2)) A::scale(buf(stage, 2), A::shift(p.r, p.r_stride, row), pre_left, power_of_two(i2));
+      if (far_y) i1 /= power_of_two(i1);
+      if (far_row<T>(i2)) ir /= power_of_two(i2);
+    }
     float s[3] = {0.f, 0.f, 0.f};
     float up[E];  // dr + i2 dn g2, kept for the second pass
     if (live) {
@@ -214,13 +232,13 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
           s[0] = fmaf(dnr, g2[e], s[0]);
           s[1] = fmaf(wy, up[i], s[1]);
           s[2] = fmaf(wy, r[e], s[2]);
-          sum2[i] = fmaf(dnr, i2, sum2[i]);
+          sum2[i] = fmaf(dnr, ir, sum2[i]);
         }
       }
     }
     sum_row<TPR, 3>(s, red, phase, p.ranks);
-    const float c2 = i2 * i2 * i2 * s[0] * inv_cols;
-    const float c1 = p.post ? i1 * i1 * i1 * (s[1] - c2 * s[2]) * inv_cols : 0.f;
+    const float c2 = (i2 * inv_cols) * ir * (ir * s[0]);
+    const float c1 = p.post ? (i1 * inv_cols) * i1 * (i1 * (s[1] - c2 * s[2])) : 0.f;
     if (live) {
       const int64_t o = static_cast<int64_t>(row) * p.cols + j0;
 #pragma unroll
@@ -252,6 +270,8 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
           if (p.dgate) A::write(static_cast<T*>(p.dgate) + o, c, left, og);
         }
       }
+      // dy = i (G w - ..) came out with i 2^-k
+      if (far_y) A::scale_row(static_cast<T*>(p.dy) + o, left, power_of_two(p.inv1[row]));
     }
 #pragma unroll
     for (int q = 0; q + 1 < STAGES; ++q) {
@@ -361,12 +381,12 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_stream_kernel(const __g
         if (s2) s2[j] = fmaf(d * i2, rv, s2[j]);
       }
       fold(s);
-      const float c2 = i2 * i2 * i2 * s[0] * inv_cols;
-      const float c1 = p.post ? i1 * i1 * i1 * (s[1] - c2 * s[2]) * inv_cols : 0.f;
+      const float c2 = (i2 * inv_cols) * (i2 * s[0]);
+      const float c1 = p.post ? (i1 * inv_cols) * (i1 * (s[1] - c2 * (i2 * s[2]))) : 0.f;
       for (int64_t j = t; j < p.cols; j += THREADS) {
         const float d = dn ? to_f(dn[j]) : 0.f, rv = rr ? to_f(rr[j]) : 0.f, yv = y ? to_f(y[j]) : 0.f;
         const float g1 = p.post && p.g1 ? p.g1[j] : 1.f;
-        const float G = fmaf(-c2, rv, fmaf(i2 * d, p.pre && p.g2 ? p.g2[j] : 1.f, dr ? to_f(dr[j]) : 0.f));
+        const float G = fmaf(-c2, rv * i2, fmaf(i2 * d, p.pre && p.g2 ? p.g2[j] : 1.f, dr ? to_f(dr[j]) : 0.f));
         float bg = p.b * G;
         const float hat = yv * i1, full = bg * hat;
         const int64_t at = row * p.cols + j;
@@ -375,7 +395,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_stream_kernel(const __g
         if (gt) bg *= to_f(gt[j]);
         if (sg) sg[j] = fmaf(full, g1, sg[j]);
         if (s1) s1[j] = fmaf(bg, hat, s1[j]);
-        static_cast<T*>(p.dy)[at] = from_f<T>(p.post ? fmaf(i1 * bg, g1, -c1 * yv) : bg);
+        static_cast<T*>(p.dy)[at] = from_f<T>(p.post ? fmaf(i1 * bg, g1, -c1 * hat) : bg);
       }
     }
     if (sg && p.cuts == 1)

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -216,6 +217,24 @@ template <class T, int V, int TPR, int E> struct RowChunks {
       if (off(c, 0) < left) row[off(c, 0)] = from_f<T>(v[0]);
       if (off(c, 1) < left) row[off(c, 1)] = from_f<T>(v[1]);
     }
+  }
+  // multiplies the thread's own values of a staged row, or of the row it wrote, by a power of two
+  static __device__ __forceinline__ void scale(unsigned char* array, int shift, int left, float by) {
+    if constexpr (V > 1) {
+#pragma unroll 1
+      for (int c = 0; c < N; ++c) {
+        Vec<T, V>& v = *reinterpret_cast<Vec<T, V>*>(slot(array, c));
+        for (int e = 0; e < V; ++e) v.v[e] = from_f<T>(to_f(v.v[e]) * by);
+      }
+    } else {
+      scale_row(reinterpret_cast<T*>(region(array) + shift) + lane(), left, by);
+    }
+  }
+  static __device__ __forceinline__ void scale_row(T* row, int left, float by) {
+#pragma unroll 1
+    for (int c = 0; c < N; ++c)
+      for (int e = 0; e < C; ++e)
+        if (off(c, e) < left) row[off(c, e)] = from_f<T>(to_f(row[off(c, e)]) * by);
   }
   // per-column fp32 factors in the thread's own slots
   static __device__ __forceinline__ float* fslot(unsigned char* array, int c, int e) {
