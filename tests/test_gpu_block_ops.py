@@ -1058,3 +1058,28 @@ def test_gradients_of_rows_of_any_magnitude(kernels, dtype, cols):
     want = want * gp.double() * 1e15
     close("residual_norm_backward dy, zero rows", dy, want, want.abs(), k)
     assert (dgp == 0).all() and (dgn == 0).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [64, 333, 512, 1365, 4096, 16384, 20001])
+def test_rmsnorm_gradients_from_8_bits_of_rows_of_any_magnitude(kernels, fmt, dtype, cols):
+    g = gen(cols + 3)
+    gamma = 1 + 0.1 * randn(g, (cols,))
+    k = row_steps(cols) + -(-cols // 256) - min(128, -(-cols // 256)) + 7   # seven rows for a column sum
+    for rms, top in ((1e17, 1.0), (1e15, 1e-6), (3e13, 1.0), (1e-12, 1.0), (1e-17, 10.0)):
+        x, dy = randn(g, (7, cols), dtype, rms), randn(g, (7, cols), dtype, top)
+        inv = x.double().pow(2).mean(-1).rsqrt().float()
+        c = kernels.checkpoint8(x, fmt)
+        kept = c.q.double() * c.scale.double().repeat_interleave(128, 1)[:, :cols]
+        for gam in (gamma, None):
+            dx, dgamma = kernels.rmsnorm_backward(dy, c, inv, gam)
+            want = join_bwd_ref(None, dy, None, kept, None, inv, None, None, gam, 1.0, 1.0)
+            close("rmsnorm_backward of a checkpoint, dx, any magnitude", dx, *want["dx"], k)
+            if gam is not None:
+                close("rmsnorm_backward of a checkpoint, dgamma, any magnitude", dgamma, *want["dgn"], k)
+    z, d = kernels.checkpoint8(torch.zeros((7, cols), dtype=dtype, device="cuda"), fmt), randn(g, (7, cols), dtype, 1e-6)
+    dx, dgamma = kernels.rmsnorm_backward(d, z, torch.full((7,), 1e15, device="cuda"), gamma)   # an eps of 1e-30
+    want = d.double() * gamma.double() * 1e15
+    close("rmsnorm_backward of a checkpoint, zero rows", dx, want, want.abs(), k)
+    assert (dgamma == 0).all()

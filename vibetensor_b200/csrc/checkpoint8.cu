@@ -5,6 +5,8 @@
 //   rmsnorm_checkpoint8    RMSNorm and the 8-bit copy of its input from one read of x
 //   rmsnorm_backward8      the backward of RMSNorm with x' in the place of x:
 //                            n = x' r;  dx = r (dy g - n mean(dy g n));  dg = sum_rows dy n
+//                          no power of r is formed, which would leave the normal numbers where x does not:
+//                          n comes from the levels in one product, level (scale r)
 //   silu_mul               h = silu(gate) * up, with the 8-bit copies of both factors on request
 //   silu_mul_backward      dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, s = sigmoid(gate)
 //
@@ -505,7 +507,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
     A::sync();
     const int64_t row = begin + r0 + rl;
     const float inv = inv_next;
-    float x[E];
+    float x[E];  // normed
     Vec<T, C> dy[A::N];
     float s[1] = {0.f};
     if (live) {
@@ -516,7 +518,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
         A::read_factors(gbuf, c, g);
         Vec<uint8_t, C> lv;
         Q::read_raw(qbuf, Q::shift(p.q, p.cols, row), c, left, lv);
-        const float sc = sc_next[c / GC];
+        const float sc = sc_next[c / GC] * inv;
         if constexpr (V > 1) {
           q8_widen<F, V>(*reinterpret_cast<const typename Q8Raw<V>::type*>(&lv), sc, *reinterpret_cast<float(*)[V]>(&x[c * C]));
         } else {
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
         for (int e = 0; e < C; ++e) {
           const int i = c * C + e;
           const float t = to_f(dy[c].v[e]) * x[i];
-          sum[i] = fmaf(t, inv, sum[i]);
+          sum[i] += t;
           s[0] = fmaf(t, g[e], s[0]);
         }
       }
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
       fetch();
     }
     sum_row<TPR, 1>(s, &red[0][0], phase);
-    const float k = inv * inv * inv * s[0] * inv_cols;
+    const float k = inv * inv_cols * s[0];
     if (live) {
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
@@ -596,11 +598,11 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd8_stream_kernel(const __grid_c
       s[0] = fmaf(d, p.gamma ? p.gamma[j] : 1.f, s[0]);
     }
     fold(s);
-    const float c = inv * inv * (s[0] * inv / static_cast<float>(p.cols));
+    const float c = s[0] * inv / static_cast<float>(p.cols) * inv;  // dx = r (dy g - c x')
     for (int64_t j = t; j < p.cols; j += 256) {
       const float x = __fmul_rn(q8_level1<F>(q[j]), sc[j / kQ8Group]);
       static_cast<T*>(p.out)[row * p.cols + j] =
-          from_f<T>(fmaf(inv * to_f(dy[j]), p.gamma ? p.gamma[j] : 1.f, -c * x));
+          from_f<T>(inv * fmaf(to_f(dy[j]), p.gamma ? p.gamma[j] : 1.f, -c * x));
     }
   }
 }
