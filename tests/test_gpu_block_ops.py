@@ -1083,3 +1083,20 @@ def test_rmsnorm_gradients_from_8_bits_of_rows_of_any_magnitude(kernels, fmt, dt
     want = d.double() * gamma.double() * 1e15
     close("rmsnorm_backward of a checkpoint, zero rows", dx, want, want.abs(), k)
     assert (dgamma == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_silu_mul_keeps_what_exp_leaves(kernels, dtype):
+    """Down to where exp(-gate) overflows (gate = -88.72) the activation is a number of 1e-37, and a
+    large factor brings it back.  The sigmoid is below the normal numbers there: up to 2^-23 of it
+    (u = 2^-24 is 2 of these at most four times over), besides the usual eight roundings."""
+    a = torch.linspace(-88.7, -80, 301, device="cuda").to(dtype)
+    a = a[a >= -88.72]
+    b, d = torch.full_like(a, 1e30), torch.full_like(a, 3.0)
+    (hw, hm), (daw, dam), (dbw, dbm) = silu_ref(d, a, b)
+    # the exponent's argument is rounded: |gate| u, and exp by 2 u beside it
+    k = 88.72 * 2 + 16
+    close("silu_mul near exp's end", kernels.silu_mul(a, b), hw, hm, k)
+    da, db = kernels.silu_mul_backward(d, a, b)
+    close("silu_mul_backward gate near exp's end", da, daw, dam, k)
+    close("silu_mul_backward up near exp's end", db, dbw, dbm, k)

@@ -194,12 +194,19 @@ __global__ void __launch_bounds__(kCkThreads) restore8_kernel(const __grid_const
 // 1 / (1 + exp(-x)).  For 16-bit storage exp(-x) is 2^(-x log2 e) on the special-function unit: the
 // rounded product is off by at most |x| 2^-23 in the exponent, 2^-18 of the value where that is
 // smallest (|x| < 40; further out the sigmoid itself is below 2^-57 or rounds to one).
+// Below x = -87.3 the result is no normal number, and times x and another factor it may be one again in
+// fp32 and bf16.  fp32 takes the reciprocal that keeps it; bf16, where that costs 3 to 8 % ([16384,8192],
+// both passes), divides 1/16 + exp(-x) / 16 instead, the sixteenth taken off in the exponent.
 template <class T> __device__ __forceinline__ float sigmoid(float x) {
   float e, r;
-  if constexpr (sizeof(T) == 2) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
-  else e = expf(-x);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return r;
+  if constexpr (sizeof(T) == 4) {
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + expf(-x)));
+    return r;
+  }
+  constexpr bool WIDE = std::is_same_v<T, __nv_bfloat16>;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(x, -1.4426950408889634f, WIDE ? -4.f : 0.f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((WIDE ? 0.0625f : 1.f) + e));
+  return WIDE ? 0.0625f * r : r;
 }
 
 struct GluParams {
