@@ -1100,3 +1100,92 @@ def test_silu_mul_keeps_what_exp_leaves(kernels, dtype):
     da, db = kernels.silu_mul_backward(d, a, b)
     close("silu_mul_backward gate near exp's end", da, daw, dam, k)
     close("silu_mul_backward up near exp's end", db, dbw, dbm, k)
+
+
+# ---------------------------------------------------------------------- more rows than fit the card
+def column_steps(rows, cols, per):
+    """Roundings on the longest path of a sum over rows: a worker -- one of at least 148, or 16 clusters
+    where blocks share a row -- takes at most twice its share one after the other, the rows of one gate row
+    at most all, and a fold adds at most 64 partial rows per thread and 15 levels."""
+    return 2 * -(-rows // (16 if cols > 8192 else 148)) + per + 80
+
+
+# rows well above the workers of a launch and no multiple of them, gate rows in numbers around them, rows
+# per gate row that a warp's rows at once do not divide
+MANY = [((1819, 11), 64), ((6670, 3), 120), ((20011, 1), 130), ((1297, 7), 200), ((9007,), 333), ((811, 7), 512), ((8, 769), 1365),
+        ((3001,), 1000), ((43, 70), 4096), ((37, 41), 4095), ((29, 53), 5000), ((601, 2), 8192), ((3, 117), 12345), ((4, 90), 16384),
+        ((2, 151), 20001), ((2, 307), 66000)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lead,cols", MANY)
+def test_residual_norm_and_backward_of_many_rows(kernels, dtype, lead, cols):
+    g = gen(cols + 4)
+    shape, rows = lead + (cols,), int(np.prod(lead))
+    k = row_steps(cols)
+    x, y, dr, dn = (randn(g, shape, dtype) for _ in range(4))
+    gp, gn = 1 + 0.1 * randn(g, (cols,)), 1 + 0.1 * randn(g, (cols,))
+    for kind in ("none", "sample", "channel", "full"):
+        if kind == "sample" and len(lead) == 1 or kind == "full" and rows * cols > 1 << 24:
+            continue
+        gate = gate_for(g, kind, shape, dtype)
+        r, n, i1, i2 = kernels.residual_norm(x, y, gp, gate, gn, 1e-6, residual_scale=0.7, branch_scale=1.3)
+        w = join_ref(x, y, gp, gate, gn, 1e-6, True, True, 0.7, 1.3)
+        close("residual_norm r, many rows", r, w["r"], w["mass"], k)
+        close("residual_norm n, many rows", n, w["n"], w["n_mass"], k)
+        close("residual_norm inv_post, many rows", i1, w["i1"], w["i1"], k)
+        close("residual_norm inv_pre, many rows", i2, w["i2"], w["i2"] * (1 + 2 * w["rho"]), k)
+        del w, n
+        got = dict(zip(("dx", "dy", "dgp", "dgate", "dgn"), kernels.residual_norm_backward(
+            dr, dn, y, r, i1, i2, gp, gate, gn, residual_scale=0.7, branch_scale=1.3)))
+        want = join_bwd_ref(dr, dn, y, r, i1, i2, gp, gate, gn, 0.7, 1.3)
+        per = rows // lead[0] if kind == "sample" else 0
+        for name, (t, mass) in want.items():
+            over = 0 if name in ("dx", "dy") else column_steps(rows, cols, per)
+            close(f"residual_norm_backward {name}, many rows", got[name], t, mass, k + over)
+        del want, got
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(20011, 64), (20011, 130), (9007, 200), (9007, 333), (6151, 512), (6151, 1365), (3001, 4096),
+                                       (1507, 4095), (1507, 8192), (613, 16384), (1811, 20001)])
+def test_rmsnorm_kept_in_8_bits_of_many_rows(kernels, fmt, dtype, rows, cols):
+    g = gen(cols + 5)
+    k = row_steps(cols) + max(0, -(-cols // 256) - 128)
+    x, dy, gamma = acts(g, (rows, cols), dtype), randn(g, (rows, cols), dtype), 1 + 0.1 * randn(g, (cols,))
+    out, inv, c = kernels.rmsnorm_checkpoint8(x, gamma, 1e-6, fmt)
+    flat = kernels.checkpoint8(x, fmt)                 # compared bit for bit with the host's elsewhere
+    assert torch.equal(c.q.view(torch.int8), flat.q.view(torch.int8)) and torch.equal(c.scale, flat.scale)
+    some = torch.randint(0, rows, (64,), generator=g, device="cuda")
+    check_held(kernels.Checkpoint8(c.q[some], c.scale[some], fmt, dtype), x[some], fmt)
+    w = join_ref(x, x, None, None, gamma, 1e-6, False, True, 1.0, 0.0)
+    close("rmsnorm_checkpoint8 out, many rows", out, w["n"], w["n"].abs(), k)
+    close("rmsnorm_checkpoint8 inv_rms, many rows", inv, w["i2"], w["i2"], k)
+    del w
+    dx, dgamma = kernels.rmsnorm_backward(dy, c, inv, gamma)
+    kept = kernels.checkpoint8_restore(c, F32)
+    want = join_bwd_ref(None, dy, None, kept, None, inv, None, None, gamma, 1.0, 1.0)
+    close("rmsnorm_backward of a checkpoint, dx, many rows", dx, *want["dx"], k)
+    close("rmsnorm_backward of a checkpoint, dgamma, many rows", dgamma, *want["dgn"], k + column_steps(rows, cols, 0))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("b,t,hq,hk,dim,half,sections", [(7, 2857, 2, 1, 64, 32, (8, 12, 12)), (1, 20011, 1, 1, 32, 16, (16,)),
+                                                         (3, 4001, 3, 2, 80, 20, (5, 15)), (1201, 5, 4, 1, 40, 20, (7, 6, 7)),
+                                                         (2, 3989, 2, 2, 7, 3, (1, 2)), (64, 300, 1, 1, 8, 4, (1, 1, 1, 1)),
+                                                         (5, 1201, 8, 2, 128, 64, (16, 24, 24))])
+def test_rotary_several_tokens_per_block(kernels, dtype, interleaved, b, t, hq, hk, dim, half, sections):
+    """Enough tokens that a block takes several of them, across the samples' ends and with a ragged last
+    block; queries and keys are parts of one projection."""
+    g = gen(t)
+    freq = torch.exp(-torch.arange(half, device="cuda") * 0.13)
+    qkv = randn(g, (b, t, (hq + 2 * hk) * dim), dtype)
+    q, k = qkv[..., :hq * dim].unflatten(-1, (hq, dim)), qkv[..., hq * dim:(hq + hk) * dim].unflatten(-1, (hk, dim))
+    pos = torch.randint(-10, 2000000, (len(sections), b, t), generator=g, device="cuda")
+    for inverse, call in ((False, kernels.rotary), (True, kernels.rotary_backward)):
+        for x, o in zip((q, k), call(q, k, pos, freq, sections, interleaved)):
+            want, mass = rotary_ref(x, pos, freq, sections, interleaved, inverse)
+            close("rotary, several tokens per block", o, want, mass, 8)
+            assert torch.equal(o[..., 2 * half:], x[..., 2 * half:])
