@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const __grid_consta
 inline bool aligned(const void* q, int bytes) { return reinterpret_cast<uintptr_t>(q) % bytes == 0; }
 
 template <class T>
-int launch_write(KvWriteParams p, int format, cudaStream_t s) {
+int launch_write(KvWriteParams p, int format, cudaStream_t s, int sms) {
   constexpr int V = 16 / sizeof(T);
   bool vec = p.dim % V == 0 && p.dim / V <= 256;
   for (int i = 0; i < 2; ++i)
@@ -251,7 +251,7 @@ int launch_write(KvWriteParams p, int format, cudaStream_t s) {
   // about eight rounds of rows per thread, as long as the card is full of blocks
   const int64_t rows = 2 * int64_t{p.heads};
   int64_t tb = std::max<int64_t>(1, 8 * (kKvThreads / lanes) / rows);
-  tb = std::min<int64_t>(tb, std::max<int64_t>(1, p.tokens / 592));
+  tb = std::min<int64_t>(tb, std::max<int64_t>(1, p.tokens / (4 * sms)));
   p.tb = static_cast<int>(std::min<int64_t>(tb, kKvMaxTokens));
   p.scan = p.tokens <= 512;
   int launches = 1;
@@ -274,7 +274,7 @@ int launch_write(KvWriteParams p, int format, cudaStream_t s) {
 }
 
 template <class T>
-int launch_read(KvReadParams p, int format, cudaStream_t s) {
+int launch_read(KvReadParams p, int format, cudaStream_t s, int sms) {
   int v = 16 / static_cast<int>(sizeof(T));
   for (; v > 1; v /= 2) {
     if (v == 2) continue;
@@ -289,7 +289,7 @@ int launch_read(KvReadParams p, int format, cudaStream_t s) {
   p.div_head = FastDiv(static_cast<uint32_t>(p.dim / v));
   constexpr int U = 2;
   int64_t tb = std::max<int64_t>(1, 8 * U * kKvThreads / (2 * int64_t{p.chunks}));
-  tb = std::min<int64_t>(tb, std::max<int64_t>(1, p.rows / 592));
+  tb = std::min<int64_t>(tb, std::max<int64_t>(1, p.rows / (4 * sms)));
   p.tb = static_cast<int>(std::min<int64_t>(tb, kKvMaxTokens));
   const unsigned g = static_cast<unsigned>((p.rows + p.tb - 1) / p.tb);
 #define VB_KR(V) VB_KV_FORMAT(format, F, (kv_read_kernel<T, V, F, U><<<g, kKvThreads, 0, s>>>(p)))
@@ -342,10 +342,11 @@ vbt_b200_status vbt_b200_kv_cache_write(void* k_cache, float* k_scale, void* v_c
   p.heads = static_cast<int>(heads); p.dim = static_cast<int>(dim);
   p.div_heads = FastDiv(static_cast<uint32_t>(heads));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(scope.device());
   switch (dtype) {
-    case VBT_B200_F32: launch_write<float>(p, format, s); break;
-    case VBT_B200_F16: launch_write<__half>(p, format, s); break;
-    default: launch_write<__nv_bfloat16>(p, format, s); break;
+    case VBT_B200_F32: launch_write<float>(p, format, s, sms); break;
+    case VBT_B200_F16: launch_write<__half>(p, format, s, sms); break;
+    default: launch_write<__nv_bfloat16>(p, format, s, sms); break;
   }
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;
@@ -380,10 +381,11 @@ vbt_b200_status vbt_b200_kv_cache_read(void* k_out, void* v_out, int32_t dtype, 
   p.rows = rows; p.num_pages = num_slots / page_size; p.page_size = page_size;
   p.heads = static_cast<int>(heads); p.dim = static_cast<int>(dim); p.fill = fill;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count(scope.device());
   switch (dtype) {
-    case VBT_B200_F32: launch_read<float>(p, format, s); break;
-    case VBT_B200_F16: launch_read<__half>(p, format, s); break;
-    default: launch_read<__nv_bfloat16>(p, format, s); break;
+    case VBT_B200_F32: launch_read<float>(p, format, s, sms); break;
+    case VBT_B200_F16: launch_read<__half>(p, format, s, sms); break;
+    default: launch_read<__nv_bfloat16>(p, format, s, sms); break;
   }
   VB_LAUNCH_CHECK();
   return VBT_B200_OK;

@@ -158,7 +158,7 @@ bool side_fits(const RotSide& s, int values) {
 }
 
 template <class T>
-vbt_b200_status launch_rotary(RotParams p, int interleaved, cudaStream_t s) {
+vbt_b200_status launch_rotary(RotParams p, int interleaved, cudaStream_t s, int sms) {
   constexpr int most = 16 / sizeof(T);
   const bool has_k = p.heads > p.q_heads, has_q = p.q_heads > 0;
   auto fits = [&](int values) {
@@ -181,9 +181,9 @@ vbt_b200_status launch_rotary(RotParams p, int interleaved, cudaStream_t s) {
   const int64_t per_token = int64_t{p.heads} * p.items * (interleaved ? 1 : 2);
   p.tb = static_cast<int>(std::min<int64_t>({int64_t{kRotTokens}, 8 * kRotThreads / std::max<int64_t>(per_token, 1), int64_t{4096 / std::max(p.half, 1)}}));
   // but no fewer than four blocks per SM
-  p.tb = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tb, p.count / 592)));
+  p.tb = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tb, p.count / (4 * sms))));
   p.hb = p.heads;
-  if (p.count <= 296) {
+  if (p.count <= 2 * sms) {
     p.tb = 1;
     p.hb = std::max(1, std::min(p.heads, kRotThreads / std::max(p.items, 1)));
   }
@@ -263,9 +263,9 @@ vbt_b200_status vbt_b200_rotary(void* q_out, const void* q, int64_t q_heads, voi
   p.sign = inverse ? -1.f : 1.f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case VBT_B200_F32: return launch_rotary<float>(p, interleaved, s);
-    case VBT_B200_F16: return launch_rotary<__half>(p, interleaved, s);
-    default: return launch_rotary<__nv_bfloat16>(p, interleaved, s);
+    case VBT_B200_F32: return launch_rotary<float>(p, interleaved, s, sm_count(scope.device()));
+    case VBT_B200_F16: return launch_rotary<__half>(p, interleaved, s, sm_count(scope.device()));
+    default: return launch_rotary<__nv_bfloat16>(p, interleaved, s, sm_count(scope.device()));
   }
 }
 
