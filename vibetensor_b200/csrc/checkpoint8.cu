@@ -358,6 +358,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
   unsigned char* gbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (A::WARP_FACTORS + A::WARP_ARRAY);
   unsigned char* xbuf = gbuf + A::WARP_FACTORS;
   A::zero_rest(xbuf, true, left);
+  A::sync();
   const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
   const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   const int64_t begin = min(worker * p.chunk, p.rows);
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 4 : 1) rmsnorm8_kernel
       Vec<T, C> raw[GC];
 #pragma unroll
       for (int k = 0; k < GC; ++k) {
-        A::read_raw(xbuf, A::shift(p.x, p.stride, begin + r0 + rl), c0 + k, live ? left : 0, raw[k]);
+        A::read_raw(xbuf, A::shift(p.x, p.stride, begin + r0 + rl), c0 + k, raw[k]);
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           x[(c0 + k) * C + e] = to_f(raw[k].v[e]);
@@ -472,6 +473,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
   unsigned char* qbuf = dbuf + A::WARP_ARRAY;
   A::zero_rest(dbuf, true, left);
   Q::zero_rest(qbuf, true, left);
+  A::sync();
   const int seg = A::segment(), seg_left = static_cast<int>(p.cols) - seg;
   const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   const int64_t begin = min(worker * p.chunk, p.rows);
@@ -521,10 +523,10 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float g[C];
-        A::read_raw(dbuf, A::shift(p.dy, p.stride, row), c, left, dy[c]);
+        A::read_raw(dbuf, A::shift(p.dy, p.stride, row), c, dy[c]);
         A::read_factors(gbuf, c, g);
         Vec<uint8_t, C> lv;
-        Q::read_raw(qbuf, Q::shift(p.q, p.cols, row), c, left, lv);
+        Q::read_raw(qbuf, Q::shift(p.q, p.cols, row), c, lv);
         const float sc = sc_next[c / GC] * inv;
         if constexpr (V > 1) {
           q8_widen<F, V>(*reinterpret_cast<const typename Q8Raw<V>::type*>(&lv), sc, *reinterpret_cast<float(*)[V]>(&x[c * C]));
@@ -554,7 +556,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 1024, TPR ? 2 : 1) rmsnorm_bwd8_ke
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float d[C], g[C];
-        if constexpr (!kEarly) A::read_raw(dbuf, A::shift(p.dy, p.stride, row), c, left, dy[c]);
+        if constexpr (!kEarly) A::read_raw(dbuf, A::shift(p.dy, p.stride, row), c, dy[c]);
         A::read_factors(gbuf, c, g);
 #pragma unroll
         for (int e = 0; e < C; ++e) d[e] = fmaf(inv * to_f(dy[c].v[e]), g[e], -k * x[c * C + e]);

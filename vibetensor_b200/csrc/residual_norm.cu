@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
   auto buf = [&](int array) { return ring + array * A::WARP_ARRAY; };
 #pragma unroll
   for (int a = 0; a < ARRAYS; ++a) A::zero_rest(buf(a), true, left);
+  A::sync();
   const int seg = A::segment(warp0), seg_left = static_cast<int>(p.cols) - seg;
   const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
   const float* g2 = p.pre && p.g2 ? p.g2 + j0 : nullptr;
@@ -117,8 +118,9 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
       if (live) {
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
+          if (!A::reaches(c, seg_left)) break;
           float y[C];
-          A::read(buf(0), A::shift(p.y, p.y_stride, row), c, left, y);
+          A::read(buf(0), A::shift(p.y, p.y_stride, row), c, y);
 #pragma unroll
           for (int e = 0; e < C; ++e) s[0] = fmaf(y[e], y[e], s[0]);
         }
@@ -126,18 +128,19 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
       sum_row<TPR, 1>(s, red, phase, p.ranks);
       i1 = rsqrtf(s[0] * inv_cols + p.eps);
     }
-    float r[E];
+    float r[E] = {};
     s[0] = 0.f;
     if (live) {
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
+        if (!A::reaches(c, seg_left)) break;
         float x[C], y[C], w[C];
-        A::read(buf(0), A::shift(p.y, p.y_stride, row), c, left, y);
-        A::read(buf(1), A::shift(p.x, p.x_stride, row), c, left, x);
+        A::read(buf(0), A::shift(p.y, p.y_stride, row), c, y);
+        A::read(buf(1), A::shift(p.x, p.x_stride, row), c, x);
         A::read_factors(wbuf, c, w);
         if constexpr (GATE_ROW) {
           float gt[C];
-          A::read(buf(2), A::shift(p.gate, p.gate_stride, row), c, left, gt);
+          A::read(buf(2), A::shift(p.gate, p.gate_stride, row), c, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
     fetch();
     if (live) {
 #pragma unroll
-      for (int c = 0; c < A::N; ++c) A::write(r_out, c, left, *reinterpret_cast<const float(*)[C]>(&r[c * C]));
+      for (int c = 0; c < A::N && A::reaches(c, seg_left); ++c) A::write(r_out, c, left, *reinterpret_cast<const float(*)[C]>(&r[c * C]));
     }
     if (p.pre) {
       sum_row<TPR, 1>(s, red, phase, p.ranks);
@@ -161,6 +164,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
       if (live) {
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
+          if (!A::reaches(c, seg_left)) break;
           float g[C];
           A::read_factors(gbuf, c, g);
 #pragma unroll

@@ -64,9 +64,12 @@ struct JoinBwdParams {
 // registers between the two passes.  w = b * gate * g1 and g2 lie beside them.
 // The sum over a unit of G * y * i1 gives the gate's gradient (times b * g1) and the unit's part of
 // dgamma_post (times b * gate).  A gate row of its own per row (GATE_ROW) is a factor of the sum.
-// Values of a row per thread: two sums per column and the gradient at r stay in registers for each.
-// Single values need more registers around them.
-constexpr int kVecElts = 16, kSingleElts = 8;
+// Values of a row per thread: two sums per column and the gradient at r stay in registers for each.  Single
+// values: 16-bit ones fare better with sixteen ([16384,4095] bf16, a gate row per 2048: 251 us, 364 with eight),
+// 32-bit ones with eight where blocks are small ([6151,1365], a gate row for all: 69 us, 75 with sixteen; not
+// [8192,4095] without a gate, 194 and 179).
+constexpr int kVecElts = 16;
+template <class T> constexpr int kSingleElts = sizeof(T) == 2 ? 16 : 8;
 constexpr int kBwdMaxThreads = 512;   // of a block that shares a row
 
 // A row is far from one if its i is.  16-bit floats of five exponent bits never are.
@@ -78,7 +81,7 @@ __device__ __forceinline__ float power_of_two(float i) { return __int_as_float(_
 
 template <class T, int V, int TPR, int MODE, int STAGES>
 __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
-  constexpr int E = V > 1 ? kVecElts : kSingleElts;
+  constexpr int E = V > 1 ? kVecElts : kSingleElts<T>;
   using A = RowChunks<T, V, TPR, E>;
   constexpr int C = A::C;
   constexpr int RW = TPR ? 32 / TPR : 1;                 // rows a worker takes at once
@@ -103,6 +106,7 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       const bool present = a == 0 ? p.dr != nullptr : a == 3 ? p.y != nullptr : a == 4 || p.pre;
       A::zero_rest(buf(st, a), present, left);
     }
+  A::sync();
   const int seg = A::segment(warp0), seg_left = static_cast<int>(p.cols) - seg;
   const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
   const float* g2p = p.pre && p.g2 ? p.g2 + j0 : nullptr;
@@ -134,8 +138,6 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     return group * p.per + (u - group * p.cuts) * p.chunk;
   };
   const int row0 = static_cast<int>(first_row(u0)) + rl;  // rows are fewer than 2^31
-  // an absent array reads as zeros
-  const int dr_left = p.dr ? left : 0, pre_left = p.pre ? left : 0, y_left = p.y ? left : 0;
   Walk at;
   at.u = static_cast<int>(u0);
   at.left = 0;
@@ -201,8 +203,8 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     float i1 = i1_next[0], ir = i2;  // of the rows as they lie in shared memory
     const bool far_y = far_row<T>(i1);
     if (far_y || far_row<T>(i2)) {
-      if (live && far_y) A::scale(buf(stage, 3), A::shift(p.y, p.y_stride, row), y_left, power_of_two(i1));
-      if (live && far_row<T>(i2)) A::scale(buf(stage, 2), A::shift(p.r, p.r_stride, row), pre_left, power_of_two(i2));
+      if (live && far_y) A::scale(buf(stage, 3), A::shift(p.y, p.y_stride, row), left, power_of_two(i1));
+      if (live && far_row<T>(i2)) A::scale(buf(stage, 2), A::shift(p.r, p.r_stride, row), left, power_of_two(i2));
       if (far_y) i1 /= power_of_two(i1);
       if (far_row<T>(i2)) ir /= power_of_two(i2);
     }
@@ -212,15 +214,15 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float dr[C], dn[C], r[C], y[C], w[C], g2[C];
-        A::read(buf(stage, 0), A::shift(p.dr, p.dr_stride, row), c, dr_left, dr);
-        A::read(buf(stage, 1), A::shift(p.dn, p.dn_stride, row), c, pre_left, dn);
-        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, pre_left, r);
-        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y_left, y);
+        A::read(buf(stage, 0), A::shift(p.dr, p.dr_stride, row), c, dr);
+        A::read(buf(stage, 1), A::shift(p.dn, p.dn_stride, row), c, dn);
+        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, r);
+        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y);
         A::read_factors(wbuf, c, w);
         A::read_factors(gbuf, c, g2);
         if constexpr (MODE == GATE_ROW) {
           float gt[C];
-          A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, left, gt);
+          A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }
@@ -244,10 +246,10 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float r[C], y[C], w[C], gt[C], ox[C], oy[C], og[C];
-        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, pre_left, r);
-        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y_left, y);
+        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, r);
+        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y);
         A::read_factors(wbuf, c, w);
-        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, left, gt);
+        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, gt);
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           const int i = c * C + e;
@@ -467,7 +469,7 @@ struct JoinShape {
 };
 inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) {
   JoinShape h{0, 0, 0, 0, 4, 1};
-  const int elts = vec ? kVecElts : kSingleElts;
+  const int elts = vec ? kVecElts : elt == 2 ? kSingleElts<__half> : kSingleElts<float>;
   const int64_t lanes = (cols + elts - 1) / elts;
   if (lanes > int64_t{kBwdMaxThreads} * kMaxRanks) return h;
   h.tpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 0;

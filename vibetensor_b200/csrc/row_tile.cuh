@@ -114,8 +114,9 @@ __device__ __forceinline__ void narrow2(__half* p, float2 v) { *reinterpret_cast
 // V = 1 (any alignment): the lanes of a segment copy the 16-byte granules that cover it, whole, and
 // read single values behind the segment's shift against a 16-byte boundary; sync() stands between the
 // wait and the reads, and between the reads and the next copy.  Nothing in front of the tensor's
-// first value or behind the row's last is read.  (Copies of single 4-byte values ran [6151,1365] fp32
-// at half the rate, and 2-byte ones cannot be asynchronous.)
+// first value or behind the row's last is read; every copy writes zeros behind its row up to where another
+// shift's may end, so that reads need no bounds.  (Copies of single 4-byte values ran [6151,1365] fp32 at half the rate, and
+// 2-byte ones cannot be asynchronous.)
 template <class T, int V, int TPR, int E> struct RowChunks {
   static constexpr int C = V > 1 ? V : 2;
   static constexpr int N = E / C;
@@ -135,6 +136,8 @@ template <class T, int V, int TPR, int E> struct RowChunks {
   static __device__ __forceinline__ int base(int warp0 = 0) { return segment(warp0) + lane() * V; }
   // offset of element e of chunk c from it
   static __device__ __forceinline__ constexpr int off(int c, int e) { return V > 1 ? c * STEP * V + e : (2 * c + e) * STEP; }
+  // whether a row with `len` values from the segment's first column on has any in chunk c of some lane (V = 1)
+  static __device__ __forceinline__ bool reaches(int c, int len) { return V > 1 || 2 * c * STEP < len; }
   static __device__ __forceinline__ unsigned char* region(unsigned char* array) {
     return array + (V > 1 ? 0 : static_cast<int>(threadIdx.x & 31) / STEP * REGION);
   }
@@ -170,42 +173,46 @@ template <class T, int V, int TPR, int E> struct RowChunks {
 #pragma unroll
       for (int i = 0; i < (GRANULES + STEP - 1) / STEP; ++i) {
         const int at = (lane() + i * STEP) * 16;
-        if (at >= bytes) break;
+        if (at >= min(len, STEP * E) * ELT + 16) break;  // where no shift's end lies
         if (i == 0 && at == 0 && from < floor) {
-          for (int e = shift; e < min(16, bytes); e += ELT)
-            *reinterpret_cast<T*>(to + e) = *reinterpret_cast<const T*>(from + e);
+          for (int e = shift; e < 16; e += ELT)
+            *reinterpret_cast<T*>(to + e) = e < bytes ? *reinterpret_cast<const T*>(from + e) : T{};
         } else {
+          // behind the row's end nothing is read, from an address that is the row's all the same
           const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(to + at));
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from + at), "r"(min(16, bytes - at)) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       ::"r"(d), "l"(from + min(at, (bytes - 1) & ~15)), "r"(max(0, min(16, bytes - at))) : "memory");
         }
       }
     }
   }
-  // V > 1: zeros where no copy ever lands: behind the row's end, or everywhere if the array is absent.
-  // V = 1 reads nothing there.
+  // zeros where no copy ever lands: behind the row's end (V > 1), or everywhere if the array is absent.
+  // sync() stands between this and the first copy.
   static __device__ __forceinline__ void zero_rest(unsigned char* array, bool present, int left) {
     if constexpr (V > 1) {
 #pragma unroll
       for (int c = 0; c < N; ++c)
         if (!present || off(c, 0) >= left) *reinterpret_cast<Vec<T, V>*>(slot(array, c)) = Vec<T, V>{};
+    } else {
+      for (int i = lane() * 16; i < REGION; i += STEP * 16) *reinterpret_cast<uint4*>(region(array) + i) = uint4{};
     }
   }
-  static __device__ __forceinline__ void read_raw(unsigned char* array, int shift, int c, int left, Vec<T, C>& v) {
+  static __device__ __forceinline__ void read_raw(unsigned char* array, int shift, int c, Vec<T, C>& v) {
     if constexpr (V > 1) {
       v = *reinterpret_cast<const Vec<T, V>*>(slot(array, c));
     } else {
       const T* row = reinterpret_cast<const T*>(region(array) + shift) + lane();
 #pragma unroll
-      for (int e = 0; e < 2; ++e) v.v[e] = off(c, e) < left ? row[off(c, e)] : T{};
+      for (int e = 0; e < 2; ++e) v.v[e] = row[off(c, e)];
     }
   }
-  // `left`: values of the row from the thread's first column on, 0 if the array is absent
-  static __device__ __forceinline__ void read(unsigned char* array, int shift, int c, int left, float (&v)[C]) {
+  static __device__ __forceinline__ void read(unsigned char* array, int shift, int c, float (&v)[C]) {
     Vec<T, C> raw;
-    read_raw(array, shift, c, left, raw);
+    read_raw(array, shift, c, raw);
 #pragma unroll
     for (int e = 0; e < C; ++e) v[e] = to_f(raw.v[e]);
   }
+  // `left`: values of the row from the thread's first column on
   static __device__ __forceinline__ void write(T* row, int c, int left, const float (&v)[C]) {
     if constexpr (V > 1) {
       if (off(c, 0) >= left) return;
