@@ -478,11 +478,10 @@ inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) 
   for (h.ranks = 1; h.ranks <= kMaxRanks; h.ranks *= 2) {
     const int64_t part = (lanes + h.ranks - 1) / h.ranks;
     h.threads = h.tpr ? 256 : static_cast<int>((part + 31) / 32 * 32);
-    // Of a shared row, two blocks of 256 threads per SM overlap one's reduction with the other's copies:
-    // [8192,16384] bf16 641 -> 548 us with four blocks per row, fp32 [4096,16384] 567 -> 500.  Not with a
-    // gate row per row (652 -> 765: two rows in flight of five arrays leave room for one block), nor
-    // where one block holds the row (8192 columns: 434 -> 532).
-    if (h.threads > (h.ranks > 1 && h.ranks < kMaxRanks && !gate_row ? 384 : kBwdMaxThreads)) continue;
+    // Few blocks of many threads: of [8192,16384] bf16 without a gate, two per row against four with 256 threads
+    // each, 427 us and 486; fp32 [4096,16384] 316 and 431.  With a gate row per 1024 rows, whose units end
+    // often, 605 and 527.
+    if (h.threads > kBwdMaxThreads) continue;
     // two rows ahead where they fit; the warp forms are built for that alone
     h.stages = 2;
     if (!h.tpr && smem(2) > kSmemPerBlock) h.stages = 1;

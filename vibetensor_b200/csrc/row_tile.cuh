@@ -332,11 +332,19 @@ __device__ __forceinline__ void sum_row(float (&s)[N], float4* red, int& phase, 
       if (lane < ranks) store_at_rank(row + cluster_rank() * warps + w, lane, mine);
       __syncwarp();
       cluster_sync();
-      t = row[0];
-#pragma unroll 1
-      for (int k = 1; k < warps * ranks; ++k) {
+      // a lane adds every 32nd warp's part and the lanes fold; all parts one after the other in every thread took
+      // the backward of [8192,16384] bf16 458 us, so 428
+      t = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = lane; k < warps * ranks; k += 32) {
         const float4 f = row[k];
         t.x += f.x; t.y += f.y; t.z += f.z; t.w += f.w;
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) {
+        t.x += __shfl_xor_sync(0xffffffffu, t.x, d);
+        if constexpr (N > 1) t.y += __shfl_xor_sync(0xffffffffu, t.y, d);
+        if constexpr (N > 2) t.z += __shfl_xor_sync(0xffffffffu, t.z, d);
+        if constexpr (N > 3) t.w += __shfl_xor_sync(0xffffffffu, t.w, d);
       }
     }
     s[0] = t.x;
