@@ -277,3 +277,15 @@ def test_rotary_output_values_are_apart(host_only):
     one = q[:1, :1]
     kernels.rotary(one, None, pos[:1, :1], f, out=(base.as_strided(one.shape, (0, 0, 64, 1)).as_subclass(OnCard), None))
     assert len(host_only.calls) == 5
+
+
+def test_scratch_of_as_many_rows_as_there_may_be(L):
+    need = ctypes.c_size_t()
+    f = L.vbt_b200_residual_norm_backward_workspace_bytes
+    most = (1 << 31) - 1
+    for per in (1, most):
+        for cols in (64, 4096, 4095, 16384, 70001):
+            assert f(most, cols, BF16, per, 0, ctypes.byref(need)) == 0
+            assert 8 * cols <= need.value < 1 << 40
+    refused(L, f(1 << 31, 64, BF16, 1 << 31, 0, ctypes.byref(need)), "too many rows")
+    refused(L, back(L, rows=1 << 31), "too many rows")

@@ -1189,3 +1189,24 @@ def test_rotary_several_tokens_per_block(kernels, dtype, interleaved, b, t, hq, 
             want, mass = rotary_ref(x, pos, freq, sections, interleaved, inverse)
             close("rotary, several tokens per block", o, want, mass, 8)
             assert torch.equal(o[..., 2 * half:], x[..., 2 * half:])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lead,cols", [((400, 9), 4096), ((100, 40), 4096), ((1200, 23), 1365), ((70, 90), 1365), ((9000, 50), 64),
+                                       ((40, 333), 200), ((97, 40), 16384), ((300, 7), 20001), ((2, 1), 4096), ((3, 2), 64),
+                                       ((700, 5), 33000), ((90, 8), 70001)])
+def test_gate_rows_that_are_cut(kernels, dtype, lead, cols):
+    """Gate rows fewer and more than the workers of a launch, of more and fewer rows than a worker takes:
+    whole ones, ones that two workers share and ones that many do."""
+    g = gen(lead[0])
+    shape, rows = lead + (cols,), lead[0] * lead[1]
+    if rows * cols > 1 << 26:
+        shape, rows = (lead[0] // 5,) + shape[1:], lead[0] // 5 * lead[1]
+    y, r, dr, dn = (randn(g, shape, dtype) for _ in range(4))
+    gp, gn, gate = 1 + 0.1 * randn(g, (cols,)), 1 + 0.1 * randn(g, (cols,)), gate_for(g, "sample", shape, dtype)
+    i1, i2 = (t.float().pow(2).mean(-1).add(1e-6).rsqrt().reshape(-1) for t in (y, r))
+    got = dict(zip(("dx", "dy", "dgp", "dgate", "dgn"), kernels.residual_norm_backward(dr, dn, y, r, i1, i2, gp, gate, gn)))
+    k = row_steps(cols)
+    for name, (t, mass) in join_bwd_ref(dr, dn, y, r, i1, i2, gp, gate, gn, 1.0, 1.0).items():
+        over = 0 if name in ("dx", "dy") else column_steps(rows, cols, shape[1])
+        close(f"residual_norm_backward {name}, gate rows cut", got[name], t, mass, k + over)

@@ -10,16 +10,19 @@
 // so a row costs one reduction of three sums.
 // A product of several i leaves the normal numbers for rows far from one (i^3 does for an rms above 5e12
 // or below 2e-13).  Such rows, told by their i, are brought near one in place by i's power of two, which
-// rounds nothing: r i = (r 2^k) (i 2^-k).  A factor per value instead, i (r i), took 4 to 8 % longer.
+// rounds nothing: r i = (r 2^k) (i 2^-k).  A factor per value instead, i (r i), took up to 8 % longer.
 //
 // Bound by memory and, close behind, by instructions: four rows read, two written, 14 fp32 operations
-// and six conversions per value.  [32768,4096] bf16 with a gate row per 4096 rows takes 295 us = 5.5
-// TB/s, 0.83 of the measured copy bandwidth (16 warps per SM at 128 registers, half of the issue slots
+// and six conversions per value.  [32768,4096] bf16 with a gate row per 4096 rows takes 300 us = 5.4
+// TB/s, 0.82 of the measured copy bandwidth (16 warps per SM at 128 registers, half of the issue slots
 // busy).  What it came through: rows in registers 678 us; staged by asynchronous copies 370; one base per
 // warp and compile-time offsets instead of an address per access (744 instructions per warp and row
-// against 964) 314; units of neighbouring rows rather than every n-th one 306 (379).  Arithmetic on
+// against 964) 314; runs of neighbouring rows rather than every n-th one 306 (379).  Arithmetic on
 // float pairs was slower here (335: moves to pair the registers), and so were one block per SM with
 // four rows in flight (759), eight values per thread (424), and one row in flight (333).
+// Rows shared by two blocks: [8192,16384] bf16 443 us for a floor of 245, 420 without a gate.  Rows that no
+// vector divides: [16384,4095] bf16 250 us for 123, 225 without a gate; their values are single 16-bit loads
+// from shared memory and single stores.
 #include <algorithm>
 
 #include "row_tile.cuh"
@@ -28,6 +31,24 @@ namespace vb {
 namespace {
 
 enum { GATE_NONE = 0, GATE_SHARED = 1, GATE_ROW = 2 };
+
+// How the rows (fewer than 2^31) are cut: units of `chunk` rows, `cuts` to a gate row of `per` rows (its last
+// one may be shorter), dealt out to the workers in runs of `least` units, one more to each of the first `more`.
+struct RowCut {
+  uint32_t chunk, cuts, per, units, workers, least, more;
+
+  __host__ __device__ uint32_t first_unit(uint32_t worker) const { return worker * least + min_of(worker, more); }
+  __host__ __device__ uint32_t worker_of(uint32_t unit) const {
+    const uint32_t head = more * (least + 1);
+    return unit < head ? unit / (least + 1) : more + (unit - head) / least;
+  }
+  __host__ __device__ uint32_t first_row(uint32_t unit) const {
+    if (chunk == 1 || cuts == 1) return unit * chunk;
+    const uint32_t group = unit / cuts;
+    return group * per + (unit - group * cuts) * chunk;
+  }
+  static __host__ __device__ uint32_t min_of(uint32_t a, uint32_t b) { return a < b ? a : b; }
+};
 
 struct JoinBwdParams {
   const void* dr;    // may be null
@@ -44,25 +65,24 @@ struct JoinBwdParams {
   void* dgate;       // storage dtype; null to skip
   float* ws_g1;      // [workers][cols] partial sums of dgamma_post, or null
   float* ws_g2;      // the same of dgamma_pre
-  float* ws_gate;    // [units][cols] when a gate row's rows are cut into several units; the stream
-                     // kernel sums whole ones in [gridDim.x][cols]
+  float* ws_gate;    // [workers + gate rows][cols] when gate rows' rows are cut: row worker + gate row is the
+                     // worker's part of it; the stream kernel sums whole ones in [gridDim.x][cols]
   int64_t rows, cols;
   int64_t dr_stride, dn_stride, y_stride, r_stride, gate_stride;
   int64_t per;       // rows of one gate row (GATE_SHARED), else all rows
-  int64_t chunk;     // rows of one unit
-  int64_t cuts;      // units per gate row
-  int64_t units;
-  float a, b;
+  RowCut cut;
+  float a, b, inv_cols;
+  int dense;         // the rows of dr, dn, r and y follow one another without gaps
   int post, pre;
   int ranks;         // blocks that share a row
 };
 
-// A worker (a warp when TPR lanes of it share a row, else the block) walks a range of neighbouring
-// units, each a run of rows that share one gate row.  Rows arrive in shared memory by asynchronous
+// A worker (a warp when TPR lanes of it share a row, else the block) walks one run of neighbouring
+// rows, gate row after gate row.  Rows arrive in shared memory by asynchronous
 // copies, `stages` rows ahead; a thread reads back only what it copied itself, once for the three
 // sums and once for the outputs, so a row needs no barrier but the one of its reduction, and no
 // registers between the two passes.  w = b * gate * g1 and g2 lie beside them.
-// The sum over a unit of G * y * i1 gives the gate's gradient (times b * g1) and the unit's part of
+// The sum over a gate row's rows of G * y * i1 gives the gate's gradient (times b * g1) and their part of
 // dgamma_post (times b * gate).  A gate row of its own per row (GATE_ROW) is a factor of the sum.
 // Values of a row per thread: two sums per column and the gradient at r stay in registers for each.  Single
 // values: 16-bit ones fare better with sixteen ([16384,4095] bf16, a gate row per 2048: 251 us, 364 with eight),
@@ -71,16 +91,23 @@ struct JoinBwdParams {
 constexpr int kVecElts = 16;
 template <class T> constexpr int kSingleElts = sizeof(T) == 2 ? 16 : 8;
 constexpr int kBwdMaxThreads = 512;   // of a block that shares a row
+// Two rows ahead of 32-bit vectors leave shared memory for 352 threads: they may have 184 registers each, and
+// spill with 128 ([16384,4096] fp32 304 us, 278 so).
+constexpr int bwd_max_threads(int elt, bool vec, int stages) { return elt == 4 && vec && stages == 2 ? 352 : kBwdMaxThreads; }
 
-// A row is far from one if its i is.  16-bit floats of five exponent bits never are.
+// A row is far from one if its i is: beyond 2^25 or below 2^-25, and a normal number.  16-bit floats of five
+// exponent bits never are.
 template <class T> __device__ __forceinline__ bool far_row(float i) {
   if constexpr (std::is_same_v<T, __half>) return false;
-  return (i > 0x1p25f && i < __int_as_float(0x7f800000)) || (i < 0x1p-25f && i >= 0x1p-126f);
+  const uint32_t e = __float_as_uint(i) >> 23;
+  return e - (127 - 25) > 50u && e - 1 < 254u;
 }
-__device__ __forceinline__ float power_of_two(float i) { return __int_as_float(__float_as_int(i) & 0x7f800000); }
+// its i as a power of two and a number between one and two
+__device__ __forceinline__ float power_of_two(float i) { return __uint_as_float(__float_as_uint(i) & 0x7f800000u); }
+__device__ __forceinline__ float near_one(float i) { return __uint_as_float((__float_as_uint(i) & 0x007fffffu) | 0x3f800000u); }
 
 template <class T, int V, int TPR, int MODE, int STAGES>
-__global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
+__global__ void __launch_bounds__(TPR ? 256 : bwd_max_threads(sizeof(T), V > 1, STAGES), TPR ? 2 : 1) residual_norm_bwd_kernel(const __grid_constant__ JoinBwdParams p) {
   constexpr int E = V > 1 ? kVecElts : kSingleElts<T>;
   using A = RowChunks<T, V, TPR, E>;
   constexpr int C = A::C;
@@ -92,7 +119,6 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
   if (ranks > 1) cluster_sync();  // the other blocks' shared memory is there
   const int rl = TPR ? static_cast<int>(threadIdx.x & 31) / A::STEP : 0;
   const int j0 = A::base(warp0), left = static_cast<int>(p.cols) - j0;
-  const float inv_cols = 1.f / static_cast<float>(p.cols);
   // a warp's part of the shared memory: w, g2, then STAGES times the arrays
   unsigned char* wbuf = smem + static_cast<size_t>(threadIdx.x >> 5) * (2 * A::WARP_FACTORS + STAGES * ARRAYS * A::WARP_ARRAY);
   float4* red = reinterpret_cast<float4*>(smem + static_cast<size_t>(blockDim.x >> 5) *
@@ -108,70 +134,86 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
     }
   A::sync();
   const int seg = A::segment(warp0), seg_left = static_cast<int>(p.cols) - seg;
-  const float* g1 = p.post && p.g1 ? p.g1 + j0 : nullptr;
-  const float* g2p = p.pre && p.g2 ? p.g2 + j0 : nullptr;
-  A::fill_factors(gbuf, left, [&](int o) { return g2p ? g2p[o] : 1.f; });
-  if constexpr (MODE != GATE_SHARED) A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f); });
+  // b g1 of a chunk's columns
+  auto factors = [&](int c, float (&v)[C]) {
+    const float* g1 = p.post ? p.g1 : nullptr;
+#pragma unroll
+    for (int e = 0; e < C; ++e) v[e] = p.b;
+    if (g1) {
+#pragma unroll
+      for (int e = 0; e < C; ++e)
+        if (A::off(c, e) < left) v[e] *= g1[j0 + A::off(c, e)];
+    }
+  };
+  A::fill_factors(gbuf, left, [&](int o) { return p.pre && p.g2 ? p.g2[j0 + o] : 1.f; });
+  if constexpr (MODE != GATE_SHARED) {
+#pragma unroll
+    for (int c = 0; c < A::N; ++c) {
+      float w[C];
+      factors(c, w);
+      A::write_factors(wbuf, c, w);
+    }
+  }
 
-  const int64_t worker = TPR ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x / ranks;
-  const int64_t workers = TPR ? static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) : gridDim.x / ranks;
-  // the worker's units [u, last) are one run of rows; a unit's rows are taken RW at a time
-  struct Walk {
-    int u;
-    int todo, left;  // rows of the worker, rows of the unit still to take
-    __device__ __forceinline__ void enter(const JoinBwdParams& q) {
-      const int cut = u % static_cast<int>(q.cuts);
-      left = static_cast<int>(min(q.chunk, q.per - cut * q.chunk));
-    }
-    // takes the next rows; returns how many
-    __device__ __forceinline__ int next(const JoinBwdParams& q) {
-      const int n = RW == 1 ? 1 : min(RW, left);
-      todo -= n;
-      left -= n;
-      if (left == 0 && todo > 0) { ++u; enter(q); }
-      return n;
+  const int worker = TPR ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x / ranks;
+  // the worker's rows; fewer than 2^31 in all
+  const int begin = static_cast<int>(p.cut.first_row(p.cut.first_unit(min(worker, static_cast<int>(p.cut.workers)))));
+  const int end = static_cast<int>(p.cut.first_row(p.cut.first_unit(min(worker + 1, static_cast<int>(p.cut.workers)))));
+  // Rows are taken RW at a time, up to the end of a gate row where it is shared.  `row` is the first of
+  // them, `lane_row` this lane's; a lane whose row lies behind `stop` has none.
+  // Rows are addressed from their number: a running pointer per array is 20 registers of the 128.  Dense
+  // 16-bit arrays share one offset per row: [32768,4096] without a gate 287 -> 281 us, with a row for all 301
+  // -> 291; not with a gate row per row, another array, which spills then (367 -> 386).
+  constexpr bool DENSE = sizeof(T) == 2 && MODE != GATE_ROW;
+  const int per = static_cast<int>(p.per);
+  int group = MODE == GATE_SHARED ? begin / per : 0;
+  auto group_end = [&](int g) { return MODE == GATE_SHARED && (g + 1) * int64_t{per} < end ? (g + 1) * per : end; };
+  int row = begin, stop = group_end(group);
+  int row_ahead = begin, group_ahead = group, stop_ahead = stop;  // RW > 1
+  auto next = [&](int& r, int& g, int& st) {
+    r += RW;
+    if constexpr (MODE == GATE_SHARED) {
+      if (r >= st) {
+        r = st;
+        st = group_end(++g);
+      }
     }
   };
-  const int64_t u0 = worker * p.units / workers, u1 = (worker + 1) * p.units / workers;
-  auto first_row = [&](int64_t u) {
-    const int64_t group = u / p.cuts;
-    return group * p.per + (u - group * p.cuts) * p.chunk;
-  };
-  const int row0 = static_cast<int>(first_row(u0)) + rl;  // rows are fewer than 2^31
-  Walk at;
-  at.u = static_cast<int>(u0);
-  at.left = 0;
-  at.todo = u0 < u1 ? static_cast<int>(first_row(u1) - first_row(u0)) : 0;
-  if (at.todo) at.enter(p);
-  Walk ahead = at;
-  // rows are addressed from their number: a running pointer per array is 20 registers of the 128
-  int row = row0, row_ahead = row0;
   auto at_row = [&](const void* base, int64_t stride, int r) { return static_cast<const T*>(base) + r * stride + seg; };
+  auto at = [&](const void* base, int64_t offset) { return static_cast<const T*>(base) + offset; };
   float i1_next[STAGES], i2_next[STAGES];
-  const int row_end = row0 + at.todo;
-  auto fetch = [&](int stage, float& i1, float& i2) {
+  auto fetch = [&](int stage, int steps, float& i1, float& i2) {  // `steps` ahead of `row`
     i1 = 1.f;
     i2 = 0.f;
-    if (RW == 1 ? row_ahead < row_end : ahead.todo > 0) {
-      if (RW == 1 || rl < ahead.left) {
-        if (p.dr) A::copy(buf(stage, 0), at_row(p.dr, p.dr_stride, row_ahead), seg_left, p.dr);
+    const int r = RW == 1 ? row + steps : row_ahead + rl;
+    if (r < (RW == 1 ? end : stop_ahead)) {
+      if (DENSE && p.dense) {
+        const int64_t o = r * p.cols + seg;
+        if (p.dr) A::copy(buf(stage, 0), at(p.dr, o), seg_left, p.dr);
         if (p.pre) {
-          A::copy(buf(stage, 1), at_row(p.dn, p.dn_stride, row_ahead), seg_left, p.dn);
-          A::copy(buf(stage, 2), at_row(p.r, p.r_stride, row_ahead), seg_left, p.r);
-          i2 = p.inv2[row_ahead];
+          A::copy(buf(stage, 1), at(p.dn, o), seg_left, p.dn);
+          A::copy(buf(stage, 2), at(p.r, o), seg_left, p.r);
+          i2 = p.inv2[r];
         }
-        if (p.y) A::copy(buf(stage, 3), at_row(p.y, p.y_stride, row_ahead), seg_left, p.y);
-        if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), at_row(p.gate, p.gate_stride, row_ahead), seg_left, p.gate);
-        if (p.post) i1 = p.inv1[row_ahead];
+        if (p.y) A::copy(buf(stage, 3), at(p.y, o), seg_left, p.y);
+        if (p.post) i1 = p.inv1[r];
+      } else {
+        if (p.dr) A::copy(buf(stage, 0), at_row(p.dr, p.dr_stride, r), seg_left, p.dr);
+        if (p.pre) {
+          A::copy(buf(stage, 1), at_row(p.dn, p.dn_stride, r), seg_left, p.dn);
+          A::copy(buf(stage, 2), at_row(p.r, p.r_stride, r), seg_left, p.r);
+          i2 = p.inv2[r];
+        }
+        if (p.y) A::copy(buf(stage, 3), at_row(p.y, p.y_stride, r), seg_left, p.y);
+        if constexpr (MODE == GATE_ROW) A::copy(buf(stage, 4), at_row(p.gate, p.gate_stride, r), seg_left, p.gate);
+        if (p.post) i1 = p.inv1[r];
       }
-      // the rows of a worker follow one another; several at once stop at a unit's end
-      if constexpr (RW == 1) ++row_ahead;
-      else row_ahead += ahead.next(p);
     }
+    if constexpr (RW > 1) next(row_ahead, group_ahead, stop_ahead);
     copy_commit();
   };
 #pragma unroll
-  for (int q = 0; q < STAGES; ++q) fetch(q, i1_next[q], i2_next[q]);
+  for (int q = 0; q < STAGES; ++q) fetch(q, q, i1_next[q], i2_next[q]);
 
   float sum1[E], sum2[E];
 #pragma unroll
@@ -185,28 +227,41 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
         for (int d = TPR; d < 32; d <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
     }
   };
-  // the gate row of unit u, from this thread's first column on
-  auto gate_of = [&](int u) { return static_cast<const T*>(p.gate) + u / static_cast<int>(p.cuts) * p.gate_stride + j0; };
-  bool first_unit = true, enter = true;
-  int phase = 0, stage = 0;
-  while (at.todo > 0) {
-    if constexpr (MODE == GATE_SHARED) {
-      if (enter) {
-        const T* gate = gate_of(at.u);
-        A::fill_factors(wbuf, left, [&](int o) { return p.b * (g1 ? g1[o] : 1.f) * to_f(gate[o]); });
-      }
+  // the gate row, from this thread's first column on
+  auto gate_of = [&](int g) { return static_cast<const T*>(p.gate) + g * p.gate_stride + j0; };
+  auto fill_gate = [&] {
+    const T* gate = gate_of(group);
+#pragma unroll
+    for (int c = 0; c < A::N; ++c) {
+      float w[C], gt[C];
+      A::load(gate, c, left, gt);
+      factors(c, w);
+#pragma unroll
+      for (int e = 0; e < C; ++e) w[e] *= gt[e];
+      A::write_factors(wbuf, c, w);
     }
+  };
+  if constexpr (MODE == GATE_SHARED) {
+    if (row < end) fill_gate();
+  }
+  int phase = 0, stage = 0;
+  while (row < end) {
     copy_wait<STAGES - 1>();
     A::sync();
-    const bool live = RW == 1 || rl < at.left;
+    const int lane_row = row + rl;
+    const bool live = RW == 1 || lane_row < stop;
     const float i2 = i2_next[0];
     float i1 = i1_next[0], ir = i2;  // of the rows as they lie in shared memory
-    const bool far_y = far_row<T>(i1);
-    if (far_y || far_row<T>(i2)) {
-      if (live && far_y) A::scale(buf(stage, 3), A::shift(p.y, p.y_stride, row), left, power_of_two(i1));
-      if (live && far_row<T>(i2)) A::scale(buf(stage, 2), A::shift(p.r, p.r_stride, row), left, power_of_two(i2));
-      if (far_y) i1 /= power_of_two(i1);
-      if (far_row<T>(i2)) ir /= power_of_two(i2);
+    const bool far = far_row<T>(i1) || (p.pre && far_row<T>(i2));
+    if (far) {
+      if (far_row<T>(i1)) {
+        if (live) A::scale(buf(stage, 3), A::shift(p.y, p.y_stride, lane_row), left, power_of_two(i1));
+        i1 = near_one(i1);
+      }
+      if (far_row<T>(i2)) {
+        if (live) A::scale(buf(stage, 2), A::shift(p.r, p.r_stride, lane_row), left, power_of_two(i2));
+        ir = near_one(i2);
+      }
     }
     float s[3] = {0.f, 0.f, 0.f};
     float up[E];  // dr + i2 dn g2, kept for the second pass
@@ -214,15 +269,15 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float dr[C], dn[C], r[C], y[C], w[C], g2[C];
-        A::read(buf(stage, 0), A::shift(p.dr, p.dr_stride, row), c, dr);
-        A::read(buf(stage, 1), A::shift(p.dn, p.dn_stride, row), c, dn);
-        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, r);
-        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y);
+        A::read(buf(stage, 0), A::shift(p.dr, p.dr_stride, lane_row), c, dr);
+        A::read(buf(stage, 1), A::shift(p.dn, p.dn_stride, lane_row), c, dn);
+        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, lane_row), c, r);
+        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, lane_row), c, y);
         A::read_factors(wbuf, c, w);
         A::read_factors(gbuf, c, g2);
         if constexpr (MODE == GATE_ROW) {
           float gt[C];
-          A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, gt);
+          A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, lane_row), c, gt);
 #pragma unroll
           for (int e = 0; e < C; ++e) w[e] *= gt[e];
         }
@@ -239,17 +294,19 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       }
     }
     sum_row<TPR, 3>(s, red, phase, p.ranks);
-    const float c2 = (i2 * inv_cols) * ir * (ir * s[0]);
-    const float c1 = p.post ? (i1 * inv_cols) * i1 * (i1 * (s[1] - c2 * s[2])) : 0.f;
+    // keeps the second reads of the row behind the sums: in front of them they cost registers that spill
+    if constexpr (TPR != 0) __syncwarp();
+    const float c2 = (i2 * p.inv_cols) * ir * (ir * s[0]);
+    const float c1 = p.post ? (i1 * p.inv_cols) * i1 * (i1 * (s[1] - c2 * s[2])) : 0.f;
     if (live) {
-      const int64_t o = static_cast<int64_t>(row) * p.cols + j0;
+      const int64_t o = static_cast<int64_t>(lane_row) * p.cols + j0;
 #pragma unroll
       for (int c = 0; c < A::N; ++c) {
         float r[C], y[C], w[C], gt[C], ox[C], oy[C], og[C];
-        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, row), c, r);
-        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, row), c, y);
+        A::read(buf(stage, 2), A::shift(p.r, p.r_stride, lane_row), c, r);
+        A::read(buf(stage, 3), A::shift(p.y, p.y_stride, lane_row), c, y);
         A::read_factors(wbuf, c, w);
-        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, row), c, gt);
+        if constexpr (MODE == GATE_ROW) A::read(buf(stage, 4), A::shift(p.gate, p.gate_stride, lane_row), c, gt);
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           const int i = c * C + e;
@@ -263,8 +320,12 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
           } else {
             sum1[i] = fmaf(Gi, y[e], sum1[i]);
           }
-          // without the norm (c1 = 0, i1 = 1) dy does not depend on y, not even on a NaN in it
-          oy[e] = p.post ? fmaf(Gi, w[e], -c1 * y[e]) : Gi * w[e];
+          oy[e] = Gi * w[e];
+        }
+        // without the norm (i1 = 1) dy does not depend on y, not even on a NaN in it
+        if (p.post) {
+#pragma unroll
+          for (int e = 0; e < C; ++e) oy[e] = fmaf(-c1, y[e], oy[e]);
         }
         A::write(static_cast<T*>(p.dx) + o, c, left, ox);
         A::write(static_cast<T*>(p.dy) + o, c, left, oy);
@@ -273,7 +334,8 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
         }
       }
       // dy = i (G w - ..) came out with i 2^-k
-      if (far_y) A::scale_row(static_cast<T*>(p.dy) + o, left, power_of_two(p.inv1[row]));
+      if (far && p.post && far_row<T>(p.inv1[lane_row]))
+        A::scale_row(static_cast<T*>(p.dy) + o, left, power_of_two(p.inv1[lane_row]));
     }
 #pragma unroll
     for (int q = 0; q + 1 < STAGES; ++q) {
@@ -281,66 +343,69 @@ __global__ void __launch_bounds__(TPR ? 256 : kBwdMaxThreads, TPR ? 2 : 1) resid
       i2_next[q] = i2_next[q + 1];
     }
     A::sync();
-    fetch(stage, i1_next[STAGES - 1], i2_next[STAGES - 1]);
+    fetch(stage, STAGES, i1_next[STAGES - 1], i2_next[STAGES - 1]);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
-    const int unit = at.u;
-    row += at.next(p);
-    enter = at.todo == 0 || at.u != unit;
+    const int done = group;
+    next(row, group, stop);
     if constexpr (MODE == GATE_SHARED) {
-      if (!enter) continue;
+      if (group == done && row < end) continue;
       over_rows(sum1);
-      const int64_t group = unit / static_cast<int>(p.cuts);
-      const T* gate = gate_of(unit);
+      const T* gate = gate_of(done);
+      // all of the gate row's rows, or a part for the fold
+      const bool whole = p.ws_gate == nullptr || (int64_t{done} * per >= begin && (done + 1) * int64_t{per} <= end);
+      const bool first = done == begin / per;
       if (rl == 0) {
 #pragma unroll
         for (int c = 0; c < A::N; ++c) {
-          float og[C];
+          float gt[C], og[C];
+          A::load(gate, c, left, gt);
+          factors(c, og);
+          float* sums = p.ws_g1 + int64_t{worker} * p.cols + j0;  // the worker's running part of dgamma_post
+          float* part = p.ws_gate + (worker + int64_t{done}) * p.cols + j0;
 #pragma unroll
           for (int e = 0; e < C; ++e) {
-            const int o = A::off(c, e);
-            const float P = p.b * sum1[c * C + e];
-            const float Pg = o < left && g1 ? P * g1[o] : P;
-            og[e] = Pg;
-            if (o >= left) continue;
-            if (p.ws_gate) p.ws_gate[unit * p.cols + j0 + o] = Pg;
-            if (p.ws_g1) {  // the worker's running part, in its own row
-              float* part = p.ws_g1 + worker * p.cols + j0 + o;
-              *part = (first_unit ? 0.f : *part) + P * to_f(gate[o]);
-            }
+            og[e] *= sum1[c * C + e];
+            gt[e] *= p.b * sum1[c * C + e];
           }
-          if (p.dgate && p.ws_gate == nullptr)
-            A::write(static_cast<T*>(p.dgate) + group * p.cols + j0, c, left, og);
+          if (p.ws_g1 && !first) {
+#pragma unroll
+            for (int e = 0; e < C; ++e)
+              if (A::off(c, e) < left) gt[e] += sums[A::off(c, e)];
+          }
+#pragma unroll
+          for (int e = 0; e < C; ++e) {
+            if (A::off(c, e) >= left) continue;
+            if (p.ws_g1) sums[A::off(c, e)] = gt[e];
+            if (!whole) part[A::off(c, e)] = og[e];
+          }
+          if (p.dgate && whole) A::write(static_cast<T*>(p.dgate) + int64_t{done} * p.cols + j0, c, left, og);
         }
       }
-      first_unit = false;
 #pragma unroll
       for (int i = 0; i < E; ++i) sum1[i] = 0.f;
+      if (row < end) fill_gate();
     }
   }
   copy_wait<0>();
   if (ranks > 1) cluster_sync();  // no block leaves while another may still write to its shared memory
   if constexpr (MODE != GATE_SHARED) over_rows(sum1);
   over_rows(sum2);
-  if (rl == 0) {
+  if (rl == 0 && worker < static_cast<int>(p.cut.workers)) {
 #pragma unroll
     for (int c = 0; c < A::N; ++c)
 #pragma unroll
       for (int e = 0; e < C; ++e) {
         if (A::off(c, e) >= left) continue;
-        const int64_t o = worker * p.cols + j0 + A::off(c, e);
-        if (p.ws_g1) {
-          if constexpr (MODE == GATE_SHARED) {
-            if (first_unit) p.ws_g1[o] = 0.f;  // a worker without rows
-          } else {
-            p.ws_g1[o] = p.b * sum1[c * C + e];
-          }
+        const int64_t o = int64_t{worker} * p.cols + j0 + A::off(c, e);
+        if constexpr (MODE != GATE_SHARED) {
+          if (p.ws_g1) p.ws_g1[o] = p.b * sum1[c * C + e];
         }
         if (p.ws_g2) p.ws_g2[o] = sum2[c * C + e];
       }
   }
 }
 
-// any length and alignment: a block per unit, scalar accesses, each row read twice (again from L2);
+// any length and alignment: a block walks its rows, scalar accesses, each row read twice (again from L2);
 // the column sums live in the block's own workspace rows (a column is always the same thread's)
 template <class T, int MODE>
 __global__ void __launch_bounds__(512) residual_norm_bwd_stream_kernel(const __grid_constant__ JoinBwdParams p) {
@@ -348,18 +413,18 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_stream_kernel(const __g
   __shared__ float red[2][3][THREADS / 32];
   RowFold<THREADS, 3, THREADS> fold{red};
   const int t = threadIdx.x;
-  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  const float inv_cols = p.inv_cols;
   float* s1 = p.ws_g1 ? p.ws_g1 + static_cast<int64_t>(blockIdx.x) * p.cols : nullptr;
   float* s2 = p.ws_g2 ? p.ws_g2 + static_cast<int64_t>(blockIdx.x) * p.cols : nullptr;
   for (int64_t j = t; j < p.cols; j += THREADS) {
     if (s1) s1[j] = 0.f;
     if (s2) s2[j] = 0.f;
   }
-  for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
-    const int64_t group = u / p.cuts;
-    const int64_t begin = group * p.per + (u - group * p.cuts) * p.chunk;
-    const int64_t end = min(begin + p.chunk, (group + 1) * p.per);
-    float* sg = MODE == GATE_SHARED && p.ws_gate ? p.ws_gate + (p.cuts > 1 ? u : blockIdx.x) * p.cols : nullptr;
+  const int64_t start = p.cut.first_row(p.cut.first_unit(blockIdx.x)), last = p.cut.first_row(p.cut.first_unit(blockIdx.x + 1));
+  for (int64_t begin = start, end; begin < last; begin = end) {
+    const int64_t group = begin / p.per;
+    end = min(last, (group + 1) * p.per);
+    float* sg = MODE == GATE_SHARED && p.ws_gate ? p.ws_gate + (p.cut.cuts > 1 ? blockIdx.x + group : blockIdx.x) * p.cols : nullptr;
     if (sg)
       for (int64_t j = t; j < p.cols; j += THREADS) sg[j] = 0.f;
     for (int64_t row = begin; row < end; ++row) {
@@ -400,19 +465,19 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_stream_kernel(const __g
         static_cast<T*>(p.dy)[at] = from_f<T>(p.post ? fmaf(i1 * bg, g1, -c1 * hat) : bg);
       }
     }
-    if (sg && p.cuts == 1)
+    if (sg && group * p.per >= start && (group + 1) * p.per <= last)
       for (int64_t j = t; j < p.cols; j += THREADS) static_cast<T*>(p.dgate)[group * p.cols + j] = from_f<T>(sg[j]);
   }
 }
 
 // Column sums of partial rows in a fixed order.  blockIdx.y says which: dgamma_post and dgamma_pre over the
-// workers' rows, the gradient of one gate row that serves all over its units.
+// workers' rows, the gradient of one gate row that serves all.
 struct JoinFoldParams {
   float* out[2];
   const float* ws[2];
   void* dgate;
   const float* ws_gate;
-  int64_t cols, parts, cuts;
+  int64_t cols, parts;
   int what[3];
 };
 template <class T>
@@ -420,40 +485,51 @@ __global__ void __launch_bounds__(kStripThreads) residual_norm_fold_kernel(const
   __shared__ float sm[kStripThreads / 32][8];
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x;
   const int what = p.what[blockIdx.y];
-  const float s = what < 2 ? strip_sum(p.ws[what], p.parts, p.cols, sm) : strip_sum(p.ws_gate, p.cuts, p.cols, sm);
+  const float s = strip_sum(what < 2 ? p.ws[what] : p.ws_gate, p.parts, p.cols, sm);
   if (threadIdx.x < 8 && c < p.cols) {
     if (what < 2) p.out[what][c] = s;
     else static_cast<T*>(p.dgate)[c] = from_f<T>(s);
   }
 }
-// Several gate rows, few units each: 32 columns per block, eight warps take every eighth unit.
-template <class T>
-__global__ void __launch_bounds__(256) residual_norm_gate_fold_kernel(T* dgate, const float* ws, int64_t cuts, int64_t cols,
-                                                                      int64_t gates) {
+// Several gate rows, workers' parts of the ones that are cut: WARPS warps take 32 columns of one.  There are as
+// many to look at as gate rows, or as workers that may begin in the middle of one if these are fewer.
+// Eight warps where the gate rows are few and their parts many, else one (8 gate rows of 4096 rows: 305 us with
+// eight, 316 with one; 1024 of 32 rows: 409 and 335).
+template <class T, int WARPS>
+__global__ void __launch_bounds__(256) residual_norm_gate_fold_kernel(T* dgate, const float* ws,
+                                                                      const __grid_constant__ RowCut cut, int64_t cols) {
   __shared__ float sm[8][32];
+  constexpr int AT_ONCE = 8 / WARPS;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  for (int64_t g = blockIdx.y; g < gates; g += gridDim.y) {
-    const float* src = ws + g * cuts * cols + c;
+  const uint32_t gates = cut.units / cut.cuts, n = RowCut::min_of(gates, cut.workers);
+  for (uint32_t i = blockIdx.y * AT_ONCE + w / WARPS; i < n; i += gridDim.y * AT_ONCE) {
+    const uint32_t g = gates <= cut.workers ? i : cut.first_unit(i) / cut.cuts;
+    const uint32_t w0 = cut.worker_of(g * cut.cuts), parts = cut.worker_of(g * cut.cuts + cut.cuts - 1) - w0 + 1;
+    // written by the one worker that has it; or for the next worker to look at, who begins in it second
+    if (parts == 1 || (gates > cut.workers && w0 + 1 != i)) continue;
+    const float* src = ws + static_cast<int64_t>(w0 + g) * cols + c;
     float acc = 0.f;
     if (c < cols) {
-      for (int64_t r = w; r < cuts; r += 8 * 8) {
+      for (uint32_t r = w % WARPS; r < parts; r += 8 * WARPS) {
         float v[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = r + 8 * q < cuts ? __ldcg(src + (r + 8 * q) * cols) : 0.f;
+        for (int q = 0; q < 8; ++q) v[q] = r + WARPS * q < parts ? __ldcg(src + static_cast<int64_t>(r + WARPS * q) * cols) : 0.f;
 #pragma unroll
         for (int q = 0; q < 8; ++q) acc += v[q];
       }
     }
-    sm[w][lane] = acc;
-    __syncthreads();
-    if (w == 0 && c < cols) {
-      float s = 0.f;
+    if constexpr (WARPS > 1) {
+      sm[w][lane] = acc;
+      __syncthreads();
+      if (w == 0) {
+        acc = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += sm[k][lane];
-      dgate[g * cols + c] = from_f<T>(s);
+        for (int k = 0; k < WARPS; ++k) acc += sm[k][lane];
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    if (w % WARPS == 0 && c < cols) dgate[static_cast<int64_t>(g) * cols + c] = from_f<T>(acc);
   }
 }
 
@@ -478,55 +554,46 @@ inline JoinShape join_bwd_shape(int64_t cols, int elt, bool gate_row, bool vec) 
   for (h.ranks = 1; h.ranks <= kMaxRanks; h.ranks *= 2) {
     const int64_t part = (lanes + h.ranks - 1) / h.ranks;
     h.threads = h.tpr ? 256 : static_cast<int>((part + 31) / 32 * 32);
-    // Few blocks of many threads: of [8192,16384] bf16 without a gate, two per row against four with 256 threads
-    // each, 427 us and 486; fp32 [4096,16384] 316 and 431.  With a gate row per 1024 rows, whose units end
-    // often, 605 and 527.
+    // Few blocks of many threads: of [8192,16384] bf16, two per row against four with 256 threads each, 427
+    // us and 486 without a gate, 468 and 519 with a row per 1024; fp32 [4096,16384] 316 and 431.
     if (h.threads > kBwdMaxThreads) continue;
     // two rows ahead where they fit; the warp forms are built for that alone
     h.stages = 2;
     if (!h.tpr && smem(2) > kSmemPerBlock) h.stages = 1;
     h.smem = smem(h.stages);
-    if (h.smem > kSmemPerBlock) continue;
+    if (h.smem > kSmemPerBlock || h.threads > bwd_max_threads(elt, vec, h.stages)) continue;
     // registers allow 512 threads per SM (128 each)
     h.per_sm = std::max(1, std::min(512 / h.threads, kSmemPerSm / (h.smem + 1024)));
     return h;
   }
   return JoinShape{0, 0, 0, 0, 4, 1};
 }
-// How the rows are cut: units of `chunk` rows, `cuts` of them per gate row, dealt out evenly to the
-// workers that fit the card.  At least as many units as workers, and up to eight times that where it
-// evens out what a worker gets (30 gate rows of 1000 rows of 4096 on 296 workers: 463 us with as many units
-// as workers, 335 with more); the end of a unit is counted as eight steps.
-struct JoinCut {
-  int64_t chunk, cuts, units, blocks, workers;
-};
-inline JoinCut join_cut(int64_t rows, int64_t per, const JoinShape& h, int sms) {
-  const int per_block = h.threads ? h.workers() : 1;
+// How the rows are cut: into units of as many rows as a worker takes at once, dealt out evenly in runs to the
+// workers that fit the card, which sum a gate row's part each; or into whole gate rows where that is
+// cheaper.  Units of more rows, each with a sum of its own, took [8192,16384] bf16 with a gate row per 1024
+// rows 592 us against 464, [16384,8192] with one per 2048 437 against 350.
+inline RowCut join_cut(int64_t rows, int64_t per, const JoinShape& h, int sms) {
   const int64_t groups = rows / per, most = h.most(sms);
   const int64_t at_once = h.tpr ? 32 / h.tpr : 1;
-  const int64_t least = (most + groups - 1) / groups, finest = (per + at_once - 1) / at_once;
-  JoinCut c{};
-  int64_t best = INT64_MAX;
-  for (int k = 1; k <= 8; ++k) {
-    const int64_t want = std::min(finest, least * k);
-    const int64_t steps = (finest + want - 1) / want;  // of a unit
-    const int64_t cuts = (finest + steps - 1) / steps, units = groups * cuts;
-    const int64_t cost = (units + most - 1) / most * (steps + 8);
-    if (cost < best) {
-      best = cost;
-      c.chunk = steps * at_once;
-      c.cuts = cuts;
-      c.units = units;
-    }
-  }
-  c.blocks = (std::min<int64_t>(c.units, most) + per_block - 1) / per_block;
-  c.workers = c.blocks * per_block;
+  const int64_t steps = (per + at_once - 1) / at_once;  // of a gate row
+  // in steps; the end of a gate row's run counts as eight, the fold of parts as one
+  const int64_t whole = (groups + most - 1) / most * (steps + 8);
+  const int64_t share = (groups * steps + most - 1) / most, even = share + 8 * (share / steps + 1) + 1;
+  const bool cut = steps > 1 && whole > even;
+  RowCut c{};
+  c.chunk = static_cast<uint32_t>(cut ? at_once : per);
+  c.cuts = static_cast<uint32_t>(cut ? steps : 1);
+  c.per = static_cast<uint32_t>(per);
+  c.units = static_cast<uint32_t>(groups * c.cuts);
+  c.workers = static_cast<uint32_t>(std::min<int64_t>(c.units, most));
+  c.least = c.units / c.workers;
+  c.more = c.units % c.workers;
   return c;
 }
-inline size_t join_bwd_floats(const JoinCut& c, const JoinShape& h) {
-  // dgamma_post, dgamma_pre, and the gate's: a row per unit where a gate row is cut, else one per block of
-  // the stream kernel
-  return static_cast<size_t>(2 * c.workers + (c.cuts > 1 ? c.units : h.threads ? 0 : c.blocks));
+inline size_t join_bwd_rows(const RowCut& c, const JoinShape& h) {
+  // dgamma_post, dgamma_pre, and the gate's: a row per worker and gate row where these are cut, else one per
+  // block of the stream kernel
+  return size_t{2} * c.workers + (c.cuts > 1 ? size_t{c.workers} + c.units / c.cuts : h.threads ? 0 : c.workers);
 }
 
 template <class T, int V, int TPR, int MODE, int STAGES>
@@ -544,12 +611,16 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
                    p.r_stride % VW == 0 && p.gate_stride % VW == 0 && a16(p.dr) && a16(p.dn) && a16(p.y) && a16(p.r) &&
                    a16(p.gate) && a16(p.dx) && a16(p.dy) && a16(p.dgate);
   const JoinShape h = join_bwd_shape(p.cols, sizeof(T), mode == GATE_ROW, vec);
-  const JoinCut cut = join_cut(p.rows, p.per, h, sm_count(device));
-  p.chunk = cut.chunk; p.cuts = cut.cuts; p.units = cut.units; p.ranks = h.ranks;
-  const unsigned g = static_cast<unsigned>(cut.blocks * h.ranks);
+  const RowCut cut = join_cut(p.rows, p.per, h, sm_count(device));
+  const int per_block = h.threads ? h.workers() : 1;
+  p.cut = cut;
+  p.dense = (!p.dr || p.dr_stride == p.cols) && (!p.dn || p.dn_stride == p.cols) && (!p.r || p.r_stride == p.cols) &&
+            (!p.y || p.y_stride == p.cols);
+  p.ranks = h.ranks; p.inv_cols = 1.f / static_cast<float>(p.cols);
+  const unsigned g = (cut.workers + per_block - 1) / per_block * h.ranks;
   float* at = ws;
-  if (dg1) { p.ws_g1 = at; at += cut.workers * p.cols; }
-  if (dg2) { p.ws_g2 = at; at += cut.workers * p.cols; }
+  if (dg1) { p.ws_g1 = at; at += int64_t{cut.workers} * p.cols; }
+  if (dg2) { p.ws_g2 = at; at += int64_t{cut.workers} * p.cols; }
   const bool split_gate = mode == GATE_SHARED && p.dgate != nullptr && cut.cuts > 1;
   // the stream kernel sums a gate row in memory even where it has all its rows
   if (split_gate || (mode == GATE_SHARED && p.dgate != nullptr && h.threads == 0)) p.ws_gate = at;
@@ -577,7 +648,7 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
   JoinFoldParams f{};
   f.out[0] = dg1; f.out[1] = dg2; f.ws[0] = p.ws_g1; f.ws[1] = p.ws_g2;
   f.dgate = p.dgate; f.ws_gate = p.ws_gate;
-  f.cols = p.cols; f.parts = cut.workers; f.cuts = cut.cuts;
+  f.cols = p.cols; f.parts = cut.workers;
   unsigned sums = 0;
   if (dg1) f.what[sums++] = 0;
   if (dg2) f.what[sums++] = 1;
@@ -588,8 +659,10 @@ vbt_b200_status launch_join_bwd(JoinBwdParams p, int mode, float* dg1, float* dg
     ++launches;
   }
   if (split_gate && gates > 1) {
-    const dim3 grid(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(std::min<int64_t>(gates, 65535)));
-    residual_norm_gate_fold_kernel<T><<<grid, 256, 0, s>>>(static_cast<T*>(p.dgate), p.ws_gate, cut.cuts, p.cols, gates);
+    const int64_t n = std::min<int64_t>(gates, cut.workers), at_once = n <= 64 ? 1 : 8;
+    const dim3 grid(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>((n + at_once - 1) / at_once));
+    auto fold = n <= 64 ? residual_norm_gate_fold_kernel<T, 8> : residual_norm_gate_fold_kernel<T, 1>;
+    fold<<<grid, 256, 0, s>>>(static_cast<T*>(p.dgate), p.ws_gate, cut, p.cols);
     VB_LAUNCH_CHECK();
     ++launches;
   }
@@ -610,6 +683,7 @@ vbt_b200_status vbt_b200_residual_norm_backward_workspace_bytes(int64_t rows, in
   const char* name = "residual_norm_backward";
   VB_ARG(bytes != nullptr, std::string(name) + ": null output");
   VB_ARG(rows >= 0 && cols >= 0, std::string(name) + ": negative size");
+  VB_ARG(rows < (int64_t{1} << 31), std::string(name) + ": too many rows");
   VB_ARG(is_float_dtype(dtype), std::string(name) + ": expected a floating dtype");
   VB_ARG(rows == 0 || (rows_per_gate > 0 && rows % rows_per_gate == 0),
          std::string(name) + ": rows_per_gate does not divide rows");
@@ -619,8 +693,8 @@ vbt_b200_status vbt_b200_residual_norm_backward_workspace_bytes(int64_t rows, in
   const int elt = itemsize(dtype);
   for (int form = 0; form < 4; ++form) {  // whichever the gate given and the pointers' alignment take
     const JoinShape h = join_bwd_shape(cols, elt, form & 1, form & 2);
-    const JoinCut c = join_cut(rows, rows_per_gate == 1 ? rows : rows_per_gate, h, sm_count(device));
-    *bytes = std::max(*bytes, join_bwd_floats(c, h) * static_cast<size_t>(cols) * 4);
+    const RowCut c = join_cut(rows, rows_per_gate == 1 ? rows : rows_per_gate, h, sm_count(device));
+    *bytes = std::max(*bytes, join_bwd_rows(c, h) * static_cast<size_t>(cols) * 4);
   }
   return VBT_B200_OK;
 }

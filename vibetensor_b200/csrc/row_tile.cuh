@@ -212,7 +212,18 @@ template <class T, int V, int TPR, int E> struct RowChunks {
 #pragma unroll
     for (int e = 0; e < C; ++e) v[e] = to_f(raw.v[e]);
   }
-  // `left`: values of the row from the thread's first column on
+  // chunk c of a row in global memory; `left`: values of the row from the thread's first column on
+  static __device__ __forceinline__ void load(const T* row, int c, int left, float (&v)[C]) {
+    if constexpr (V > 1) {
+      Vec<T, V> raw{};
+      if (off(c, 0) < left) raw = *reinterpret_cast<const Vec<T, V>*>(row + off(c, 0));
+#pragma unroll
+      for (int e = 0; e < C; ++e) v[e] = to_f(raw.v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < C; ++e) v[e] = off(c, e) < left ? to_f(row[off(c, e)]) : 0.f;
+    }
+  }
   static __device__ __forceinline__ void write(T* row, int c, int left, const float (&v)[C]) {
     if constexpr (V > 1) {
       if (off(c, 0) >= left) return;
@@ -253,6 +264,15 @@ template <class T, int V, int TPR, int E> struct RowChunks {
       const Vec<float, FW> f = *reinterpret_cast<const Vec<float, FW>*>(fslot(array, c, e));
 #pragma unroll
       for (int i = 0; i < FW; ++i) v[e + i] = f.v[i];
+    }
+  }
+  static __device__ __forceinline__ void write_factors(unsigned char* array, int c, const float (&v)[C]) {
+#pragma unroll
+    for (int e = 0; e < C; e += FW) {
+      Vec<float, FW> f;
+#pragma unroll
+      for (int i = 0; i < FW; ++i) f.v[i] = v[e + i];
+      *reinterpret_cast<Vec<float, FW>*>(fslot(array, c, e)) = f;
     }
   }
   // fills them: value(offset from the thread's first column), 0 behind the row's end
