@@ -128,7 +128,10 @@ __global__ void __launch_bounds__(TPR ? 256 : kFwdMaxThreads, TPR ? 4 : 1) resid
       sum_row<TPR, 1>(s, red, phase, p.ranks);
       i1 = rsqrtf(s[0] * inv_cols + p.eps);
     }
-    float r[E] = {};
+    float r[E];
+    if constexpr (V == 1)
+#pragma unroll
+      for (int i = 0; i < E; ++i) r[i] = 0.f;
     s[0] = 0.f;
     if (live) {
 #pragma unroll

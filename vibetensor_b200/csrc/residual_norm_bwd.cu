@@ -97,10 +97,9 @@ constexpr int bwd_max_threads(int elt, bool vec, int stages) { return elt == 4 &
 
 // A row is far from one if its i is: beyond 2^25 or below 2^-25, and a normal number.  16-bit floats of five
 // exponent bits never are.
+__device__ __forceinline__ bool beyond(float i) { return (__float_as_uint(i) >> 23) - (127 - 25) > 50u; }
 template <class T> __device__ __forceinline__ bool far_row(float i) {
-  if constexpr (std::is_same_v<T, __half>) return false;
-  const uint32_t e = __float_as_uint(i) >> 23;
-  return e - (127 - 25) > 50u && e - 1 < 254u;
+  return !std::is_same_v<T, __half> && beyond(i) && (__float_as_uint(i) >> 23) - 1 < 254u;
 }
 // its i as a power of two and a number between one and two
 __device__ __forceinline__ float power_of_two(float i) { return __uint_as_float(__float_as_uint(i) & 0x7f800000u); }
@@ -252,7 +251,7 @@ __global__ void __launch_bounds__(TPR ? 256 : bwd_max_threads(sizeof(T), V > 1, 
     const bool live = RW == 1 || lane_row < stop;
     const float i2 = i2_next[0];
     float i1 = i1_next[0], ir = i2;  // of the rows as they lie in shared memory
-    const bool far = far_row<T>(i1) || (p.pre && far_row<T>(i2));
+    const bool far = !std::is_same_v<T, __half> && (beyond(i1) || (p.pre && beyond(i2)));
     if (far) {
       if (far_row<T>(i1)) {
         if (live) A::scale(buf(stage, 3), A::shift(p.y, p.y_stride, lane_row), left, power_of_two(i1));

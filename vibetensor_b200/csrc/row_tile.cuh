@@ -355,6 +355,7 @@ __device__ __forceinline__ void sum_row(float (&s)[N], float4* red, int& phase, 
       // a lane adds every 32nd warp's part and the lanes fold; all parts one after the other in every thread took
       // the backward of [8192,16384] bf16 458 us, so 428
       t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
       for (int k = lane; k < warps * ranks; k += 32) {
         const float4 f = row[k];
         t.x += f.x; t.y += f.y; t.z += f.z; t.w += f.w;
