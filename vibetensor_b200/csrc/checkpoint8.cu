@@ -12,9 +12,10 @@
 //
 // All are bound by memory: every operand is touched once.  The lanes that hold one group are
 // neighbours, so a group's largest magnitude is a few shuffles and nothing goes through shared memory.
-// [16384,8192] bf16: silu_mul with both copies and its backward from them 350 us = 6.2 TB/s over the two,
-// copy and restore 133 us = 6.1 TB/s; [32768,4096] bf16: RMSNorm with the copy and its backward 283 us
-// = 4.8 TB/s (0.73 of the measured copy bandwidth: 64 registers, two thirds of the issue slots busy).
+// [16384,8192] bf16, calls by themselves: silu_mul with both copies and its backward from them 346 us = 6.3
+// TB/s over the two, silu_mul alone 129 us, its backward from tensors 201, copy and restore 133 us = 6.1 TB/s;
+// [32768,4096] bf16: RMSNorm with the copy and its backward 283 us = 4.8 TB/s (0.73 of the measured copy
+// bandwidth: 64 registers, some spilled in the backward, two thirds of the issue slots busy).
 #include <algorithm>
 
 #include "quant8.cuh"

@@ -7,8 +7,8 @@
 // The two sums stay apart: sum(r^2) expanded in x and v would save a reduction and cancel where the
 // branch nearly undoes the stream.
 //
-// Bound by memory: two rows read, two written.  [32768,4096] bf16 with a gate row per 4096 rows takes
-// 178 us = 6.0 TB/s, 0.92 of the measured copy bandwidth; rows in registers, read when they are
+// Bound by memory: two rows read, two written.  [32768,4096] bf16 with a gate row per 4096 rows takes, a
+// call by itself, 178 us = 6.0 TB/s, 0.92 of the measured copy bandwidth; rows in registers, read when they are
 // needed, took 254 us (93 registers, two blocks per SM, nothing in flight during the reductions).
 #include <algorithm>
 

@@ -13,15 +13,15 @@
 // rounds nothing: r i = (r 2^k) (i 2^-k).  A factor per value instead, i (r i), took up to 8 % longer.
 //
 // Bound by memory and, close behind, by instructions: four rows read, two written, 14 fp32 operations
-// and six conversions per value.  [32768,4096] bf16 with a gate row per 4096 rows takes 300 us = 5.4
-// TB/s, 0.82 of the measured copy bandwidth (16 warps per SM at 128 registers, half of the issue slots
-// busy).  What it came through: rows in registers 678 us; staged by asynchronous copies 370; one base per
-// warp and compile-time offsets instead of an address per access (744 instructions per warp and row
+// and six conversions per value.  [32768,4096] bf16 with a gate row per 4096 rows takes, a call by
+// itself, 300 us = 5.4 TB/s, 0.82 of the measured copy bandwidth (16 warps per SM at 128 registers, half
+// of the issue slots busy).  What it came through: rows in registers 678 us; staged by asynchronous copies
+// 370; one base per warp and compile-time offsets instead of an address per access (744 instructions per warp and row
 // against 964) 314; runs of neighbouring rows rather than every n-th one 306 (379).  Arithmetic on
 // float pairs was slower here (335: moves to pair the registers), and so were one block per SM with
 // four rows in flight (759), eight values per thread (424), and one row in flight (333).
-// Rows shared by two blocks: [8192,16384] bf16 443 us for a floor of 245, 420 without a gate.  Rows that no
-// vector divides: [16384,4095] bf16 250 us for 123, 225 without a gate; their values are single 16-bit loads
+// Rows shared by two blocks: [8192,16384] bf16 440 us for a floor of 245, 415 without a gate.  Rows that no
+// vector divides: [16384,4095] bf16 253 us for 123, 228 without a gate; their values are single 16-bit loads
 // from shared memory and single stores.
 #include <algorithm>
 

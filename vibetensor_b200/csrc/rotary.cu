@@ -7,7 +7,7 @@
 // quarter, so a position of a million keeps every bit of its angle; sine and cosine of what is left
 // are 32-bit.  A block computes the table of its tokens' cosines and sines once in shared memory
 // and turns all the heads it owns with it: the operator moves every value once and is bound by
-// memory.  18432 tokens of 40 heads of 128 bf16: 72 us = 5.3 TB/s, 0.80 of the measured copy
+// memory.  18432 tokens of 40 heads of 128 bf16, among other calls: 72 us = 5.3 TB/s, 0.80 of the measured copy
 // bandwidth (32 registers, full SMs).  With few heads the table is the larger part: 147,456 tokens of
 // five heads take 100 us, 0.58.
 #include <algorithm>

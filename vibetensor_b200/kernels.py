@@ -723,7 +723,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     [axes, ..., tokens], without it [..., tokens]; int64, int32 or float32, dims of size 1
     broadcast.  A pair is (i, pairs + i), or (2i, 2i + 1) with ``interleaved``.  The angle is formed
     in 64 bits: far positions keep it exact.  Returns (q, k) turned, dense, or written to the pair
-    ``out`` (which may be (q, k) itself)."""
+    ``out``, each of which may be its own operand (not the other one)."""
     return _rotary(q, k, positions, inv_freq, sections, interleaved, False, out, "rotary")
 
 
